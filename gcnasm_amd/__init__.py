@@ -11,6 +11,8 @@ Python modules:
   opus_gemm  mirror of the reference's opus_gemm drivers (fp32-scale paths)
   flatmm_splitk  mirror of the reference's a16w16 split-K driver, workspace
              handle and split-K reduce
+  mx4_cache  a key/value cache in MXFP4: append, attention over it, the weights of
+             its tokens, eviction
   ops        tensor-level conveniences (torch tensors as device buffers)
 """
 from ._lib import GaError, lib  # noqa: F401

@@ -171,13 +171,53 @@ class FlatmmSplitkKargs(ctypes.Structure):
           "stride_bias_batch"]]
 
 
+class Mx4Cache(ctypes.Structure):
+    """ga_mx4_cache."""
+
+    _fields_ = [("pages", ctypes.c_void_p), ("num_pages", ctypes.c_longlong),
+                ("stride_page", ctypes.c_longlong), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int)]
+
+
+class Mx4AttentionArgs(ctypes.Structure):
+    """ga_mx4_attention_args."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ["q", "out", "lse", "table", "lens", "q_starts"]
+                ] + [(n, ctypes.c_longlong) for n in
+                     ["stride_q_row", "stride_q_head", "stride_out_row", "stride_out_head",
+                      "stride_lse_row", "stride_table"]
+                     ] + [(n, ctypes.c_int) for n in
+                          ["seqs", "rows", "heads", "table_pages", "max_q", "max_len", "causal",
+                           "window"]
+                          ] + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
+
+
+class Mx4EvictArgs(ctypes.Structure):
+    """ga_mx4_evict_args."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ["table", "lens", "dst_table", "weights", "kept", "new_lens", "new_weights"]
+                ] + [(n, ctypes.c_longlong) for n in
+                     ["stride_table", "stride_dst_table", "stride_w_seq", "stride_w_head",
+                      "stride_new_seq", "stride_new_head"]
+                     ] + [(n, ctypes.c_int) for n in
+                          ["seqs", "table_pages", "dst_pages", "width", "new_width", "keep",
+                           "recent"]]
+
+
 assert ctypes.sizeof(OpusGemmKargs) == 96
 assert ctypes.sizeof(F4gemmKargs) == 0x174
 assert ctypes.sizeof(SplitkWsHandle) == 16
 assert ctypes.sizeof(FlatmmSplitkKargs) == 96
 
+assert ctypes.sizeof(Mx4Cache) == 40
+assert ctypes.sizeof(Mx4AttentionArgs) == 136
+assert ctypes.sizeof(Mx4EvictArgs) == 136
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_ll = ctypes.c_longlong
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
 
@@ -243,6 +283,18 @@ SIGNATURES = {
     "ga_ws_handle_reserve": (_i, [_vp, _sz]),
     "ga_ws_handle_query": (_i, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_sz)]),
     "ga_ws_handle_destroy": (_i, [_vp]),
+    "ga_mx4_page_bytes": (_sz, [_i, _i]),
+    "ga_mx4_append": (_i, [ctypes.POINTER(Mx4Cache), _vp, _vp, _i, _i, _ll, _ll, _ll, _ll, _vp, _i,
+                           _vp]),
+    "ga_mx4_read": (_i, [ctypes.POINTER(Mx4Cache), _vp, _i, _vp, _vp, _i, _vp]),
+    "ga_mx4_attention_workspace_bytes": (_i, [ctypes.POINTER(Mx4Cache),
+                                              ctypes.POINTER(Mx4AttentionArgs),
+                                              ctypes.POINTER(_sz)]),
+    "ga_mx4_attention": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4AttentionArgs), _vp, _sz,
+                              _vp]),
+    "ga_mx4_attention_weights": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4AttentionArgs),
+                                      _vp, _ll, _ll, _vp, _ll, _ll, _i, _vp]),
+    "ga_mx4_evict": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4EvictArgs), _vp]),
     "ga_device_num_cu": (_i, [ctypes.POINTER(_i)]),
 }
 

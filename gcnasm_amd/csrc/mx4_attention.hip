@@ -1,0 +1,910 @@
+// mx4_attention.hip -- attention over the MXFP4 key/value cache, and the weights it gives
+// to the cached tokens (layout and operand order: ga_mx4_cache.hpp).
+//
+// For row i (position len - n + i) of a sequence and the tokens t that it sees:
+//   x_t = scale q.k_t  (or softcap tanh(scale q.k_t / softcap)),  in powers of two:
+//   m = max x_t,  l = sum 2^(x_t - m),  out = sum 2^(x_t - m) v_t / l,  lse = (m + log2 l) ln 2
+// kept as running values over the tokens, so the scores are never stored.
+#include "ga_device.hpp"
+#include "ga_internal.hpp"
+#include "ga_mx4_cache.hpp"
+
+#include <algorithm>
+
+namespace ga {
+
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf16 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnParams {
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;
+    const int *table, *lens, *q_starts;
+    const uint8_t* pages;
+    long long num_pages, stride_page;
+    long long sq_row, sq_head, so_row, so_head, sl_row, s_table;
+    int seqs, rows, heads, kv_heads, group, table_pages, log2p;
+    int causal, window;
+    float to_log2; // scores to powers of two: scale * log2(e), or softcap * log2(e)
+    float to_cap;  // scale / softcap
+    int row_blocks; // workgroups along a sequence's rows; each takes every row_blocks-th block
+    int splits, chunk; // workgroups along the tokens, tokens of each
+    float* ws;         // [splits][rows][heads] {m, l}, then [splits][rows][heads][D]
+};
+
+__host__ __device__ inline size_t stats_floats(int splits, int rows, int heads)
+{
+    return ((size_t)splits * rows * heads * 2 + 3) / 4 * 4;
+}
+
+// A sequence's rows and tokens; whatever the tables hold, inside the operands.
+struct Sequence {
+    int q0, n, len;
+    __device__ __forceinline__ Sequence(const AttnParams& p, int b)
+    {
+        q0 = b;
+        n = 1;
+        if (p.q_starts) {
+            q0 = min(max(p.q_starts[b], 0), p.rows);
+            n = min(max(p.q_starts[b + 1] - q0, 0), p.rows - q0);
+        }
+        const long long cap = (long long)p.table_pages << p.log2p;
+        len = (int)min((long long)max(p.lens[b], 0), min(cap, 0x7FFFFF00ll));
+    }
+};
+
+// Rows r0 .. r0 + count - 1 of a sequence's n * group (row r: query r / group, head
+// r % group) and what they see: tokens in (lo, hi] of each row, and over all.
+struct Block {
+    int r0, count;
+    int hi_min, hi_max, lo_min, lo_max;
+    __device__ __forceinline__ Block(const AttnParams& p, const Sequence& s, int first, int most)
+    {
+        r0 = first;
+        count = min(most, s.n * p.group - first);
+        const int i0 = first / p.group, i1 = (first + count - 1) / p.group;
+        hi_min = p.causal ? min(s.len - s.n + i0, s.len - 1) : s.len - 1;
+        hi_max = p.causal ? min(s.len - s.n + i1, s.len - 1) : s.len - 1;
+        lo_min = p.window ? max(s.len - s.n + i0 - p.window, -1) : -1;
+        lo_max = p.window ? max(s.len - s.n + i1 - p.window, -1) : -1;
+    }
+    // the tokens that some row sees: [begin, end), begin a multiple of 64
+    __device__ __forceinline__ int begin() const { return (lo_min + 1) & ~63; }
+    __device__ __forceinline__ int end() const { return hi_max + 1; }
+};
+
+struct Row {
+    bool real;
+    int head;      // query head
+    long long at;  // row of q and out
+    int hi, lo;    // sees tokens in (lo, hi]
+    __device__ __forceinline__ Row(const AttnParams& p, const Sequence& s, const Block& blk,
+                                   int kv_head, int r)
+    {
+        real = r < blk.count;
+        const int x = real ? blk.r0 + r : blk.r0;
+        const int i = x / p.group;
+        head = kv_head * p.group + (x - i * p.group);
+        at = s.q0 + i;
+        hi = !real ? -1 : (p.causal ? min(s.len - s.n + i, s.len - 1) : s.len - 1);
+        lo = p.window ? s.len - s.n + i - p.window : -1;
+    }
+};
+
+template <bool CAP>
+__device__ __forceinline__ float score_log2(const AttnParams& p, float qk)
+{
+    return CAP ? tanhf(qk * p.to_cap) * p.to_log2 : qk * p.to_log2;
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
+{
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf16));
+}
+
+// A row's D elements as the second operand of D/32 products: lane 16*g + r the
+// elements g*D/4 .. (g+1)*D/4 - 1 of row r.
+template <int D>
+__device__ __forceinline__ void load_q(const AttnParams& p, const Row& row, int g,
+                                       v4i (&q)[D / 32])
+{
+    const uint16_t* src = p.q + row.at * p.sq_row + row.head * p.sq_head + g * (D / 4);
+#pragma unroll
+    for (int m = 0; m < D / 32; m++)
+        q[m] = row.real ? *(const v4i*)(src + 8 * m) : (v4i){0, 0, 0, 0};
+}
+
+// Where 16 tokens lie: their page (clamped into the cache, ok says whether it
+// was in it) and the place of the first in it.
+struct Sixteen {
+    const uint8_t* page;
+    uint32_t t;
+    bool ok;
+};
+template <int D>
+__device__ __forceinline__ Sixteen locate(const AttnParams& p, Mx4Page<D> lay, const int* table,
+                                          int head, int t, int end)
+{
+    const int id = table[min(t, end - 1) >> p.log2p];
+    const bool ok = id >= 0 && id < p.num_pages;
+    return {p.pages + (ok ? id : 0) * p.stride_page + (size_t)head * lay.bytes(),
+            (uint32_t)t & ((1u << p.log2p) - 1u), ok};
+}
+
+// A lane's codes and scales of 16 tokens' keys (row lane % 16), or values.
+template <int D>
+struct KeyCodes {
+    static constexpr int kWords = D / 32;
+    uint32_t w[kWords];
+    uint32_t scale; // D = 256: two bytes, else one
+    __device__ __forceinline__ void load(const Sixteen& s, Mx4Page<D> lay, int lane)
+    {
+        const uint32_t r = lane & 15, g = lane >> 4, t = s.t + r;
+        const uint8_t* src = s.page + lay.k_row(t) + g * (D / 8);
+        if constexpr (D == 64) {
+            const uint2 x = *(const uint2*)src;
+            w[0] = x.x;
+            w[1] = x.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kWords / 4; j++) {
+                const v4i x = *(const v4i*)(src + 16 * j);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    w[4 * j + i] = (uint32_t)x[i];
+            }
+        }
+        const uint8_t* sc = s.page + lay.k_scale(t);
+        if constexpr (D == 256)
+            scale = *(const uint16_t*)(sc + 2 * g);
+        else
+            scale = sc[D == 64 ? g / 2 : g];
+    }
+    // the first operand of product m
+    __device__ __forceinline__ v4i operand(int m) const
+    {
+        return fp4_oct_bf16(w[m], D == 256 && m >= 4 ? e8m0_of<1>(scale) : e8m0_of<0>(scale));
+    }
+};
+
+template <int D>
+struct ValueCodes {
+    static constexpr int kWords = D / 32; // of 4 tokens, D/32 bytes each
+    uint32_t w[kWords];
+    uint32_t scale; // a byte for each of the 4 tokens
+    __device__ __forceinline__ void load(const Sixteen& s, Mx4Page<D> lay, int lane)
+    {
+        const uint32_t i = lane & 15, quad = s.t / 4 + (lane >> 4);
+        const uint8_t* src = s.page + lay.v_quad(quad, i);
+        if constexpr (D == 64) {
+            const uint2 x = *(const uint2*)src;
+            w[0] = x.x;
+            w[1] = x.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kWords / 4; j++) {
+                const v4i x = *(const v4i*)(src + 16 * j);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    w[4 * j + k] = (uint32_t)x[k];
+            }
+        }
+        scale = *(const uint32_t*)(s.page + lay.v_scale(quad, i * (D / 16) / 32));
+    }
+    // byte B (elements 2B and 2B + 1 of the lane's D/16) of the 4 tokens, each a pair of bf16
+    template <int B>
+    __device__ __forceinline__ void pairs(uint32_t (&x)[4]) const
+    {
+        constexpr int kBytes = D / 32; // of a token
+        static_for<4>([&](auto u) {
+            constexpr int at = u * kBytes + B;
+            x[u] = fp4_pair_bf16<at % 4>(w[at / 4], e8m0_of<u>(scale));
+        });
+    }
+};
+
+// The two products' first operands of output elements 2B and 2B + 1: eight
+// tokens of each.
+template <int D, int B>
+__device__ __forceinline__ void value_operands(const ValueCodes<D> (&v)[2], v4i& even, v4i& odd)
+{
+    uint32_t x[2][4];
+    v[0].template pairs<B>(x[0]);
+    v[1].template pairs<B>(x[1]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t a = x[j / 2][j % 2 * 2], b = x[j / 2][j % 2 * 2 + 1];
+        even[j] = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
+        odd[j] = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+}
+
+// Nonzero if one of a dword's four scale bytes is 253 or more: its values may pass bf16
+// (4 * 2^126), or are NaN.
+__device__ __forceinline__ uint32_t any_huge(uint32_t w)
+{
+    return ((w & 0x7F7F7F7Fu) + 0x03030303u) & w & 0x80808080u;
+}
+
+// 32 tokens of one kv head as a wave holds them.
+template <int D>
+struct Tile {
+    KeyCodes<D> k[2];
+    ValueCodes<D> v[2];
+    bool ok[2];
+    __device__ __forceinline__ void load(const AttnParams& p, Mx4Page<D> lay, const int* table,
+                                         int head, int t0, int end, int lane)
+    {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const Sixteen x = locate<D>(p, lay, table, head, t0 + 16 * s, end);
+            k[s].load(x, lay, lane);
+            v[s].load(x, lay, lane);
+            ok[s] = x.ok;
+        }
+    }
+};
+
+// ---- few rows -------------------------------------------------------------------------
+// A wave goes over its tiles of 32 tokens with 16 * RT rows, the next tile's loads in flight: the
+// scores leave the first product as the second one takes its probabilities (a
+// lane: 8 tokens of row lane % 16), so nothing passes through LDS until the waves'
+// results are joined. The tokens are split over the four waves and over
+// p.splits workgroups, whose results mx4_join_kernel joins.
+//
+// The running maximum is raised only when a score passes it by 2^8: until
+// then probabilities up to 2^8 stand in the same sums, which fp32 holds as exactly,
+// and neither the exchange between lanes nor the rescaling is needed.
+//
+// Probabilities enter the second product as two bf16 terms (16 bits of
+// significand together): one alone would add as much error as the output's own
+// rounding to bf16, and the matrix cores wait for memory here anyway.
+constexpr float kRaise = 8.0f;
+
+template <int D, int RT, bool CAP>
+__global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
+{
+    constexpr int NT = D / 16; // output tiles of 16 elements
+    constexpr int kRows = 16 * RT;
+    __shared__ v4f red[2][RT * NT][64];
+    __shared__ float red_m[4][kRows], red_l[4][kRows];
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned unit = blockIdx.x;
+    const int split = unit % p.splits;
+    unit /= p.splits;
+    const int rb = unit % p.row_blocks;
+    unit /= p.row_blocks;
+    const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
+    const Sequence seq(p, b);
+    const Mx4Page<D> lay(1 << p.log2p);
+    const int* table = p.table + b * p.s_table;
+
+    for (int first = rb * kRows; first < seq.n * p.group; first += p.row_blocks * kRows) {
+        const Block blk(p, seq, first, kRows);
+        const int begin = blk.begin() + split * p.chunk;
+        const int end = split == p.splits - 1 ? blk.end() : min(blk.end(), begin + p.chunk);
+        v4i q[RT][D / 32];
+        int hi[RT], lo[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const Row row(p, seq, blk, kv_head, rt * 16 + (lane & 15));
+            load_q<D>(p, row, g, q[rt]);
+            hi[rt] = row.hi;
+            lo[rt] = row.lo;
+        }
+        v4f acc[RT][NT];
+        float m[RT], base[RT], l[RT]; // base: m, or 0 where no score was finite yet
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            m[rt] = -INFINITY;
+            base[rt] = 0.0f;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                acc[rt][j] = (v4f){0, 0, 0, 0};
+        }
+        auto step = [&](Tile<D>& tile, int t0) {
+            v4f s[RT][2];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+                    s[rt][half] = (v4f){0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) {
+                    const v4i a = tile.k[half].operand(i);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+                        s[rt][half] = mfma_bf16_16x16x32(a, q[rt][i], s[rt][half]);
+                }
+            }
+            const bool whole = t0 > blk.lo_max && t0 + 31 <= blk.hi_min && tile.ok[0] && tile.ok[1];
+            float x[RT][8];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    x[rt][j] = score_log2<CAP>(p, s[rt][j / 4][j % 4]);
+            if (!whole) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    uint32_t keep = 0;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int t = t0 + 16 * half + 4 * g + u;
+                        const bool seen = tile.ok[half] && t <= blk.hi_max && t > blk.lo_min;
+                        keep |= seen ? 0xFFu << (8 * u) : 0u;
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+                            if (!tile.ok[half] || t > hi[rt] || t <= lo[rt])
+                                x[rt][4 * half + u] = -INFINITY;
+                    }
+                    // hidden from every row: a scale that makes finite values, times 0
+                    tile.v[half].scale &= keep;
+                }
+            }
+            const bool huge = __builtin_amdgcn_ballot_w64(any_huge(tile.v[0].scale) |
+                                                          any_huge(tile.v[1].scale)) != 0;
+            bool raise = false;
+            float top[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                top[rt] = x[rt][0];
+#pragma unroll
+                for (int j = 1; j < 8; j++)
+                    top[rt] = fmaxf(top[rt], x[rt][j]);
+                raise |= top[rt] > m[rt] + kRaise;
+            }
+            if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    float t = fmaxf(top[rt], m[rt]);
+                    t = fmaxf(t, __shfl_xor(t, 16, 64));
+                    t = fmaxf(t, __shfl_xor(t, 32, 64));
+                    const float f = m[rt] == -INFINITY ? 0.0f : exp2_of(m[rt] - t);
+                    m[rt] = t;
+                    base[rt] = t == -INFINITY ? 0.0f : t;
+                    l[rt] *= f;
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            acc[rt][j][r] *= f;
+                }
+            }
+            v4i ph[RT], pl[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    x[rt][j] = exp2_of(x[rt][j] - base[rt]);
+                    l[rt] += x[rt][j];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t h = pack_bf16(x[rt][2 * j], x[rt][2 * j + 1]);
+                    ph[rt][j] = (int)h;
+                    pl[rt][j] = (int)pack_bf16(x[rt][2 * j] - __uint_as_float(h << 16),
+                                               x[rt][2 * j + 1] - __uint_as_float(h & 0xFFFF0000u));
+                }
+            }
+            if (huge) {
+                // infinite values: 0 * infinity would reach rows that do not see the
+                // token, and the second term's sign undo it. One token at a time, each
+                // row only what it sees
+                float* px = (float*)red + wave * (2 * RT * NT * 64); // this wave's share
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        px[(rt * 8 + j) * 64 + lane] = x[rt][j];
+                for (int t = 0; t < 32; t++) {
+                    const Sixteen at = locate<D>(p, lay, table, kv_head, t0 + (t & 16), end);
+                    const uint32_t in = at.t + (t & 15);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        if (!at.ok || t0 + t > hi[rt] || t0 + t <= lo[rt])
+                            continue;
+                        const float w = px[(rt * 8 + (t >> 4) * 4 + (t & 3)) * 64 +
+                                           (t >> 2 & 3) * 16 + (lane & 15)];
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+#pragma unroll
+                            for (int j = 0; j < NT; j++) {
+                                const uint32_t i = 4 * g + r;
+                                const uint8_t code =
+                                    at.page[lay.v_quad(in / 4, i) + in % 4 * (D / 32) + j / 2];
+                                const uint8_t sc =
+                                    at.page[lay.v_scale(in / 4, i * NT / 32) + in % 4];
+                                acc[rt][j][r] =
+                                    fmaf(w, fp4_value(code >> (j % 2 * 4) & 15u, sc), acc[rt][j][r]);
+                            }
+                    }
+                }
+            } else {
+                static_for<D / 32>([&](auto byte) {
+                    constexpr int B = decltype(byte)::value;
+                    v4i even, odd;
+                    value_operands<D, B>(tile.v, even, odd);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        acc[rt][2 * B] = mfma_bf16_16x16x32(even, ph[rt], acc[rt][2 * B]);
+                        acc[rt][2 * B + 1] = mfma_bf16_16x16x32(odd, ph[rt], acc[rt][2 * B + 1]);
+                        acc[rt][2 * B] = mfma_bf16_16x16x32(even, pl[rt], acc[rt][2 * B]);
+                        acc[rt][2 * B + 1] = mfma_bf16_16x16x32(odd, pl[rt], acc[rt][2 * B + 1]);
+                    }
+                });
+            }
+        };
+        int t0 = begin + 32 * wave;
+        if (t0 < end) {
+            Tile<D> cur;
+            cur.load(p, lay, table, kv_head, t0, end, lane);
+            while (true) {
+                const int next = t0 + 128;
+                if (next >= end)
+                    break;
+                Tile<D> ahead;
+                ahead.load(p, lay, table, kv_head, next, end, lane);
+                step(cur, t0);
+                cur = ahead;
+                t0 = next;
+            }
+            step(cur, t0);
+        }
+
+        // join the four waves: a common maximum, then the sums pairwise
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            l[rt] += __shfl_xor(l[rt], 16, 64);
+            l[rt] += __shfl_xor(l[rt], 32, 64);
+            if (g == 0) {
+                red_m[wave][rt * 16 + lane] = m[rt];
+                red_l[wave][rt * 16 + lane] = l[rt];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const int r = rt * 16 + (lane & 15);
+            float top = red_m[0][r];
+#pragma unroll
+            for (int w = 1; w < 4; w++)
+                top = fmaxf(top, red_m[w][r]);
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                sum += red_m[w][r] == -INFINITY ? red_l[w][r]
+                                                : red_l[w][r] * exp2_of(red_m[w][r] - top);
+            const float f = m[rt] == -INFINITY ? 1.0f : exp2_of(m[rt] - top);
+            m[rt] = top;
+            l[rt] = sum;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    acc[rt][j][k] *= f;
+        }
+        for (int half = 2; half >= 1; half /= 2) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        red[wave - half][rt * NT + j][lane] = acc[rt][j];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        const v4f o = red[wave][rt * NT + j][lane];
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            acc[rt][j][k] += o[k];
+                    }
+            }
+            __syncthreads();
+        }
+        if (wave != 0)
+            continue;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const Row row(p, seq, blk, kv_head, rt * 16 + (lane & 15));
+            if (!row.real)
+                continue;
+            if (p.splits == 1) {
+                const float inv = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
+                uint16_t* out = p.out + row.at * p.so_row + row.head * p.so_head;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t o[NT / 2];
+#pragma unroll
+                    for (int j = 0; j < NT / 2; j++)
+                        o[j] = pack_bf16(acc[rt][2 * j][k] * inv, acc[rt][2 * j + 1][k] * inv);
+                    uint32_t* dst = (uint32_t*)(out + (4 * g + k) * NT);
+#pragma unroll
+                    for (int j = 0; j < NT / 2; j += 2)
+                        *(uint2*)(dst + j) = make_uint2(o[j], o[j + 1]);
+                }
+                if (p.lse && g == 0)
+                    p.lse[row.at * p.sl_row + row.head] = (m[rt] + __log2f(l[rt])) * kLn2;
+            } else {
+                const size_t at = ((size_t)split * p.rows + row.at) * p.heads + row.head;
+                if (g == 0)
+                    *(float2*)(p.ws + at * 2) = make_float2(m[rt], l[rt]);
+                if (m[rt] == -INFINITY && l[rt] == 0.0f)
+                    continue; // nothing seen: the sums are not read
+                float* dst = p.ws + stats_floats(p.splits, p.rows, p.heads) + at * D;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int j = 0; j < NT; j += 4)
+                        *(v4f*)(dst + (4 * g + k) * NT + j) =
+                            (v4f){acc[rt][j][k], acc[rt][j + 1][k], acc[rt][j + 2][k],
+                                  acc[rt][j + 3][k]};
+            }
+        }
+    }
+}
+
+// The splits of a row joined, one wave a row: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s,
+// in the order of the splits. Bound by its launch and by reading the partial sums.
+template <int D>
+__global__ __launch_bounds__(256) void mx4_join_kernel(AttnParams p)
+{
+    constexpr int E = D / 64; // elements of a lane
+    const int lane = threadIdx.x & 63;
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= (long long)p.rows * p.heads)
+        return;
+    const long long row = unit / p.heads;
+    const int head = (int)(unit - row * p.heads);
+    const size_t step = (size_t)p.rows * p.heads;
+    const float2* stats = (const float2*)p.ws + unit;
+    const float* part = p.ws + stats_floats(p.splits, p.rows, p.heads) + unit * D + lane * E;
+    float top = -INFINITY;
+    for (int s = lane; s < p.splits; s += 64)
+        top = fmaxf(top, stats[s * step].x);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+    float acc[E] = {}, sum = 0.0f;
+    for (int s = 0; s < p.splits; s++) {
+        const float2 ml = stats[s * step];
+        if (ml.x == -INFINITY && ml.y == 0.0f)
+            continue;
+        const float f = ml.x == -INFINITY ? 1.0f : exp2_of(ml.x - top);
+        sum += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            acc[e] += part[s * step * D + e] * f;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* out = p.out + row * p.so_row + head * p.so_head + lane * E;
+    if constexpr (E == 1) {
+        out[0] = f32_to_bf16(acc[0] * inv);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+            *(uint32_t*)(out + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+    }
+    if (p.lse && lane == 0)
+        p.lse[row * p.sl_row + head] = (top + __log2f(sum)) * kLn2;
+}
+
+// ---- the weights of the tokens ------------------------------------------------------------
+// A wave holds 32 tokens' keys as operands and goes over the rows that see them, 16 at a time;
+// a lane adds up the probabilities of 8 tokens over its rows (lane % 16 of
+// each 16), and the 16 lanes are added once at the end: no atomics, a fixed order.
+// Few rows: bound by reading the keys; prompts: by the exponentials.
+template <int D, bool CAP>
+__global__ __launch_bounds__(256) void mx4_weights_kernel(AttnParams p, const float* w_in,
+                                                          long long si_seq, long long si_head,
+                                                          float* w_out, long long so_seq,
+                                                          long long so_head, int width,
+                                                          int blocks)
+{
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned unit = blockIdx.x;
+    const int t0 = (int)(unit % blocks) * 128 + 32 * wave;
+    unit /= blocks;
+    const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
+    const Sequence seq(p, b);
+    if (t0 >= width)
+        return;
+    float sum[8] = {};
+    const int rows = seq.n * p.group;
+    if (t0 < seq.len) {
+        const Mx4Page<D> lay(1 << p.log2p);
+        KeyCodes<D> k[2];
+        bool ok[2];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const Sixteen x =
+                locate<D>(p, lay, p.table + b * p.s_table, kv_head, t0 + 16 * s, seq.len);
+            k[s].load(x, lay, lane);
+            ok[s] = x.ok;
+        }
+        v4i kop[2][D / 32];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < D / 32; i++)
+                kop[s][i] = k[s].operand(i);
+        // the rows that see some of the tokens: positions t0 .. t0 + 31 + window - 1
+        const int pos0 = seq.len - seq.n;
+        const int i0 = p.causal ? max(t0 - pos0, 0) : 0;
+        const long long last = p.window ? (long long)t0 + 31 + p.window - 1 - pos0 : seq.n - 1;
+        const int r_end = (int)min((long long)rows, (min(last, (long long)seq.n) + 1) * p.group);
+        for (int r = i0 * p.group; r < r_end; r += 16) {
+            const Block blk(p, seq, r, 16);
+            const Row row(p, seq, blk, kv_head, lane & 15);
+            v4i q[D / 32];
+            load_q<D>(p, row, g, q);
+            const float lse2 = row.real ? p.lse[row.at * p.sl_row + row.head] * kLog2e : 0.0f;
+            const bool whole = t0 > blk.lo_max && t0 + 31 <= blk.hi_min && ok[0] && ok[1] &&
+                               blk.count == 16;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                v4f s = (v4f){0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < D / 32; i++)
+                    s = mfma_bf16_16x16x32(kop[half][i], q[i], s);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int t = t0 + 16 * half + 4 * g + u;
+                    const float w = exp2_of(score_log2<CAP>(p, s[u]) - lse2);
+                    if (whole || (ok[half] && t <= row.hi && t > row.lo))
+                        sum[4 * half + u] += w;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1)
+            sum[j] += __shfl_xor(sum[j], o, 64);
+    // lane 16*g + j (j < 8) stores token 16 * (j / 4) + 4 * g + j % 4
+    const int j = lane & 15;
+    float x = sum[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++)
+        x = j == i ? sum[i] : x;
+    const int t = t0 + 16 * (j / 4) + 4 * g + j % 4;
+    if (j < 8 && t < width) {
+        const float old =
+            w_in && t < seq.len ? w_in[b * si_seq + kv_head * si_head + t] : 0.0f;
+        w_out[b * so_seq + kv_head * so_head + t] = t < seq.len ? old + x : 0.0f;
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------
+ga_status mx4_cache_check(const ga_mx4_cache* c);
+
+static ga_status attention_check(const ga_mx4_cache* c, const ga_mx4_attention_args* a,
+                                 bool pointers)
+{
+    if (const ga_status st = mx4_cache_check(c))
+        return st;
+    if (!a)
+        return fail(GA_ERR_ARG, "mx4 attention: null arguments");
+    if (a->seqs < 0 || a->rows < 0 || a->table_pages < 0 || a->max_q < 0 || a->max_len < 0 ||
+        a->heads <= 0 || a->window < 0 || !(a->softcap >= 0.0f))
+        return fail(GA_ERR_ARG, "mx4 attention: negative size, window or softcap");
+    if (a->heads % c->kv_heads)
+        return fail(GA_ERR_SHAPE, "mx4 attention: %d heads over %d kv heads", a->heads, c->kv_heads);
+    if (a->window > 0 && !a->causal)
+        return fail(GA_ERR_ARG, "mx4 attention: a window needs causal rows");
+    if (!a->q_starts && a->rows != a->seqs)
+        return fail(GA_ERR_SHAPE, "mx4 attention: %d rows of %d sequences need q_starts", a->rows,
+                    a->seqs);
+    if ((long long)a->rows * a->heads > 0x7FFFFFFFll)
+        return fail(GA_ERR_SHAPE, "mx4 attention: too many rows for one call");
+    if (!pointers || a->seqs == 0 || a->rows == 0)
+        return GA_OK;
+    if (!a->q || !a->lens || (!a->table && a->table_pages))
+        return fail(GA_ERR_ARG, "mx4 attention: null pointer");
+    if ((uintptr_t)a->q % 16 || a->stride_q_row % 8 || a->stride_q_head % 8)
+        return fail(GA_ERR_SHAPE, "mx4 attention: q must be 16-byte aligned with strides that are "
+                                  "multiples of 8");
+    return GA_OK;
+}
+
+static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& a)
+{
+    AttnParams p{};
+    p.q = (const uint16_t*)a.q;
+    p.out = (uint16_t*)a.out;
+    p.lse = a.lse;
+    p.table = a.table;
+    p.lens = a.lens;
+    p.q_starts = a.q_starts;
+    p.pages = (const uint8_t*)c.pages;
+    p.num_pages = c.num_pages;
+    p.stride_page = c.stride_page;
+    p.sq_row = a.stride_q_row;
+    p.sq_head = a.stride_q_head;
+    p.so_row = a.stride_out_row;
+    p.so_head = a.stride_out_head;
+    p.sl_row = a.stride_lse_row;
+    p.s_table = a.stride_table;
+    p.seqs = a.seqs;
+    p.rows = a.rows;
+    p.heads = a.heads;
+    p.kv_heads = c.kv_heads;
+    p.group = a.heads / c.kv_heads;
+    p.table_pages = a.table_pages;
+    p.log2p = __builtin_ctz((unsigned)c.page_size);
+    p.causal = a.causal != 0;
+    p.window = a.window;
+    p.to_log2 = (a.softcap > 0.0f ? a.softcap : a.scale) * kLog2e;
+    p.to_cap = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+    return p;
+}
+
+// How a call is cut. Row blocks of 16 rows while a sequence has no more, else of
+// 32 (D = 256: always 16, two blocks' sums do not fit the registers); tokens in chunks of a multiple of 128 (a tile for each of the four waves), as
+// many as give every CU a few workgroups.
+struct RowsPlan {
+    int tiles; // of 16 rows
+    int row_blocks, splits, chunk;
+    size_t ws_floats;
+};
+
+static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a, int num_cu)
+{
+    RowsPlan r{};
+    const int group = a.heads / c.kv_heads;
+    const long long max_q = a.q_starts ? std::min<long long>(std::max(a.max_q, 1), a.rows) : 1;
+    const long long rows = max_q * group;
+    r.tiles = rows <= 16 || c.head_dim == 256 ? 1 : 2;
+    r.row_blocks = (int)((rows + 16 * r.tiles - 1) / (16 * r.tiles));
+    long long span = std::min<long long>(a.max_len, (long long)a.table_pages * c.page_size);
+    if (a.window > 0) // a row block's rows and the alignment of its first token
+        span = std::min<long long>(span, (long long)a.window + 16 * r.tiles / group + 64);
+    span = std::max<long long>(span, 1);
+    const long long units = (long long)a.seqs * c.kv_heads * r.row_blocks;
+    const long long want = std::max<long long>(1, 4ll * num_cu / units);
+    r.chunk = (int)(((span + want - 1) / want + 127) / 128 * 128);
+    r.splits = (int)((span + r.chunk - 1) / r.chunk);
+    if (r.splits > 1)
+        r.ws_floats = stats_floats(r.splits, a.rows, a.heads) +
+                      (size_t)r.splits * a.rows * a.heads * c.head_dim;
+    return r;
+}
+
+template <int D, bool CAP>
+static void launch_rows(const AttnParams& p, const RowsPlan& r, unsigned grid, hipStream_t s)
+{
+    if constexpr (D < 256) {
+        if (r.tiles == 2) {
+            hipLaunchKernelGGL((mx4_rows_kernel<D, 2, CAP>), dim3(grid), dim3(256), 0, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((mx4_rows_kernel<D, 1, CAP>), dim3(grid), dim3(256), 0, s, p);
+}
+
+// f(std::integral_constant<int, D>, std::bool_constant<capped>)
+template <class F>
+static void with_dim_cap(int d, bool cap, F&& f)
+{
+    auto with = [&](auto dim) {
+        if (cap)
+            f(dim, std::true_type{});
+        else
+            f(dim, std::false_type{});
+    };
+    if (d == 64)
+        with(std::integral_constant<int, 64>{});
+    else if (d == 128)
+        with(std::integral_constant<int, 128>{});
+    else
+        with(std::integral_constant<int, 256>{});
+}
+
+} // namespace ga
+
+using namespace ga;
+
+extern "C" {
+
+ga_status ga_mx4_attention_workspace_bytes(const ga_mx4_cache* cache,
+                                           const ga_mx4_attention_args* args, size_t* bytes)
+{
+    if (!bytes)
+        return fail(GA_ERR_ARG, "mx4 attention: null pointer");
+    if (const ga_status st = attention_check(cache, args, false))
+        return st;
+    *bytes = 0;
+    if (args->seqs == 0 || args->rows == 0)
+        return GA_OK;
+    int num_cu = 0;
+    if (const ga_status st = device_cu_count(&num_cu))
+        return st;
+    *bytes = rows_plan(*cache, *args, num_cu).ws_floats * 4;
+    return GA_OK;
+}
+
+ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_args* args,
+                           void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (const ga_status st = attention_check(cache, args, true))
+        return st;
+    const ga_mx4_attention_args& a = *args;
+    if (a.seqs == 0 || a.rows == 0)
+        return GA_OK;
+    if (!a.out || (uintptr_t)a.out % 16 || a.stride_out_row % 8 || a.stride_out_head % 8)
+        return fail(GA_ERR_SHAPE, "mx4 attention: out must be 16-byte aligned with strides that are "
+                                  "multiples of 8");
+    int num_cu = 0;
+    if (const ga_status st = device_cu_count(&num_cu))
+        return st;
+    const RowsPlan r = rows_plan(*cache, a, num_cu);
+    if (r.ws_floats && (!workspace || workspace_bytes < r.ws_floats * 4))
+        return fail(GA_ERR_WORKSPACE, "mx4 attention: workspace holds %zu bytes, need %zu",
+                    workspace ? workspace_bytes : (size_t)0, r.ws_floats * 4);
+    if ((uintptr_t)workspace % 16)
+        return fail(GA_ERR_ARG, "mx4 attention: workspace must be 16-byte aligned");
+    const long long grid = (long long)a.seqs * cache->kv_heads * r.row_blocks * r.splits;
+    if (grid > 0x7FFFFFFFll)
+        return fail(GA_ERR_SHAPE, "mx4 attention: too many rows for one call");
+    AttnParams p = params_of(*cache, a);
+    p.row_blocks = r.row_blocks;
+    p.splits = r.splits;
+    p.chunk = r.chunk;
+    p.ws = (float*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    with_dim_cap(cache->head_dim, a.softcap > 0.0f, [&](auto dim, auto cap) {
+        constexpr int D = decltype(dim)::value;
+        launch_rows<D, decltype(cap)::value>(p, r, (unsigned)grid, st);
+        if (r.splits > 1)
+            hipLaunchKernelGGL((mx4_join_kernel<D>),
+                               dim3((unsigned)(((long long)a.rows * a.heads + 3) / 4)), dim3(256), 0,
+                               st, p);
+    });
+    GA_HIP_CHECK(hipGetLastError());
+    return GA_OK;
+}
+
+ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_attention_args* args,
+                                   const float* w_in, long long stride_in_seq,
+                                   long long stride_in_head, float* w_out,
+                                   long long stride_out_seq, long long stride_out_head, int width,
+                                   void* stream)
+{
+    if (const ga_status st = attention_check(cache, args, true))
+        return st;
+    const ga_mx4_attention_args& a = *args;
+    if (width < 0)
+        return fail(GA_ERR_ARG, "mx4 attention weights: negative width");
+    if (a.seqs == 0 || width == 0)
+        return GA_OK;
+    if (!w_out || !a.lens || (a.rows && !a.lse))
+        return fail(GA_ERR_ARG, "mx4 attention weights: null pointer");
+    const long long blocks = ((long long)width + 127) / 128;
+    const long long grid = (long long)a.seqs * cache->kv_heads * blocks;
+    if (grid > 0x7FFFFFFFll)
+        return fail(GA_ERR_SHAPE, "mx4 attention weights: too many sequences for one call");
+    const AttnParams p = params_of(*cache, a);
+    with_dim_cap(cache->head_dim, a.softcap > 0.0f, [&](auto dim, auto cap) {
+        hipLaunchKernelGGL((mx4_weights_kernel<decltype(dim)::value, decltype(cap)::value>),
+                           dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, p, w_in,
+                           stride_in_seq, stride_in_head, w_out, stride_out_seq, stride_out_head,
+                           width, (int)blocks);
+    });
+    GA_HIP_CHECK(hipGetLastError());
+    return GA_OK;
+}
+
+} // extern "C"

@@ -1,0 +1,553 @@
+// mx4_cache.hip -- writing, reading back and thinning out the MXFP4 key/value cache
+// (layout: ga_mx4_cache.hpp).
+#include "ga_device.hpp"
+#include "ga_internal.hpp"
+#include "ga_mx4_cache.hpp"
+#include "ga_quant.hpp"
+
+namespace ga {
+
+struct CacheView {
+    uint8_t* pages;
+    long long num_pages, stride_page;
+    int heads, log2p;
+
+    __device__ __forceinline__ int page_size() const { return 1 << log2p; }
+    // one head's page; in_cache() has to hold
+    __device__ __forceinline__ uint8_t* page(long long id, int head, uint32_t bytes) const
+    {
+        return pages + id * stride_page + (size_t)head * bytes;
+    }
+    __device__ __forceinline__ bool in_cache(long long id) const
+    {
+        return id >= 0 && id < num_pages;
+    }
+};
+
+static CacheView view_of(const ga_mx4_cache& c)
+{
+    return {(uint8_t*)c.pages, c.num_pages, c.stride_page, c.kv_heads,
+            __builtin_ctz((unsigned)c.page_size)};
+}
+
+// ---- append -----------------------------------------------------------------------
+// A lane quantises EPL elements of a token's key and the same ones of its value,
+// 32 / EPL lanes a block: both loads are in flight before the first maximum is
+// taken. Bound by bytes: the input once, 17/32 of a byte per element out.
+template <int D, int EPL>
+__device__ __forceinline__ void store_value_codes(uint8_t* page, Mx4Page<D> lay, uint32_t t,
+                                                  uint32_t d, uint32_t w)
+{
+    constexpr uint32_t kPer = D / 16; // elements of one i
+    const uint32_t u = t % 4 * (D / 32);
+    if constexpr (EPL == 8 && D == 64) { // two i's of 4 elements
+        *(uint16_t*)(page + lay.v_quad(t / 4, d / kPer) + u) = (uint16_t)w;
+        *(uint16_t*)(page + lay.v_quad(t / 4, d / kPer + 1) + u) = (uint16_t)(w >> 16);
+    } else {
+        uint8_t* dst = page + lay.v_quad(t / 4, d / kPer) + u + d % kPer / 2;
+        if constexpr (EPL == 8)
+            *(uint32_t*)dst = w;
+        else
+            *(uint16_t*)dst = (uint16_t)w;
+    }
+}
+
+template <int EPL, bool NAN_RULE>
+__device__ __forceinline__ uint32_t scaled_codes(const float (&v)[EPL], int e)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; j += 4)
+        w |= e2m1_encode4<NAN_RULE>(ldexpf(v[j], -e), ldexpf(v[j + 1], -e), ldexpf(v[j + 2], -e),
+                                    ldexpf(v[j + 3], -e))
+             << (4 * j);
+    return w;
+}
+
+template <int IN, int EPL, int D>
+__global__ __launch_bounds__(256) void mx4_append_kernel(
+    CacheView c, const void* __restrict__ k, const void* __restrict__ v, int tokens,
+    long long sk_row, long long sk_head, long long sv_row, long long sv_head,
+    const long long* __restrict__ slots, int rule)
+{
+    constexpr int LPB = 32 / EPL, LPR = D / EPL; // lanes per block, per row
+    const long long lane = (long long)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t row = (uint32_t)(lane / LPR);
+    const uint32_t d = (uint32_t)(lane % LPR) * EPL;
+    const uint32_t tok = row / (uint32_t)c.heads;
+    const int head = (int)(row - tok * (uint32_t)c.heads);
+    const bool real = tok < (uint32_t)tokens;
+    Raw<IN, EPL> rk, rv;
+    rk.load(k, (size_t)(tok * sk_row + head * sk_head + d), real);
+    rv.load(v, (size_t)(tok * sv_row + head * sv_head + d), real);
+    const long long slot = real ? slots[tok] : -1;
+    const MxScaleRule scale(2, rule);
+    float vk[EPL], vv[EPL];
+    rk.unpack(real, vk);
+    rv.unpack(real, vv);
+    bool nan_k, nan_v;
+    const int ek = scale.exp(block_amax<LPB, EPL>(vk, nan_k));
+    const int ev = scale.exp(block_amax<LPB, EPL>(vv, nan_v));
+    const long long id = slot >> c.log2p;
+    if (!real || !c.in_cache(id))
+        return;
+    const Mx4Page<D> lay(c.page_size());
+    uint8_t* page = c.page(id, head, lay.bytes());
+    const uint32_t t = (uint32_t)slot & (uint32_t)(c.page_size() - 1);
+    const uint32_t wk = nan_k ? scaled_codes<EPL, true>(vk, ek) : scaled_codes<EPL, false>(vk, ek);
+    const uint32_t wv = nan_v ? scaled_codes<EPL, true>(vv, ev) : scaled_codes<EPL, false>(vv, ev);
+    if constexpr (EPL == 8)
+        *(uint32_t*)(page + lay.k_row(t) + d / 2) = wk;
+    else
+        *(uint16_t*)(page + lay.k_row(t) + d / 2) = (uint16_t)wk;
+    store_value_codes<D, EPL>(page, lay, t, d, wv);
+    if (d % 32 == 0) {
+        page[lay.k_scale(t) + d / 32] = (uint8_t)(ek + 127);
+        page[lay.v_scale(t / 4, d / 32) + t % 4] = (uint8_t)(ev + 127);
+    }
+}
+
+// ---- read back ---------------------------------------------------------------------
+// Eight elements of a token's key and value per lane; bound by the bytes written.
+template <int D>
+__device__ __forceinline__ uint32_t value_codes8(const uint8_t* page, Mx4Page<D> lay, uint32_t t,
+                                                 uint32_t d)
+{
+    constexpr uint32_t kPer = D / 16;
+    const uint32_t u = t % 4 * (D / 32);
+    if constexpr (D == 64)
+        return *(const uint16_t*)(page + lay.v_quad(t / 4, d / kPer) + u) |
+               (uint32_t) * (const uint16_t*)(page + lay.v_quad(t / 4, d / kPer + 1) + u) << 16;
+    else
+        return *(const uint32_t*)(page + lay.v_quad(t / 4, d / kPer) + u + d % kPer / 2);
+}
+
+template <int OUT>
+__device__ __forceinline__ void store_values8(void* dst, size_t at, uint32_t w, uint32_t scale)
+{
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        x[j] = fp4_value(w >> (4 * j) & 15u, scale);
+    if constexpr (OUT == GA_DTYPE_BF16) {
+        v4i o;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] = (int)(f32_to_bf16(x[2 * j]) | (uint32_t)f32_to_bf16(x[2 * j + 1]) << 16);
+        *(v4i*)((uint16_t*)dst + at) = o;
+    } else {
+        *(v4f*)((float*)dst + at) = (v4f){x[0], x[1], x[2], x[3]};
+        *(v4f*)((float*)dst + at + 4) = (v4f){x[4], x[5], x[6], x[7]};
+    }
+}
+
+template <int OUT, int D>
+__global__ __launch_bounds__(256) void mx4_read_kernel(CacheView c,
+                                                       const long long* __restrict__ slots,
+                                                       int tokens, void* __restrict__ k,
+                                                       void* __restrict__ v)
+{
+    const long long lane = (long long)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t row = (uint32_t)(lane / (D / 8));
+    const uint32_t d = (uint32_t)(lane % (D / 8)) * 8;
+    const uint32_t tok = row / (uint32_t)c.heads;
+    if (tok >= (uint32_t)tokens)
+        return;
+    const int head = (int)(row - tok * (uint32_t)c.heads);
+    const long long slot = slots[tok], id = slot >> c.log2p;
+    const Mx4Page<D> lay(c.page_size());
+    uint32_t wk = 0, wv = 0, sk = 0, sv = 0;
+    if (c.in_cache(id)) {
+        const uint8_t* page = c.page(id, head, lay.bytes());
+        const uint32_t t = (uint32_t)slot & (uint32_t)(c.page_size() - 1);
+        wk = *(const uint32_t*)(page + lay.k_row(t) + d / 2);
+        wv = value_codes8<D>(page, lay, t, d);
+        sk = page[lay.k_scale(t) + d / 32];
+        sv = page[lay.v_scale(t / 4, d / 32) + t % 4];
+    }
+    const size_t at = (size_t)row * D + d;
+    store_values8<OUT>(k, at, wk, sk);
+    store_values8<OUT>(v, at, wv, sv);
+}
+
+// ---- eviction: which tokens stay --------------------------------------------------------
+struct EvictArgs {
+    ga_mx4_evict_args a;
+    CacheView c;
+};
+
+__device__ __forceinline__ int evict_length(const EvictArgs& e, int b)
+{
+    const long long cap = min((long long)e.a.table_pages << e.c.log2p, (long long)e.a.width);
+    return (int)min((long long)max(e.a.lens[b], 0), cap);
+}
+
+// Order of weights as unsigned integers: larger weight, larger key; both zeros
+// alike, every NaN above everything.
+__device__ __forceinline__ uint32_t weight_key(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u)
+        return 0xFFFFFFFFu;
+    if ((u & 0x7FFFFFFFu) == 0)
+        return 0x80000000u;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
+
+// One workgroup per sequence and kv head. The (keep - recent)-th largest key is
+// found by its digits (11, 11 and 10 bits, a histogram each), then every wave
+// goes over a stretch of the weights twice: once to count what is above
+// the key and equal to it, once to write the indices at the place that the
+// stretches before it leave. No atomics on anything but the histograms' counts,
+// so the result does not depend on an order. Five passes over weights that the first
+// one brings into the L2.
+__global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
+{
+    __shared__ int hist[kSelBins];
+    __shared__ int wave_sum[kSelWaves], wave_gt[kSelWaves], wave_eq[kSelWaves];
+    __shared__ int found_bin, found_left;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = blockIdx.x / e.c.heads, head = blockIdx.x - b * e.c.heads;
+    const int len = evict_length(e, b), keep = e.a.keep;
+    const float* w = e.a.weights + b * e.a.stride_w_seq + head * e.a.stride_w_head;
+    int* kept = e.a.kept + (size_t)blockIdx.x * keep;
+    float* nw = e.a.new_weights + b * e.a.stride_new_seq + head * e.a.stride_new_head;
+    const int new_len = min(len, keep);
+    if (head == 0 && tid == 0)
+        e.a.new_lens[b] = new_len;
+    for (int j = new_len + tid; j < keep; j += kSelThreads)
+        kept[j] = -1;
+    for (int j = new_len + tid; j < e.a.new_width; j += kSelThreads)
+        nw[j] = 0.0f;
+    if (len <= keep) {
+        for (int j = tid; j < len; j += kSelThreads) {
+            kept[j] = j;
+            nw[j] = w[j];
+        }
+        return;
+    }
+    const int old = len - e.a.recent, want = keep - e.a.recent; // old > want
+    for (int j = tid; j < e.a.recent; j += kSelThreads) {
+        kept[want + j] = old + j;
+        nw[want + j] = w[old + j];
+    }
+    if (want == 0)
+        return;
+    uint32_t key_at = 0;
+    int left = want; // of the keys that share key_at's digits so far
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+        const int bits = pass == 2 ? 10 : 11;
+        const uint32_t fixed = pass == 0 ? 0u : ~0u << (shift + bits);
+        for (int j = tid; j < kSelBins; j += kSelThreads)
+            hist[j] = 0;
+        __syncthreads();
+        for (int j = tid; j < old; j += kSelThreads) {
+            const uint32_t key = weight_key(w[j]);
+            if (((key ^ key_at) & fixed) == 0)
+                atomicAdd(&hist[key >> shift & ((1u << bits) - 1u)], 1);
+        }
+        __syncthreads();
+        // thread i holds bins hi = 2047 - 2i and hi - 1: keys above come first
+        const int hi = kSelBins - 1 - 2 * tid;
+        const int n1 = hist[hi], n0 = hist[hi - 1];
+        int sum = n1 + n0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(sum, o, 64);
+            sum += lane >= o ? t : 0;
+        }
+        if (lane == 63)
+            wave_sum[wave] = sum;
+        __syncthreads();
+        int before = sum - n1 - n0; // keys in bins above hi
+        for (int i = 0; i < wave; i++)
+            before += wave_sum[i];
+        if (before < left && left <= before + n1 + n0) {
+            const bool upper = left <= before + n1;
+            found_bin = upper ? hi : hi - 1;
+            found_left = left - (upper ? before : before + n1);
+        }
+        __syncthreads();
+        key_at |= (uint32_t)found_bin << shift;
+        left = found_left;
+    }
+    // each wave's stretch of the tokens
+    const int per = (old + kSelThreads - 1) / kSelThreads * 64;
+    const int lo = min(old, wave * per), hi = min(old, lo + per);
+    int gt = 0, eq = 0;
+    for (int j = lo; j < hi; j += 64) {
+        const uint32_t key = j + lane < hi ? weight_key(w[j + lane]) : 0u;
+        const bool in = j + lane < hi;
+        gt += __popcll(__builtin_amdgcn_ballot_w64(in && key > key_at));
+        eq += __popcll(__builtin_amdgcn_ballot_w64(in && key == key_at));
+    }
+    if (lane == 0) {
+        wave_gt[wave] = gt;
+        wave_eq[wave] = eq;
+    }
+    __syncthreads();
+    int at_gt = 0, at_eq = 0;
+    for (int i = 0; i < wave; i++) {
+        at_gt += wave_gt[i];
+        at_eq += wave_eq[i];
+    }
+    int at = at_gt + min(at_eq, left);
+    const uint64_t below = (1ull << lane) - 1ull;
+    for (int j = lo; j < hi; j += 64) {
+        const bool in = j + lane < hi;
+        const float x = in ? w[j + lane] : 0.0f;
+        const uint32_t key = weight_key(x);
+        const uint64_t eqs = __builtin_amdgcn_ballot_w64(in && key == key_at);
+        const bool stays = in && (key > key_at ||
+                                  (key == key_at && at_eq + __popcll(eqs & below) < left));
+        const uint64_t stay = __builtin_amdgcn_ballot_w64(stays);
+        if (stays) {
+            const int to = at + __popcll(stay & below);
+            kept[to] = j + lane;
+            nw[to] = x;
+        }
+        at_eq += __popcll(eqs);
+        at += __popcll(stay);
+    }
+}
+
+// ---- eviction: moving them ---------------------------------------------------------------
+// A workgroup moves 64 kept tokens of one head, at their new places in whole
+// quads of four, so that each lane writes a value's piece of four tokens at once;
+// the reads are as scattered as the kept tokens are. Bound by bytes.
+constexpr int kMoveTokens = 64;
+
+template <int D>
+__global__ __launch_bounds__(256) void mx4_move_kernel(EvictArgs e, int blocks)
+{
+    constexpr int kPiece = D / 32; // code bytes of a token's value under one i
+    __shared__ const uint8_t* src_page[kMoveTokens];
+    __shared__ uint8_t* dst_page[kMoveTokens];
+    __shared__ int src_at[kMoveTokens];
+    const Mx4Page<D> lay(e.c.page_size());
+    const int unit = blockIdx.x / blocks, first = (blockIdx.x - unit * blocks) * kMoveTokens;
+    const int b = unit / e.c.heads, head = unit - b * e.c.heads;
+    const int mask = e.c.page_size() - 1;
+    const int n = min(min(evict_length(e, b), e.a.keep) - first, kMoveTokens);
+    if (n <= 0)
+        return;
+    if (threadIdx.x < kMoveTokens) {
+        const int i = threadIdx.x;
+        const uint8_t* sp = nullptr;
+        uint8_t* dp = nullptr;
+        int at = 0;
+        if (i < n) {
+            const int t = e.a.kept[(size_t)unit * e.a.keep + first + i];
+            const int j = (first + i) >> e.c.log2p;
+            const long long to = j < e.a.dst_pages ? e.a.dst_table[b * e.a.stride_dst_table + j]
+                                                   : -1;
+            const long long from = e.a.table[b * e.a.stride_table + (t >> e.c.log2p)];
+            if (e.c.in_cache(from) && e.c.in_cache(to)) {
+                sp = e.c.page(from, head, lay.bytes());
+                dp = e.c.page(to, head, lay.bytes());
+                at = t & mask;
+            }
+        }
+        src_page[i] = sp;
+        dst_page[i] = dp;
+        src_at[i] = at;
+    }
+    __syncthreads();
+    // keys: 16 bytes a lane
+    for (int x = threadIdx.x; x < kMoveTokens * (D / 32); x += 256) {
+        const int i = x / (D / 32), o = x % (D / 32) * 16;
+        if (src_page[i])
+            *(v4i*)(dst_page[i] + lay.k_row((first + i) & mask) + o) =
+                *(const v4i*)(src_page[i] + lay.k_row(src_at[i]) + o);
+    }
+    // values: the four tokens of a quad, each kPiece bytes
+    for (int x = threadIdx.x; x < kMoveTokens / 4 * 16; x += 256) {
+        const int quad = x / 16, i = x % 16;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int j = quad * 4 + u, to = (first + j) & mask;
+            if (!src_page[j])
+                continue;
+            const uint8_t* s = src_page[j] + lay.v_quad(src_at[j] / 4, i) + src_at[j] % 4 * kPiece;
+            uint8_t* d = dst_page[j] + lay.v_quad(to / 4, i) + to % 4 * kPiece;
+            if constexpr (kPiece == 2)
+                *(uint16_t*)d = *(const uint16_t*)s;
+            else if constexpr (kPiece == 4)
+                *(uint32_t*)d = *(const uint32_t*)s;
+            else
+                *(uint2*)d = *(const uint2*)s;
+        }
+    }
+    // scales
+    for (int x = threadIdx.x; x < kMoveTokens * kPiece; x += 256) {
+        const int i = x / kPiece, blk = x % kPiece, to = (first + i) & mask;
+        if (!src_page[i])
+            continue;
+        dst_page[i][lay.k_scale(to) + blk] = src_page[i][lay.k_scale(src_at[i]) + blk];
+        dst_page[i][lay.v_scale(to / 4, blk) + to % 4] =
+            src_page[i][lay.v_scale(src_at[i] / 4, blk) + src_at[i] % 4];
+    }
+}
+
+ga_status mx4_cache_check(const ga_mx4_cache* c)
+{
+    if (!c || !c->pages)
+        return fail(GA_ERR_ARG, "mx4 cache: null pages");
+    const size_t bytes = ga_mx4_page_bytes(c->page_size, c->head_dim);
+    if (!bytes)
+        return fail(GA_ERR_SHAPE, "mx4 cache: head_dim must be 64, 128 or 256 and page_size 16, 32, "
+                                  "64, 128 or 256");
+    if (c->num_pages <= 0 || c->kv_heads <= 0)
+        return fail(GA_ERR_ARG, "mx4 cache: num_pages and kv_heads must be positive");
+    if ((uintptr_t)c->pages % 16 || c->stride_page % 16 ||
+        c->stride_page < (long long)bytes * c->kv_heads)
+        return fail(GA_ERR_ARG, "mx4 cache: pages must be 16-byte aligned, stride_page a multiple "
+                                "of 16 and at least kv_heads pages' bytes");
+    return GA_OK;
+}
+
+// f(std::integral_constant<int, D>) for the cache's head_dim.
+template <class F>
+static void with_dim(int d, F&& f)
+{
+    if (d == 64)
+        f(std::integral_constant<int, 64>{});
+    else if (d == 128)
+        f(std::integral_constant<int, 128>{});
+    else
+        f(std::integral_constant<int, 256>{});
+}
+
+static bool aligned_rows(const void* p, long long row, long long head, int elems, int bytes)
+{
+    return (uintptr_t)p % bytes == 0 && row % elems == 0 && head % elems == 0;
+}
+
+} // namespace ga
+
+using namespace ga;
+
+extern "C" {
+
+size_t ga_mx4_page_bytes(int page_size, int head_dim)
+{
+    const bool dim = head_dim == 64 || head_dim == 128 || head_dim == 256;
+    const bool size = page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
+    return dim && size ? (size_t)page_size * (size_t)(head_dim + head_dim / 16) : 0;
+}
+
+ga_status ga_mx4_append(const ga_mx4_cache* cache, const void* k, const void* v, int in_dtype,
+                        int tokens, long long stride_k_row, long long stride_k_head,
+                        long long stride_v_row, long long stride_v_head, const long long* slots,
+                        int scale_rule, void* stream)
+{
+    if (const ga_status st = mx4_cache_check(cache))
+        return st;
+    if (in_dtype != GA_IN_F32 && in_dtype != GA_IN_BF16)
+        return fail(GA_ERR_ARG, "mx4_append: input dtype must be GA_IN_F32 or GA_IN_BF16");
+    if (tokens < 0 || scale_rule < 0 || scale_rule > 2)
+        return fail(GA_ERR_ARG, "mx4_append: bad token count or scale rule");
+    if (tokens == 0)
+        return GA_OK;
+    if (!k || !v || !slots)
+        return fail(GA_ERR_ARG, "mx4_append: null pointer");
+    const int least = in_dtype == GA_IN_F32 ? 16 : 8;
+    if (!aligned_rows(k, stride_k_row, stride_k_head, 4, least) ||
+        !aligned_rows(v, stride_v_row, stride_v_head, 4, least))
+        return fail(GA_ERR_SHAPE, "mx4_append: k and v must be %d-byte aligned with strides that "
+                                  "are multiples of 4", least);
+    const bool wide = in_dtype == GA_IN_BF16 &&
+                      aligned_rows(k, stride_k_row, stride_k_head, 8, 16) &&
+                      aligned_rows(v, stride_v_row, stride_v_head, 8, 16);
+    const long long rows = (long long)tokens * cache->kv_heads;
+    const long long blocks = (rows * (cache->head_dim / (wide ? 8 : 4)) + 255) / 256;
+    if (rows > 0x7FFFFFFFll || blocks > 0x7FFFFFFFll)
+        return fail(GA_ERR_SHAPE, "mx4_append: too many tokens for one call");
+    with_dim(cache->head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
+                               view_of(*cache), k, v, tokens, stride_k_row, stride_k_head,
+                               stride_v_row, stride_v_head, slots, scale_rule);
+        };
+        if (in_dtype == GA_IN_F32)
+            run(mx4_append_kernel<GA_IN_F32, 4, D>);
+        else if (wide)
+            run(mx4_append_kernel<GA_IN_BF16, 8, D>);
+        else
+            run(mx4_append_kernel<GA_IN_BF16, 4, D>);
+    });
+    GA_HIP_CHECK(hipGetLastError());
+    return GA_OK;
+}
+
+ga_status ga_mx4_read(const ga_mx4_cache* cache, const long long* slots, int tokens, void* k,
+                      void* v, int out_dtype, void* stream)
+{
+    if (const ga_status st = mx4_cache_check(cache))
+        return st;
+    if (out_dtype != GA_DTYPE_F32 && out_dtype != GA_DTYPE_BF16)
+        return fail(GA_ERR_ARG, "mx4_read: output dtype must be GA_DTYPE_F32 or GA_DTYPE_BF16");
+    if (tokens < 0)
+        return fail(GA_ERR_ARG, "mx4_read: bad token count");
+    if (tokens == 0)
+        return GA_OK;
+    if (!slots || !k || !v || (uintptr_t)k % 16 || (uintptr_t)v % 16)
+        return fail(GA_ERR_ARG, "mx4_read: k and v must be 16-byte aligned, nothing null");
+    const long long rows = (long long)tokens * cache->kv_heads;
+    const long long blocks = (rows * (cache->head_dim / 8) + 255) / 256;
+    if (rows > 0x7FFFFFFFll || blocks > 0x7FFFFFFFll)
+        return fail(GA_ERR_SHAPE, "mx4_read: too many tokens for one call");
+    with_dim(cache->head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
+                               view_of(*cache), slots, tokens, k, v);
+        };
+        if (out_dtype == GA_DTYPE_F32)
+            run(mx4_read_kernel<GA_DTYPE_F32, D>);
+        else
+            run(mx4_read_kernel<GA_DTYPE_BF16, D>);
+    });
+    GA_HIP_CHECK(hipGetLastError());
+    return GA_OK;
+}
+
+ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args, void* stream)
+{
+    if (const ga_status st = mx4_cache_check(cache))
+        return st;
+    if (!args)
+        return fail(GA_ERR_ARG, "mx4_evict: null arguments");
+    const ga_mx4_evict_args& a = *args;
+    if (a.keep <= 0 || a.recent < 0 || a.recent > a.keep)
+        return fail(GA_ERR_ARG, "mx4_evict: keep must be positive and recent 0 .. keep");
+    if (a.seqs < 0 || a.table_pages < 0 || a.dst_pages < 0 || a.width < 0 || a.new_width < a.keep)
+        return fail(GA_ERR_ARG, "mx4_evict: negative size, or new_width below keep");
+    if ((long long)a.dst_pages * cache->page_size < min(a.keep, a.width))
+        return fail(GA_ERR_SHAPE, "mx4_evict: dst_table's pages hold fewer than keep tokens");
+    if (a.seqs == 0)
+        return GA_OK;
+    if (!a.table || !a.lens || !a.dst_table || !a.weights || !a.kept || !a.new_lens ||
+        !a.new_weights)
+        return fail(GA_ERR_ARG, "mx4_evict: null pointer");
+    const long long units = (long long)a.seqs * cache->kv_heads;
+    const int blocks = (a.keep + kMoveTokens - 1) / kMoveTokens;
+    if (units * blocks > 0x7FFFFFFFll)
+        return fail(GA_ERR_SHAPE, "mx4_evict: too many sequences for one call");
+    const EvictArgs e{a, view_of(*cache)};
+    hipLaunchKernelGGL(mx4_select_kernel, dim3((unsigned)units), dim3(kSelThreads), 0,
+                       (hipStream_t)stream, e);
+    with_dim(cache->head_dim, [&](auto dim) {
+        hipLaunchKernelGGL((mx4_move_kernel<decltype(dim)::value>), dim3((unsigned)(units * blocks)),
+                           dim3(256), 0, (hipStream_t)stream, e, blocks);
+    });
+    GA_HIP_CHECK(hipGetLastError());
+    return GA_OK;
+}
+
+} // extern "C"

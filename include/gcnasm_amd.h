@@ -573,6 +573,136 @@ ga_status ga_ws_handle_reserve(ga_splitk_ws_handle* ws_handle, size_t bytes);
 ga_status ga_ws_handle_query(const ga_splitk_ws_handle* ws_handle, void** ptr, size_t* bytes);
 ga_status ga_ws_handle_destroy(ga_splitk_ws_handle* ws_handle);
 
+/* ------------------------------------------------------------------------- */
+/* A key/value cache in MXFP4 and what reads it (no counterpart in the        */
+/* reference).                                                                */
+/* ------------------------------------------------------------------------- */
+/* A cache is num_pages pages, stride_page bytes apart; a page holds page_size
+ * (P: 16, 32, 64, 128 or 256) tokens of every kv head, page bytes
+ * P * D * 17/16 after page bytes, D = head_dim 64, 128 or 256. In the page of
+ * one head, in this order, elements as e2m1 codes (the even one in the low
+ * nibble) and one E8M0 scale per 32 elements of a token's key or value:
+ *   K codes   [P][D/2]
+ *   V codes   [P/4][16][4][D/32]  of d = i*D/16 .. (i+1)*D/16 - 1 the bytes of
+ *                                 tokens 4q .. 4q+3 side by side: what a lane of
+ *                                 the matrix instruction takes
+ *   K scales  [P][D/32]
+ *   V scales  [P/4][D/32][4]
+ * pages 16-byte aligned, stride_page a multiple of 16 and at least
+ * kv_heads * page bytes. A token's slot is page * P + its place in the page. */
+typedef struct ga_mx4_cache {
+    void* pages;
+    long long num_pages;
+    long long stride_page;
+    int kv_heads;
+    int head_dim;
+    int page_size;
+} ga_mx4_cache;
+
+/* Bytes of one kv head's page (0: no such page). */
+size_t ga_mx4_page_bytes(int page_size, int head_dim);
+
+/* k, v [tokens, kv_heads, D] (fp32 or bf16; row and head strides in elements,
+ * multiples of 4; 16-byte aligned fp32, 8-byte aligned bf16) quantised by
+ * ga_quant_mxfp4's rules into slots[0 .. tokens - 1]. A slot outside the cache
+ * (a negative one, say) writes nothing; the others have to differ. */
+ga_status ga_mx4_append(const ga_mx4_cache* cache, const void* k, const void* v, int in_dtype,
+                        int tokens, long long stride_k_row, long long stride_k_head,
+                        long long stride_v_row, long long stride_v_head, const long long* slots,
+                        int scale_rule, void* stream);
+
+/* The values of slots[0 .. tokens - 1]: k, v [tokens, kv_heads, D] contiguous,
+ * fp32 or bf16 (out_dtype GA_DTYPE_*; bf16 holds every value that fp32 holds),
+ * 16-byte aligned; zeros where a slot lies outside the cache. */
+ga_status ga_mx4_read(const ga_mx4_cache* cache, const long long* slots, int tokens, void* k,
+                      void* v, int out_dtype, void* stream);
+
+/* Attention of the rows of this step over the cached tokens, grouped heads:
+ * query head h reads kv head h / (heads / kv_heads).
+ *   q, out   [rows, heads, D] bf16, rows and heads stride_* elements apart
+ *            (multiples of 8, 16-byte aligned)
+ *   lse      [rows, heads] fp32, rows stride_lse_row apart: natural logarithm of
+ *            the sum of exponentials; may be NULL in ga_mx4_attention
+ *   table    [seqs, table_pages] page numbers, rows stride_table apart; tokens of
+ *            a page outside the cache count as hidden
+ *   lens     [seqs] tokens of each sequence, this step's rows among them (at most
+ *            table_pages * P are used)
+ *   q_starts [seqs + 1] first row of each sequence (q_starts[seqs] = rows), or
+ *            NULL: row b is sequence b's only one
+ *   max_q, max_len  bounds of a sequence's rows and tokens, for the launch
+ *            alone: a longer sequence is slower, not wrong
+ * Row i of a sequence's n is at position len - n + i and sees, if causal,
+ * tokens up to its position, and with window > 0 (causal only) the last
+ * `window` of them. Scores are scale * q.k, with softcap > 0
+ * softcap * tanh(scale * q.k / softcap). A row that sees no token gets zeros,
+ * and lse -inf. */
+typedef struct ga_mx4_attention_args {
+    const void* q;
+    void* out;
+    float* lse;
+    const int* table;
+    const int* lens;
+    const int* q_starts;
+    long long stride_q_row, stride_q_head;
+    long long stride_out_row, stride_out_head;
+    long long stride_lse_row;
+    long long stride_table;
+    int seqs, rows, heads, table_pages;
+    int max_q, max_len;
+    int causal, window;
+    float scale, softcap;
+} ga_mx4_attention_args;
+
+/* Device scratch of ga_mx4_attention for these sizes on the current device (0:
+ * none). It need not be cleared; calls that overlap in time must not share it. */
+ga_status ga_mx4_attention_workspace_bytes(const ga_mx4_cache* cache,
+                                           const ga_mx4_attention_args* args, size_t* bytes);
+ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_args* args,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* What each cached token has been given: w_out[b, h, t] = w_in[b, h, t] + the
+ * sum of exp(score - lse) over the rows that see token t and the query heads of
+ * kv head h, fp32 [seqs, kv_heads, width], tokens contiguous, the other strides
+ * in elements. Zero from the sequence's length on; tokens past `width` are left
+ * out. w_in NULL counts as zeros, and may be w_out with the same strides. args: those
+ * of the attention; lse is read, out is not looked at. Sums run in a fixed
+ * order. */
+ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_attention_args* args,
+                                   const float* w_in, long long stride_in_seq,
+                                   long long stride_in_head, float* w_out,
+                                   long long stride_out_seq, long long stride_out_head, int width,
+                                   void* stream);
+
+/* Eviction: of each sequence longer than `keep` (>= 1), every kv head keeps its last
+ * `recent` (0 .. keep) tokens and of the others the keep - recent of largest
+ * weight (equal ones: the lowest index first; NaN counts as largest), in their
+ * order, moved to the pages of dst_table; a sequence of at most `keep` is moved
+ * whole.
+ *   weights     [seqs, kv_heads, width] fp32, width >= every length
+ *   kept        [seqs, kv_heads, keep] the kept tokens' indices, -1 behind them
+ *   new_lens    [seqs]
+ *   new_weights [seqs, kv_heads, new_width >= keep] the kept tokens' weights,
+ *               zeros behind them
+ * The pages of dst_table that a sequence needs (ceil(new_len / P)) must be pages
+ * that no table holds for tokens in use, and new_weights and new_lens no part of
+ * weights and lens. Kept tokens of a page outside the cache keep whatever the
+ * new page held. */
+typedef struct ga_mx4_evict_args {
+    const int* table;
+    const int* lens;
+    const int* dst_table;
+    const float* weights;
+    int* kept;
+    int* new_lens;
+    float* new_weights;
+    long long stride_table, stride_dst_table;
+    long long stride_w_seq, stride_w_head;
+    long long stride_new_seq, stride_new_head;
+    int seqs, table_pages, dst_pages, width, new_width;
+    int keep, recent;
+} ga_mx4_evict_args;
+ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args, void* stream);
+
 /* Device count of compute units of the current device (hipDeviceProp). */
 ga_status ga_device_num_cu(int* num_cu);
 
