@@ -196,6 +196,20 @@ struct ValueCodes {
         }
         scale = *(const uint32_t*)(s.page + lay.v_scale(quad, i * (D / 16) / 32));
     }
+    // zero the codes of tokens whose scale byte is 253 or more, and that byte
+    __device__ __forceinline__ void drop_huge()
+    {
+        static_for<4>([&](auto u) {
+            if ((scale >> (8 * u) & 0xFFu) < 253u)
+                return;
+            scale &= ~(0xFFu << (8 * u));
+            if constexpr (D == 64)
+                w[u / 2] &= ~(0xFFFFu << (u % 2 * 16));
+            else
+                for (int j = 0; j < D / 128; j++)
+                    w[u * (D / 128) + j] = 0;
+        });
+    }
     // byte B (elements 2B and 2B + 1 of the lane's D/16) of the 4 tokens, each a pair of bf16
     template <int B>
     __device__ __forceinline__ void pairs(uint32_t (&x)[4]) const
@@ -250,11 +264,28 @@ struct Tile {
     }
 };
 
+// Scores of 16 tokens (first operand) with RT blocks of 16 rows.
+template <int D, int RT>
+__device__ __forceinline__ void scores16(const KeyCodes<D>& k, const v4i (&q)[RT][D / 32],
+                                         v4f (&s)[RT])
+{
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+        s[rt] = (v4f){0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        const v4i a = k.operand(i);
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+            s[rt] = mfma_bf16_16x16x32(a, q[rt][i], s[rt]);
+    }
+}
+
 // ---- few rows -------------------------------------------------------------------------
-// A wave goes over its tiles of 32 tokens with 16 * RT rows, the next tile's loads in flight: the
-// scores leave the first product as the second one takes its probabilities (a
-// lane: 8 tokens of row lane % 16), so nothing passes through LDS until the waves'
-// results are joined. The tokens are split over the four waves and over
+// A wave goes over its tiles of 32 tokens with 16 * RT rows, the next tile's loads in
+// flight: the scores leave the first product as the second one takes its
+// probabilities (a lane: 8 tokens of row lane % 16), so nothing passes through LDS
+// until the waves' results are joined. The tokens are split over the waves and over
 // p.splits workgroups, whose results mx4_join_kernel joins.
 //
 // The running maximum is raised only when a score passes it by 2^8: until
@@ -264,20 +295,83 @@ struct Tile {
 // Probabilities enter the second product as two bf16 terms (16 bits of
 // significand together): one alone would add as much error as the output's own
 // rounding to bf16, and the matrix cores wait for memory here anyway.
+//
+// Bound by reading the cache: 4 x 131072 tokens (64 heads over 8, D = 128, 570 MB)
+// 114 us with the join, 5.0 TB/s, where a copy reaches 5.16; 64 sequences of 2048 to 8192
+// tokens (361 MB) 97 us, where every workgroup's first loads and the waves' join show.
+// The scheduling barriers keep the operands of one product live at a time: without
+// them and with the rare path below inside the loop the registers left room for 2
+// waves a SIMD instead of 3 (134 us of 64 x 8192, 143 of 4 x 131072).
 constexpr float kRaise = 8.0f;
 
+// What the sums lack: the tokens with a scale byte of 253 or more, whose values
+// pass bf16 or are NaN. In a product 0 * infinity would reach rows that do not
+// see the token, and the probabilities' second term undo an infinity by its sign; here
+// every row adds, in fp32, what it sees. Caches hold such scales only where their
+// input was infinite or near the end of fp32, so this is one token at a time.
 template <int D, int RT, bool CAP>
-__global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
+__device__ __forceinline__ void add_huge(const AttnParams& p, Mx4Page<D> lay, const int* table,
+                                         int head, int from, int step, int end, int lane,
+                                         const v4i (&q)[RT][D / 32], const int (&hi)[RT],
+                                         const int (&lo)[RT], const float (&base)[RT],
+                                         v4f (&acc)[RT][D / 16])
+{
+    constexpr int NT = D / 16;
+    const int g = lane >> 4;
+    for (int t0 = from; t0 < end; t0 += step) {
+#pragma unroll 1
+        for (int half = 0; half < 2; half++) {
+            const Sixteen at = locate<D>(p, lay, table, head, t0 + 16 * half, end);
+            KeyCodes<D> k;
+            k.load(at, lay, lane);
+            v4f s[RT];
+            scores16<D, RT>(k, q, s);
+#pragma unroll 1
+            for (int u = 0; u < 16; u++) {
+                const int t = t0 + 16 * half + u;
+                const uint32_t in = at.t + u;
+                const uint8_t own = at.page[lay.v_scale(in / 4, lane % (D / 32)) + in % 4];
+                if (!at.ok || !__builtin_amdgcn_ballot_w64(own >= 253u))
+                    continue;
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    const float mine = (u & 2) ? ((u & 1) ? s[rt][3] : s[rt][2])
+                                               : ((u & 1) ? s[rt][1] : s[rt][0]);
+                    const float x = __shfl(mine, u / 4 * 16 + (lane & 15), 64);
+                    const float w = exp2_of(score_log2<CAP>(p, x) - base[rt]);
+                    const bool sees = t <= hi[rt] && t > lo[rt];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t i = 4 * g + r;
+                        const uint32_t sc = at.page[lay.v_scale(in / 4, i * NT / 32) + in % 4];
+                        const uint8_t* codes = at.page + lay.v_quad(in / 4, i) + in % 4 * (D / 32);
+#pragma unroll
+                        for (int j = 0; j < NT; j++)
+                            if (sees && sc >= 253u)
+                                acc[rt][j][r] = fmaf(
+                                    w, fp4_value(codes[j / 2] >> (j % 2 * 4) & 15u, sc),
+                                    acc[rt][j][r]);
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <int D, int RT, bool CAP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mx4_rows_kernel(AttnParams p)
 {
     constexpr int NT = D / 16; // output tiles of 16 elements
     constexpr int kRows = 16 * RT;
-    __shared__ v4f red[2][RT * NT][64];
-    __shared__ float red_m[4][kRows], red_l[4][kRows];
+    __shared__ v4f red[WAVES / 2][RT * NT][64];
+    __shared__ float red_m[WAVES][kRows], red_l[WAVES][kRows];
     const int lane = threadIdx.x & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned unit = blockIdx.x;
-    const int split = unit % p.splits;
-    unit /= p.splits;
+    // splits outermost: the last ones, which short sequences leave empty, start last
+    // and spread over the XCDs
+    const unsigned units = gridDim.x / p.splits;
+    const int split = blockIdx.x / units;
+    unsigned unit = blockIdx.x - split * units;
     const int rb = unit % p.row_blocks;
     unit /= p.row_blocks;
     const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
@@ -309,28 +403,20 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
             for (int j = 0; j < NT; j++)
                 acc[rt][j] = (v4f){0, 0, 0, 0};
         }
+        bool huge = false; // a tile had values past bf16, or NaN
         auto step = [&](Tile<D>& tile, int t0) {
-            v4f s[RT][2];
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-                    s[rt][half] = (v4f){0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    const v4i a = tile.k[half].operand(i);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++)
-                        s[rt][half] = mfma_bf16_16x16x32(a, q[rt][i], s[rt][half]);
-                }
-            }
+            v4f s[2][RT];
+            scores16<D, RT>(tile.k[0], q, s[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            scores16<D, RT>(tile.k[1], q, s[1]);
+            __builtin_amdgcn_sched_barrier(0);
             const bool whole = t0 > blk.lo_max && t0 + 31 <= blk.hi_min && tile.ok[0] && tile.ok[1];
             float x[RT][8];
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    x[rt][j] = score_log2<CAP>(p, s[rt][j / 4][j % 4]);
+                    x[rt][j] = score_log2<CAP>(p, s[j / 4][rt][j % 4]);
             if (!whole) {
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
@@ -349,8 +435,11 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
                     tile.v[half].scale &= keep;
                 }
             }
-            const bool huge = __builtin_amdgcn_ballot_w64(any_huge(tile.v[0].scale) |
-                                                          any_huge(tile.v[1].scale)) != 0;
+            if (__builtin_amdgcn_ballot_w64(any_huge(tile.v[0].scale) | any_huge(tile.v[1].scale))) {
+                huge = true; // left to the end, one by one
+                tile.v[0].drop_huge();
+                tile.v[1].drop_huge();
+            }
             bool raise = false;
             float top[RT];
 #pragma unroll
@@ -394,72 +483,35 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
                                                x[rt][2 * j + 1] - __uint_as_float(h & 0xFFFF0000u));
                 }
             }
-            if (huge) {
-                // infinite values: 0 * infinity would reach rows that do not see the
-                // token, and the second term's sign undo it. One token at a time, each
-                // row only what it sees
-                float* px = (float*)red + wave * (2 * RT * NT * 64); // this wave's share
+            static_for<D / 32>([&](auto byte) {
+                constexpr int B = decltype(byte)::value;
+                v4i even, odd;
+                value_operands<D, B>(tile.v, even, odd);
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        px[(rt * 8 + j) * 64 + lane] = x[rt][j];
-                for (int t = 0; t < 32; t++) {
-                    const Sixteen at = locate<D>(p, lay, table, kv_head, t0 + (t & 16), end);
-                    const uint32_t in = at.t + (t & 15);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        if (!at.ok || t0 + t > hi[rt] || t0 + t <= lo[rt])
-                            continue;
-                        const float w = px[(rt * 8 + (t >> 4) * 4 + (t & 3)) * 64 +
-                                           (t >> 2 & 3) * 16 + (lane & 15)];
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-#pragma unroll
-                            for (int j = 0; j < NT; j++) {
-                                const uint32_t i = 4 * g + r;
-                                const uint8_t code =
-                                    at.page[lay.v_quad(in / 4, i) + in % 4 * (D / 32) + j / 2];
-                                const uint8_t sc =
-                                    at.page[lay.v_scale(in / 4, i * NT / 32) + in % 4];
-                                acc[rt][j][r] =
-                                    fmaf(w, fp4_value(code >> (j % 2 * 4) & 15u, sc), acc[rt][j][r]);
-                            }
-                    }
+                for (int rt = 0; rt < RT; rt++) {
+                    acc[rt][2 * B] = mfma_bf16_16x16x32(even, ph[rt], acc[rt][2 * B]);
+                    acc[rt][2 * B + 1] = mfma_bf16_16x16x32(odd, ph[rt], acc[rt][2 * B + 1]);
+                    acc[rt][2 * B] = mfma_bf16_16x16x32(even, pl[rt], acc[rt][2 * B]);
+                    acc[rt][2 * B + 1] = mfma_bf16_16x16x32(odd, pl[rt], acc[rt][2 * B + 1]);
                 }
-            } else {
-                static_for<D / 32>([&](auto byte) {
-                    constexpr int B = decltype(byte)::value;
-                    v4i even, odd;
-                    value_operands<D, B>(tile.v, even, odd);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        acc[rt][2 * B] = mfma_bf16_16x16x32(even, ph[rt], acc[rt][2 * B]);
-                        acc[rt][2 * B + 1] = mfma_bf16_16x16x32(odd, ph[rt], acc[rt][2 * B + 1]);
-                        acc[rt][2 * B] = mfma_bf16_16x16x32(even, pl[rt], acc[rt][2 * B]);
-                        acc[rt][2 * B + 1] = mfma_bf16_16x16x32(odd, pl[rt], acc[rt][2 * B + 1]);
-                    }
-                });
-            }
+                __builtin_amdgcn_sched_barrier(0);
+            });
         };
-        int t0 = begin + 32 * wave;
-        if (t0 < end) {
+        if (int t0 = begin + 32 * wave; t0 < end) {
             Tile<D> cur;
             cur.load(p, lay, table, kv_head, t0, end, lane);
-            while (true) {
-                const int next = t0 + 128;
-                if (next >= end)
-                    break;
-                Tile<D> ahead;
-                ahead.load(p, lay, table, kv_head, next, end, lane);
+            for (; t0 < end; t0 += 32 * WAVES) {
+                Tile<D> ahead; // past the end: the last tokens again, not used
+                ahead.load(p, lay, table, kv_head, t0 + 32 * WAVES, end, lane);
                 step(cur, t0);
                 cur = ahead;
-                t0 = next;
             }
-            step(cur, t0);
         }
+        if (huge)
+            add_huge<D, RT, CAP>(p, lay, table, kv_head, begin + 32 * wave, 32 * WAVES, end, lane, q,
+                                 hi, lo, base, acc);
 
-        // join the four waves: a common maximum, then the sums pairwise
+        // join the waves: a common maximum, then the sums pairwise
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             l[rt] += __shfl_xor(l[rt], 16, 64);
@@ -475,11 +527,11 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
             const int r = rt * 16 + (lane & 15);
             float top = red_m[0][r];
 #pragma unroll
-            for (int w = 1; w < 4; w++)
+            for (int w = 1; w < WAVES; w++)
                 top = fmaxf(top, red_m[w][r]);
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++)
+            for (int w = 0; w < WAVES; w++)
                 sum += red_m[w][r] == -INFINITY ? red_l[w][r]
                                                 : red_l[w][r] * exp2_of(red_m[w][r] - top);
             const float f = m[rt] == -INFINITY ? 1.0f : exp2_of(m[rt] - top);
@@ -491,7 +543,7 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
                 for (int k = 0; k < 4; k++)
                     acc[rt][j][k] *= f;
         }
-        for (int half = 2; half >= 1; half /= 2) {
+        for (int half = WAVES / 2; half >= 1; half /= 2) {
             if (wave >= half && wave < 2 * half) {
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
@@ -555,38 +607,76 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(AttnParams p)
     }
 }
 
-// The splits of a row joined, one wave a row: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s,
-// in the order of the splits. Bound by its launch and by reading the partial sums.
-template <int D>
+// The splits of a row joined: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s. A
+// workgroup of WAVES waves a row, each wave every WAVES-th split, then the waves in
+// order: the same order on every call. Bound by its launch, and with many splits by
+// the latency of reading their sums, so eight are read at a time.
+template <int D, int WAVES>
 __global__ __launch_bounds__(256) void mx4_join_kernel(AttnParams p)
 {
     constexpr int E = D / 64; // elements of a lane
-    const int lane = threadIdx.x & 63;
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= (long long)p.rows * p.heads)
-        return;
+    constexpr int kRows = 4 / WAVES;
+    __shared__ float part_acc[4][D], part_sum[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long unit = (long long)blockIdx.x * kRows + wave / WAVES;
+    const bool real = unit < (long long)p.rows * p.heads;
     const long long row = unit / p.heads;
     const int head = (int)(unit - row * p.heads);
     const size_t step = (size_t)p.rows * p.heads;
-    const float2* stats = (const float2*)p.ws + unit;
-    const float* part = p.ws + stats_floats(p.splits, p.rows, p.heads) + unit * D + lane * E;
-    float top = -INFINITY;
-    for (int s = lane; s < p.splits; s += 64)
-        top = fmaxf(top, stats[s * step].x);
+    float acc[E] = {}, sum = 0.0f, top = -INFINITY;
+    if (real) {
+        const float2* stats = (const float2*)p.ws + unit;
+        const float* part = p.ws + stats_floats(p.splits, p.rows, p.heads) + unit * D + lane * E;
+        for (int s = lane; s < p.splits; s += 64)
+            top = fmaxf(top, stats[s * step].x);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
-        top = fmaxf(top, __shfl_xor(top, o, 64));
-    float acc[E] = {}, sum = 0.0f;
-    for (int s = 0; s < p.splits; s++) {
-        const float2 ml = stats[s * step];
-        if (ml.x == -INFINITY && ml.y == 0.0f)
-            continue;
-        const float f = ml.x == -INFINITY ? 1.0f : exp2_of(ml.x - top);
-        sum += ml.y * f;
+        for (int o = 1; o < 64; o <<= 1)
+            top = fmaxf(top, __shfl_xor(top, o, 64));
+        for (int s0 = wave % WAVES; s0 < p.splits; s0 += 8 * WAVES) {
+            float2 ml[8];
+            float x[8][E];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int s = s0 + i * WAVES;
+                ml[i] = s < p.splits ? stats[s * step] : make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                // splits that saw nothing have written no sums
+                const bool none = ml[i].x == -INFINITY && ml[i].y == 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    x[i][e] = none ? 0.0f : part[(s0 + i * WAVES) * step * D + e];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float f = ml[i].x == -INFINITY ? 1.0f : exp2_of(ml[i].x - top);
+                sum += ml[i].y * f;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    acc[e] += x[i][e] * f;
+            }
+        }
+    }
+    if constexpr (WAVES > 1) {
 #pragma unroll
         for (int e = 0; e < E; e++)
-            acc[e] += part[s * step * D + e] * f;
+            part_acc[wave][lane * E + e] = acc[e];
+        if (lane == 0)
+            part_sum[wave] = sum;
+        __syncthreads();
+        if (wave != 0)
+            return;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            sum += part_sum[w];
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                acc[e] += part_acc[w][lane * E + e];
+        }
     }
+    if (!real)
+        return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint16_t* out = p.out + row * p.so_row + head * p.so_head + lane * E;
     if constexpr (E == 1) {
@@ -753,10 +843,20 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 }
 
 // How a call is cut. Row blocks of 16 rows while a sequence has no more, else of
-// 32 (D = 256: always 16, two blocks' sums do not fit the registers); tokens in chunks of a multiple of 128 (a tile for each of the four waves), as
-// many as give every CU a few workgroups.
+// 32 (D = 256: always 16, two blocks' sums do not fit the registers). Tokens in
+// chunks of a multiple of 128, a tile for each of four waves:
+// - Few tokens stay in one workgroup, of eight waves past 128, which saves the
+//   join's launch: 1 x 513 tokens of 8 kv heads (D = 128) 8.6 us against 8.9 split,
+//   and 4 us less on the host; 768 tokens 9.5 against 8.9; D = 256 already at 300
+//   tokens 10.5 against 10.7, at 520 12.4 against 10.9.
+// - Few sequences and heads get as many workgroups as the CUs hold at a time
+//   (4, 3, 2 of D = 64, 128, 256 by registers), so that all end together: 4 x
+//   131072 tokens 114 us, 4 a CU 141, 6 a CU 120.
+// - Many usually differ in length, and smaller chunks even that out: 64 sequences of
+//   2048 to 8192 tokens 97 us with up to 8 a CU, 103 with 4, 102 with 12.
 struct RowsPlan {
     int tiles; // of 16 rows
+    int waves;
     int row_blocks, splits, chunk;
     size_t ws_floats;
 };
@@ -774,7 +874,11 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
         span = std::min<long long>(span, (long long)a.window + 16 * r.tiles / group + 64);
     span = std::max<long long>(span, 1);
     const long long units = (long long)a.seqs * c.kv_heads * r.row_blocks;
-    const long long want = std::max<long long>(1, 4ll * num_cu / units);
+    const int resident = c.head_dim == 64 ? 4 : (c.head_dim == 128 ? 3 : 2);
+    const bool one = r.tiles == 1 && units < 2 * num_cu && span * c.head_dim <= 640 * 128;
+    r.waves = one && span > 128 ? 8 : 4;
+    const long long most = one ? 1 : (long long)(units < num_cu ? resident : 8) * num_cu / units;
+    const long long want = std::max<long long>(1, most);
     r.chunk = (int)(((span + want - 1) / want + 127) / 128 * 128);
     r.splits = (int)((span + r.chunk - 1) / r.chunk);
     if (r.splits > 1)
@@ -788,11 +892,14 @@ static void launch_rows(const AttnParams& p, const RowsPlan& r, unsigned grid, h
 {
     if constexpr (D < 256) {
         if (r.tiles == 2) {
-            hipLaunchKernelGGL((mx4_rows_kernel<D, 2, CAP>), dim3(grid), dim3(256), 0, s, p);
+            hipLaunchKernelGGL((mx4_rows_kernel<D, 2, CAP, 4>), dim3(grid), dim3(256), 0, s, p);
             return;
         }
     }
-    hipLaunchKernelGGL((mx4_rows_kernel<D, 1, CAP>), dim3(grid), dim3(256), 0, s, p);
+    if (r.waves == 8)
+        hipLaunchKernelGGL((mx4_rows_kernel<D, 1, CAP, 8>), dim3(grid), dim3(512), 0, s, p);
+    else
+        hipLaunchKernelGGL((mx4_rows_kernel<D, 1, CAP, 4>), dim3(grid), dim3(256), 0, s, p);
 }
 
 // f(std::integral_constant<int, D>, std::bool_constant<capped>)
@@ -868,10 +975,12 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
     with_dim_cap(cache->head_dim, a.softcap > 0.0f, [&](auto dim, auto cap) {
         constexpr int D = decltype(dim)::value;
         launch_rows<D, decltype(cap)::value>(p, r, (unsigned)grid, st);
-        if (r.splits > 1)
-            hipLaunchKernelGGL((mx4_join_kernel<D>),
-                               dim3((unsigned)(((long long)a.rows * a.heads + 3) / 4)), dim3(256), 0,
-                               st, p);
+        const long long joins = (long long)a.rows * a.heads;
+        if (r.splits > 4)
+            hipLaunchKernelGGL((mx4_join_kernel<D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
+        else if (r.splits > 1)
+            hipLaunchKernelGGL((mx4_join_kernel<D, 1>), dim3((unsigned)((joins + 3) / 4)), dim3(256),
+                               0, st, p);
     });
     GA_HIP_CHECK(hipGetLastError());
     return GA_OK;

@@ -23,13 +23,16 @@ stream that the call runs on.
 """
 import contextlib
 import ctypes
-import math
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
 from .f4gemm import _stream_handle
+
+
+# (page bytes, head size) -> tokens of a page, for every page there is
+_PAGE_SIZES = {(p * d * 17 // 16, d): p for p in (16, 32, 64, 128, 256) for d in (64, 128, 256)}
 
 
 def page_bytes(page_size, head_dim):
@@ -47,45 +50,42 @@ def new_cache(num_pages, kv_heads, head_dim, page_size=64, device="cuda"):
                        device=device)
 
 
+# The checks below run on every call, of which a decode step makes several for each
+# layer: they ask a tensor for as little as they can.
+
+
 def _cache(cache, head_dim):
-    if cache.dtype != torch.uint8 or cache.dim() != 3:
+    if cache.dtype is not torch.uint8 or cache.dim() != 3:
         raise TypeError("a cache is a uint8 tensor [pages, kv heads, page bytes]")
     pages, heads, size = cache.shape
-    page = size * 16 // (17 * head_dim) if head_dim > 0 else 0
-    if size == 0 or lib().ga_mx4_page_bytes(page, head_dim) != size:
+    page = _PAGE_SIZES.get((size, head_dim))
+    if page is None:
         raise ValueError("pages of %d bytes hold no tokens of head size %d" % (size, head_dim))
-    if cache.stride(2) != 1 or (heads > 1 and cache.stride(1) != size):
+    stride, head_stride, inner = cache.stride()
+    if inner != 1 or (heads > 1 and head_stride != size):
         raise ValueError("the heads of a page must be contiguous (strides %s)"
                          % (tuple(cache.stride()),))
-    _on_device(cache, "cache")
-    stride = cache.stride(0) if pages > 1 else heads * size
-    return _lib.Mx4Cache(cache.data_ptr(), pages, stride, heads, head_dim, page)
+    device = cache.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise ValueError("the cache is on %s, not on the current GPU" % cache.device)
+    return _lib.Mx4Cache(cache.data_ptr(), pages, stride if pages > 1 else heads * size, heads,
+                         head_dim, page), device
 
 
-def _on_device(x, what, like=None):
-    if x.device.type != "cuda":
-        raise ValueError("%s must be on the GPU" % what)
-    index = torch.cuda.current_device() if like is None else like.device.index
-    if x.device.index != index:
-        raise ValueError("%s is on %s, not on the device of the call (cuda:%d)"
-                         % (what, x.device, index))
-
-
-def _whole(x, what, dtype, shape, cache):
-    """Checks a tensor of whole numbers whose last dimension is contiguous."""
-    if x.dtype != dtype:
-        raise TypeError("%s must be %s" % (what, dtype))
-    if tuple(x.shape) != tuple(shape):
+def _check(x, what, dtype, shape, device):
+    """Checks type, shape and place of a tensor whose last dimension is contiguous, and
+    returns its strides."""
+    if x.dtype is not dtype:
+        raise TypeError("%s must be %s, is %s" % (what, dtype, x.dtype))
+    if x.shape != shape:
         raise ValueError("%s must be %s, is %s" % (what, tuple(shape), tuple(x.shape)))
-    if x.numel() > 1 and x.shape[-1] > 1 and x.stride(-1) != 1:
-        raise ValueError("%s must be contiguous along its last dimension" % what)
-    _on_device(x, what, cache)
-
-
-def _inner(x, what):
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    strides = x.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError("%s must be contiguous along its last dimension (strides %s)"
-                         % (what, tuple(x.stride())))
+                         % (what, tuple(strides)))
+    if x.get_device() != device:
+        raise ValueError("%s is on %s, not on the cache's GPU" % (what, x.device))
+    return strides
 
 
 def _on(stream):
@@ -97,74 +97,69 @@ def _on(stream):
     return torch.cuda.stream(stream)
 
 
+_IN_TYPES = {torch.float32: _lib.GA_IN_F32, torch.bfloat16: _lib.GA_IN_BF16}
+_OUT_TYPES = {torch.float32: _lib.GA_DTYPE_F32, torch.bfloat16: _lib.GA_DTYPE_BF16}
+
+
 def append(cache, k, v, slots, scale_rule=_lib.GA_MX_SCALE_FLOOR_448, stream=None):
     """Quantises k, v [tokens, kv heads, D] (float32 or bfloat16, any row and head
     strides that are multiples of 4) into slots, int64 [tokens]. A slot outside the
     cache, such as -1, writes nothing; the others have to differ. The rules are
     those of ops.quant_mxfp4."""
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError("k and v must be [tokens, kv heads, D] of one type (%s %s, %s %s)"
-                         % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
-    if k.dtype not in (torch.float32, torch.bfloat16):
+    if k.dim() != 3:
+        raise ValueError("k must be [tokens, kv heads, D], is %s" % (tuple(k.shape),))
+    kind = _IN_TYPES.get(k.dtype)
+    if kind is None:
         raise TypeError("k and v must be float32 or bfloat16")
-    tokens, heads, dim = k.shape
-    c = _cache(cache, dim)
+    tokens, heads, dim = shape = k.shape
+    c, device = _cache(cache, dim)
     if heads != c.kv_heads:
         raise ValueError("k has %d heads, the cache %d" % (heads, c.kv_heads))
-    _whole(slots, "slots", torch.int64, (tokens,), cache)
-    for x, what in ((k, "k"), (v, "v")):
-        _inner(x, what)
-        _on_device(x, what, cache)
-    kind = _lib.GA_IN_F32 if k.dtype == torch.float32 else _lib.GA_IN_BF16
-    check(lib().ga_mx4_append(ctypes.byref(c), k.data_ptr(), v.data_ptr(), kind, tokens,
-                              k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                              slots.data_ptr(), scale_rule, _stream_handle(stream)))
+    _check(slots, "slots", torch.int64, (tokens,), device)
+    sk = _check(k, "k", k.dtype, shape, device)
+    sv = _check(v, "v", k.dtype, shape, device)
+    check(lib().ga_mx4_append(c, k.data_ptr(), v.data_ptr(), kind, tokens, sk[0], sk[1], sv[0],
+                              sv[1], slots.data_ptr(), scale_rule, _stream_handle(stream)))
 
 
 def read(cache, slots, head_dim, dtype=torch.bfloat16, stream=None):
     """Keys and values [tokens, kv heads, D] that slots (int64 [tokens]) hold, bfloat16
     or float32 (both hold them exactly); zeros for a slot outside the cache."""
-    if dtype not in (torch.float32, torch.bfloat16):
+    kind = _OUT_TYPES.get(dtype)
+    if kind is None:
         raise TypeError("dtype must be float32 or bfloat16")
-    c = _cache(cache, head_dim)
-    _whole(slots, "slots", torch.int64, (slots.numel(),), cache)
+    c, device = _cache(cache, head_dim)
+    tokens = slots.numel()
+    _check(slots, "slots", torch.int64, (tokens,), device)
     with _on(stream):
-        k = torch.empty((slots.numel(), c.kv_heads, head_dim), dtype=dtype, device=cache.device)
+        k = cache.new_empty((tokens, c.kv_heads, head_dim), dtype=dtype)
         v = torch.empty_like(k)
-    kind = _lib.GA_DTYPE_F32 if dtype == torch.float32 else _lib.GA_DTYPE_BF16
-    check(lib().ga_mx4_read(ctypes.byref(c), slots.data_ptr(), slots.numel(), k.data_ptr(),
-                            v.data_ptr(), kind, _stream_handle(stream)))
+    check(lib().ga_mx4_read(c, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(), kind,
+                            _stream_handle(stream)))
     return k, v
 
 
 def _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window, softcap):
-    if q.dim() != 3 or q.dtype != torch.bfloat16:
-        raise TypeError("q must be bfloat16 [rows, heads, D]")
+    if q.dim() != 3:
+        raise ValueError("q must be [rows, heads, D], is %s" % (tuple(q.shape),))
     rows, heads, dim = q.shape
-    c = _cache(cache, dim)
-    seqs = lens.shape[0] if lens.dim() == 1 else -1
-    _whole(lens, "lens", torch.int32, (seqs,), cache)
-    if table.dim() != 2:
-        raise ValueError("table must be [sequences, pages]")
-    _whole(table, "table", torch.int32, (seqs, table.shape[1]), cache)
+    c, device = _cache(cache, dim)
+    sq = _check(q, "q", torch.bfloat16, q.shape, device)
+    if lens.dim() != 1 or table.dim() != 2:
+        raise ValueError("lens must be [sequences], table [sequences, pages]")
+    seqs, pages = lens.shape[0], table.shape[1]
+    _check(lens, "lens", torch.int32, (seqs,), device)
+    st = _check(table, "table", torch.int32, (seqs, pages), device)
+    starts = None
     if q_starts is not None:
-        _whole(q_starts, "q_starts", torch.int32, (seqs + 1,), cache)
-    _inner(q, "q")
-    _on_device(q, "q", cache)
-    a = _lib.Mx4AttentionArgs()
-    a.q = q.data_ptr()
-    a.table, a.lens = table.data_ptr(), lens.data_ptr()
-    a.q_starts = None if q_starts is None else q_starts.data_ptr()
-    a.stride_q_row, a.stride_q_head = q.stride(0), q.stride(1)
-    a.stride_table = table.stride(0)
-    a.seqs, a.rows, a.heads, a.table_pages = seqs, rows, heads, table.shape[1]
-    a.max_q = rows if max_q is None else max_q
-    full = table.shape[1] * c.page_size
-    a.max_len = min(full, 0x7FFFFFFF) if max_len is None else max_len
-    a.causal, a.window = int(bool(causal)), window
-    a.scale = 1.0 / math.sqrt(dim) if scale is None else scale
-    a.softcap = softcap
-    return c, a
+        _check(q_starts, "q_starts", torch.int32, (seqs + 1,), device)
+        starts = q_starts.data_ptr()
+    if max_len is None:
+        max_len = min(pages * c.page_size, 0x7FFFFFFF)
+    return c, device, _lib.Mx4AttentionArgs(
+        q.data_ptr(), None, None, table.data_ptr(), lens.data_ptr(), starts, sq[0], sq[1], 0, 0, 0,
+        st[0], seqs, rows, heads, pages, rows if max_q is None else max_q, max_len,
+        1 if causal else 0, window, dim ** -0.5 if scale is None else scale, softcap)
 
 
 def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, scale=None,
@@ -185,54 +180,43 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
     choose the launch and may be larger than what the tensors hold (default: all
     rows, all of the table). workspace: a tensor of at least
     attention_workspace_bytes, for callers that keep one."""
-    c, a = _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window, softcap)
-    return _attention(c, a, q, out, lse, workspace, stream)
-
-
-def _attention(c, a, q, out, lse, workspace, stream):
-    l = lib()
+    c, device, a = _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window,
+                         softcap)
     need = ctypes.c_size_t(0)
-    check(l.ga_mx4_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(a), ctypes.byref(need)))
+    check(lib().ga_mx4_attention_workspace_bytes(c, a, need))
     with _on(stream):
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if lse is None:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+            lse = q.new_empty(q.shape[:2], dtype=torch.float32)
         if workspace is None and need.value:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    if out.dtype != torch.bfloat16 or out.shape != q.shape:
-        raise ValueError("out must be bfloat16 %s" % (tuple(q.shape),))
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:2]:
-        raise ValueError("lse must be float32 %s" % (tuple(q.shape[:2]),))
-    for x, what in ((out, "out"), (lse, "lse")):
-        _inner(x, what)
-        _on_device(x, what, q)
+            workspace = q.new_empty(need.value, dtype=torch.uint8)
+    so = _check(out, "out", torch.bfloat16, q.shape, device)
+    sl = _check(lse, "lse", torch.float32, q.shape[:2], device)
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    a.stride_out_row, a.stride_out_head = out.stride(0), out.stride(1)
-    a.stride_lse_row = lse.stride(0)
+    a.stride_out_row, a.stride_out_head, a.stride_lse_row = so[0], so[1], sl[0]
     ptr, size = None, 0
     if workspace is not None:
-        _on_device(workspace, "workspace", q)
+        if workspace.get_device() != device:
+            raise ValueError("workspace is on %s, not on the cache's GPU" % workspace.device)
         ptr, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    check(l.ga_mx4_attention(ctypes.byref(c), ctypes.byref(a), ptr, size, _stream_handle(stream)))
+    check(lib().ga_mx4_attention(c, a, ptr, size, _stream_handle(stream)))
     return out, lse
 
 
 def attention_workspace_bytes(q, cache, table, lens, q_starts=None, max_q=None, max_len=None,
                               causal=True, window=0):
     """Bytes of scratch that attention() takes for these sizes."""
-    c, a = _args(q, cache, table, lens, q_starts, max_q, max_len, None, causal, window, 0.0)
+    c, _, a = _args(q, cache, table, lens, q_starts, max_q, max_len, None, causal, window, 0.0)
     need = ctypes.c_size_t(0)
-    check(lib().ga_mx4_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(a),
-                                                 ctypes.byref(need)))
+    check(lib().ga_mx4_attention_workspace_bytes(c, a, need))
     return need.value
 
 
-def _weights(x, what, seqs, heads, cache):
-    if x.dtype != torch.float32 or x.dim() != 3 or tuple(x.shape[:2]) != (seqs, heads):
-        raise ValueError("%s must be float32 [%d, %d, tokens]" % (what, seqs, heads))
-    _inner(x, what)
-    _on_device(x, what, cache)
+def _weights(x, what, seqs, heads, device):
+    if x.dim() != 3:
+        raise ValueError("%s must be [%d, %d, tokens]" % (what, seqs, heads))
+    return _check(x, what, torch.float32, (seqs, heads, x.shape[2]), device)
 
 
 def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, max_q=None,
@@ -243,27 +227,25 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
     and the query heads of the kv head. q, lse and the rest as of the attention()
     call. -> out, float32 [sequences, kv heads, width] (width: weights', or
     max_len), zeros from a sequence's length on; out may be weights."""
-    c, a = _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window, softcap)
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:2]:
-        raise ValueError("lse must be float32 %s" % (tuple(q.shape[:2]),))
-    _inner(lse, "lse")
-    _on_device(lse, "lse", cache)
-    a.lse, a.stride_lse_row = lse.data_ptr(), lse.stride(0)
+    c, device, a = _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window,
+                         softcap)
+    a.stride_lse_row = _check(lse, "lse", torch.float32, q.shape[:2], device)[0]
+    a.lse = lse.data_ptr()
+    ptr, sw = None, (0, 0)
     if weights is not None:
-        _weights(weights, "weights", a.seqs, c.kv_heads, cache)
+        sw = _weights(weights, "weights", a.seqs, c.kv_heads, device)
+        ptr = weights.data_ptr()
     if out is None:
         if width is None:
             width = a.max_len if weights is None else weights.shape[2]
         with _on(stream):
-            out = torch.empty((a.seqs, c.kv_heads, width), dtype=torch.float32,
-                              device=cache.device)
-    _weights(out, "out", a.seqs, c.kv_heads, cache)
-    if weights is not None and weights.shape[2] < out.shape[2]:
-        raise ValueError("weights hold %d tokens, out %d" % (weights.shape[2], out.shape[2]))
-    w, sw = (None, (0, 0)) if weights is None else (weights.data_ptr(), weights.stride())
-    check(lib().ga_mx4_attention_weights(ctypes.byref(c), ctypes.byref(a), w, sw[0], sw[1],
-                                         out.data_ptr(), out.stride(0), out.stride(1),
-                                         out.shape[2], _stream_handle(stream)))
+            out = q.new_empty((a.seqs, c.kv_heads, width), dtype=torch.float32)
+    so = _weights(out, "out", a.seqs, c.kv_heads, device)
+    width = out.shape[2]
+    if weights is not None and weights.shape[2] < width:
+        raise ValueError("weights hold %d tokens, out %d" % (weights.shape[2], width))
+    check(lib().ga_mx4_attention_weights(c, a, ptr, sw[0], sw[1], out.data_ptr(), so[0], so[1],
+                                         width, _stream_handle(stream)))
     return out
 
 
@@ -279,32 +261,25 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
     the width of the new_weights given], zeros behind). The pages of dst_table must
     be pages that no table holds for tokens in use; those of `table` are free
     for others once the call has run on its stream."""
-    c = _cache(cache, head_dim)
-    seqs = lens.shape[0] if lens.dim() == 1 else -1
-    _whole(lens, "lens", torch.int32, (seqs,), cache)
-    for x, what in ((table, "table"), (dst_table, "dst_table")):
-        if x.dim() != 2:
-            raise ValueError("%s must be [sequences, pages]" % what)
-        _whole(x, what, torch.int32, (seqs, x.shape[1]), cache)
-    _weights(weights, "weights", seqs, c.kv_heads, cache)
+    c, device = _cache(cache, head_dim)
+    if lens.dim() != 1 or table.dim() != 2 or dst_table.dim() != 2:
+        raise ValueError("lens must be [sequences], the tables [sequences, pages]")
+    seqs, pages, dst_pages = lens.shape[0], table.shape[1], dst_table.shape[1]
+    _check(lens, "lens", torch.int32, (seqs,), device)
+    st = _check(table, "table", torch.int32, (seqs, pages), device)
+    sd = _check(dst_table, "dst_table", torch.int32, (seqs, dst_pages), device)
+    sw = _weights(weights, "weights", seqs, c.kv_heads, device)
     if keep <= 0 or not 0 <= recent <= keep:
         raise ValueError("keep must be positive and recent 0 .. keep")
     with _on(stream):
-        kept = torch.empty((seqs, c.kv_heads, keep), dtype=torch.int32, device=cache.device)
+        kept = lens.new_empty((seqs, c.kv_heads, keep))
         new_lens = torch.empty_like(lens)
         if new_weights is None:
-            new_weights = torch.empty((seqs, c.kv_heads, keep), dtype=torch.float32,
-                                      device=cache.device)
-    _weights(new_weights, "new_weights", seqs, c.kv_heads, cache)
-    a = _lib.Mx4EvictArgs()
-    a.table, a.lens, a.dst_table = table.data_ptr(), lens.data_ptr(), dst_table.data_ptr()
-    a.weights, a.kept = weights.data_ptr(), kept.data_ptr()
-    a.new_lens, a.new_weights = new_lens.data_ptr(), new_weights.data_ptr()
-    a.stride_table, a.stride_dst_table = table.stride(0), dst_table.stride(0)
-    a.stride_w_seq, a.stride_w_head = weights.stride(0), weights.stride(1)
-    a.stride_new_seq, a.stride_new_head = new_weights.stride(0), new_weights.stride(1)
-    a.seqs, a.table_pages, a.dst_pages = seqs, table.shape[1], dst_table.shape[1]
-    a.width, a.new_width = weights.shape[2], new_weights.shape[2]
-    a.keep, a.recent = keep, recent
-    check(lib().ga_mx4_evict(ctypes.byref(c), ctypes.byref(a), _stream_handle(stream)))
+            new_weights = weights.new_empty((seqs, c.kv_heads, keep))
+    sn = _weights(new_weights, "new_weights", seqs, c.kv_heads, device)
+    a = _lib.Mx4EvictArgs(
+        table.data_ptr(), lens.data_ptr(), dst_table.data_ptr(), weights.data_ptr(),
+        kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(), st[0], sd[0], sw[0], sw[1],
+        sn[0], sn[1], seqs, pages, dst_pages, weights.shape[2], new_weights.shape[2], keep, recent)
+    check(lib().ga_mx4_evict(c, a, _stream_handle(stream)))
     return kept, new_lens, new_weights
