@@ -293,7 +293,10 @@ SIGNATURES = {
     "ga_mx4_attention": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4AttentionArgs), _vp, _sz,
                               _vp]),
     "ga_mx4_attention_weights": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4AttentionArgs),
-                                      _vp, _ll, _ll, _vp, _ll, _ll, _i, _vp]),
+                                      _vp, _ll, _ll, _vp, _ll, _ll, _i, _vp, _sz, _vp]),
+    "ga_mx4_attention_weights_workspace_bytes": (_i, [ctypes.POINTER(Mx4Cache),
+                                                      ctypes.POINTER(Mx4AttentionArgs), _i,
+                                                      ctypes.POINTER(_sz)]),
     "ga_mx4_evict": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4EvictArgs), _vp]),
     "ga_device_num_cu": (_i, [ctypes.POINTER(_i)]),
 }

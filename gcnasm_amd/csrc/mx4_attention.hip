@@ -172,6 +172,22 @@ struct KeyCodes {
     }
 };
 
+// The keys of 16 tokens as operands whose product m sums d = 32m .. 32m + 31, lane 16*g + r
+// the eight from 32m + 8g. The queries are then read 64 bytes of a row at a time instead of 16 bytes
+// 64 apart, which is four times the rate of the L1, where many queries meet each
+// key; the keys' loads are four times as many.
+template <int D>
+__device__ __forceinline__ void load_keys_in_order(const Sixteen& s, Mx4Page<D> lay, int lane,
+                                                   v4i (&k)[D / 32])
+{
+    const uint32_t g = lane >> 4, t = s.t + (lane & 15);
+    const uint8_t* src = s.page + lay.k_row(t) + 4 * g;
+    const uint8_t* sc = s.page + lay.k_scale(t);
+#pragma unroll
+    for (int m = 0; m < D / 32; m++)
+        k[m] = fp4_oct_bf16(*(const uint32_t*)(src + 16 * m), e8m0_of<0>(sc[m]));
+}
+
 template <int D>
 struct ValueCodes {
     static constexpr int kWords = D / 32; // of 4 tokens, D/32 bytes each
@@ -691,91 +707,380 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(AttnParams p)
 }
 
 // ---- the weights of the tokens ------------------------------------------------------------
-// A wave holds 32 tokens' keys as operands and goes over the rows that see them, 16 at a time;
-// a lane adds up the probabilities of 8 tokens over its rows (lane % 16 of
-// each 16), and the 16 lanes are added once at the end: no atomics, a fixed order.
-// Few rows: bound by reading the keys; prompts: by the exponentials.
-template <int D, bool CAP>
-__global__ __launch_bounds__(256) void mx4_weights_kernel(AttnParams p, const float* w_in,
-                                                          long long si_seq, long long si_head,
-                                                          float* w_out, long long so_seq,
-                                                          long long so_head, int width,
-                                                          int blocks)
+// w[t] += sum over rows and heads of 2^(x_t - lse log2 e). The scores' product has tokens on its
+// rows, so a lane adds up the probabilities of its tokens over its rows (lane % 16 of each 16),
+// and the 16 lanes are added once at the end: no atomics, a fixed order.
+struct WeightsParams {
+    AttnParams a;
+    const float* w_in;
+    float* w_out;
+    long long si_seq, si_head, so_seq, so_head;
+    int width, chunk; // chunk: tokens of a workgroup (few rows), or rows (many)
+    int splits;       // workgroups along the rows (many)
+    float* ws;        // their sums, [splits][seqs][kv heads][width]
+
+    __device__ __forceinline__ void store(const Sequence& s, int b, int head, int t, float x) const
+    {
+        if (t >= width)
+            return;
+        float y = 0.0f;
+        if (t < s.len) {
+            y = x;
+            if (w_in)
+                y += w_in[b * si_seq + head * si_head + t];
+        }
+        w_out[b * so_seq + head * so_head + t] = y;
+    }
+};
+
+// Sum over aligned groups of 16 lanes, in every lane of them.
+__device__ __forceinline__ float sum16(float x)
 {
+    auto dpp = [](float v, auto ctrl) {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+            0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, false));
+    };
+    x += dpp(x, std::integral_constant<int, 0xB1>{});  // quad_perm(1,0,3,2)
+    x += dpp(x, std::integral_constant<int, 0x4E>{});  // quad_perm(2,3,0,1)
+    x += dpp(x, std::integral_constant<int, 0x141>{}); // row_half_mirror
+    x += dpp(x, std::integral_constant<int, 0x140>{}); // row_mirror
+    return x;
+}
+
+// sum[4 * s + u] over its lanes, for token 16 * s + 4 * g + u in lane 16 * g + 4 * s + u.
+template <int N>
+__device__ __forceinline__ float own_sum(const float (&sum)[N], int lane)
+{
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float y = sum16(sum[i]);
+        x = (lane & 15) == i ? y : x;
+    }
+    return x;
+}
+
+__device__ __forceinline__ int own_token(int lane)
+{
+    return 16 * (lane >> 2 & 3) + 4 * (lane >> 4) + (lane & 3);
+}
+
+// 16 rows' queries and what their probabilities need.
+template <int D>
+struct WeightRows {
+    v4i q[D / 32];
+    float lse2; // lse log2 e
+    int hi, lo;
+};
+
+// A lane's row of a sequence's n * group (row x: query x / group, head x % group), and steps of
+// `step` rows from it without a division.
+struct RowCursor {
+    long long q, lse;                             // offsets of the row, in elements
+    long long q0, lse0;                           // of the sequence's first row
+    long long q_step, q_wrap, lse_step, lse_wrap; // of a step, and if the head wraps besides
+    int in, d_in, group;                          // head of the kv head's
+    int hi, lo, top, d_hi, wrap_hi, d_lo, wrap_lo;
+    RowCursor() = default;
+    __device__ __forceinline__ RowCursor(const AttnParams& p, const Sequence& s, int kv_head, int x,
+                                         int step, int offset)
+    {
+        group = p.group;
+        const int i = x / group;
+        in = x - i * group;
+        const int di = step / group;
+        d_in = step - di * group;
+        q0 = s.q0 * p.sq_row + kv_head * group * p.sq_head + offset;
+        lse0 = s.q0 * p.sl_row + kv_head * group;
+        q = q0 + i * p.sq_row + in * p.sq_head;
+        lse = lse0 + i * p.sl_row + in;
+        q_step = di * p.sq_row + d_in * p.sq_head;
+        q_wrap = p.sq_row - group * p.sq_head;
+        lse_step = di * p.sl_row + d_in;
+        lse_wrap = p.sl_row - group;
+        top = s.len - 1;
+        hi = p.causal ? s.len - s.n + i : top;
+        d_hi = p.causal ? di : 0;
+        wrap_hi = p.causal ? 1 : 0;
+        lo = p.window ? s.len - s.n + i - p.window : -1;
+        d_lo = p.window ? di : 0;
+        wrap_lo = p.window ? 1 : 0;
+    }
+    // the lane's operands; real: the row is one of the sequence's (which has one), otherwise
+    // the first row is read, for nothing
+    template <int D>
+    __device__ __forceinline__ void load(const AttnParams& p, WeightRows<D>& r, bool real) const
+    {
+        const uint16_t* src = p.q + (real ? q : q0);
+#pragma unroll
+        for (int m = 0; m < D / 32; m++)
+            r.q[m] = *(const v4i*)(src + 8 * m);
+        r.lse2 = p.lse[real ? lse : lse0] * kLog2e;
+        r.hi = real ? min(hi, top) : -1;
+        r.lo = lo;
+    }
+    __device__ __forceinline__ void advance()
+    {
+        in += d_in;
+        const bool wrap = in >= group;
+        in -= wrap ? group : 0;
+        q += q_step + (wrap ? q_wrap : 0);
+        lse += lse_step + (wrap ? lse_wrap : 0);
+        hi += d_hi + (wrap ? wrap_hi : 0);
+        lo += d_lo + (wrap ? wrap_lo : 0);
+    }
+};
+
+// N tiles of 16 tokens' probabilities under 16 rows added to the tokens' sums: all products
+// first, so that each one's latency is behind the others.
+template <int D, int N, bool CAP>
+__device__ __forceinline__ void add_weights(const AttnParams& p, const v4i (&k)[N][D / 32],
+                                            const WeightRows<D>& r, bool whole,
+                                            const bool (&ok)[N], int t, float (&sum)[4 * N])
+{
+    v4f s[N];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        s[n] = (v4f){0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+        for (int n = 0; n < N; n++)
+            s[n] = mfma_bf16_16x16x32(k[n][i], r.q[i], s[n]);
+    float w[4 * N];
+#pragma unroll
+    for (int j = 0; j < 4 * N; j++) {
+        const float x = s[j / 4][j % 4];
+        w[j] = exp2_of(CAP ? score_log2<CAP>(p, x) - r.lse2 : fmaf(x, p.to_log2, -r.lse2));
+    }
+    if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 4 * N; j++) {
+            const int at = t + 16 * (j / 4) + j % 4;
+            w[j] = ok[j / 4] && at <= r.hi && at > r.lo ? w[j] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4 * N; j++)
+        sum[j] += w[j];
+}
+
+// Few rows (16 of a kv head's; more take the loop inside): a wave goes over its tiles of 32 tokens,
+// the next one's keys in flight. Bound by reading the keys.
+template <int D, bool CAP>
+__global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
+{
+    const AttnParams& p = w.a;
     const int lane = threadIdx.x & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned unit = blockIdx.x;
-    const int t0 = (int)(unit % blocks) * 128 + 32 * wave;
-    unit /= blocks;
+    const unsigned units = p.seqs * p.kv_heads;
+    const int part = blockIdx.x / units;
+    const unsigned unit = blockIdx.x - part * units;
     const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
     const Sequence seq(p, b);
-    if (t0 >= width)
-        return;
-    float sum[8] = {};
+    const Mx4Page<D> lay(1 << p.log2p);
+    const int* table = p.table + b * p.s_table;
     const int rows = seq.n * p.group;
-    if (t0 < seq.len) {
-        const Mx4Page<D> lay(1 << p.log2p);
-        KeyCodes<D> k[2];
-        bool ok[2];
+    const int begin = part * w.chunk + 32 * wave, end = min((part + 1) * w.chunk, w.width);
+    const int last = min(end, seq.len); // of the tokens that have keys
+    WeightRows<D> r;
+    auto load_rows = [&](int x0) {
+        const int x = x0 + (lane & 15);
+        RowCursor(p, seq, kv_head, x, 0, g * (D / 4)).load(p, r, x < rows);
+    };
+    if (rows > 0)
+        load_rows(0);
+    KeyCodes<D> k[2], ahead[2];
+    bool ok[2], ok_ahead[2];
+    auto load_keys = [&](int t0) {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const Sixteen x =
-                locate<D>(p, lay, p.table + b * p.s_table, kv_head, t0 + 16 * s, seq.len);
-            k[s].load(x, lay, lane);
-            ok[s] = x.ok;
+            const Sixteen x = locate<D>(p, lay, table, kv_head, t0 + 16 * s, last);
+            ahead[s].load(x, lay, lane);
+            ok_ahead[s] = x.ok;
         }
-        v4i kop[2][D / 32];
+    };
+    if (begin < last)
+        load_keys(begin);
+    for (int t0 = begin; t0 < end; t0 += 128) {
+        float sum[8] = {};
+        if (t0 < last) {
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+            for (int s = 0; s < 2; s++) {
+                k[s] = ahead[s];
+                ok[s] = ok_ahead[s];
+            }
+            load_keys(t0 + 128); // past the end: the last tokens again, not used
+            v4i kop[2][D / 32];
 #pragma unroll
-            for (int i = 0; i < D / 32; i++)
-                kop[s][i] = k[s].operand(i);
-        // the rows that see some of the tokens: positions t0 .. t0 + 31 + window - 1
-        const int pos0 = seq.len - seq.n;
-        const int i0 = p.causal ? max(t0 - pos0, 0) : 0;
-        const long long last = p.window ? (long long)t0 + 31 + p.window - 1 - pos0 : seq.n - 1;
-        const int r_end = (int)min((long long)rows, (min(last, (long long)seq.n) + 1) * p.group);
-        for (int r = i0 * p.group; r < r_end; r += 16) {
-            const Block blk(p, seq, r, 16);
-            const Row row(p, seq, blk, kv_head, lane & 15);
-            v4i q[D / 32];
-            load_q<D>(p, row, g, q);
-            const float lse2 = row.real ? p.lse[row.at * p.sl_row + row.head] * kLog2e : 0.0f;
-            const bool whole = t0 > blk.lo_max && t0 + 31 <= blk.hi_min && ok[0] && ok[1] &&
-                               blk.count == 16;
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                v4f s = (v4f){0, 0, 0, 0};
+            for (int s = 0; s < 2; s++)
 #pragma unroll
                 for (int i = 0; i < D / 32; i++)
-                    s = mfma_bf16_16x16x32(kop[half][i], q[i], s);
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int t = t0 + 16 * half + 4 * g + u;
-                    const float w = exp2_of(score_log2<CAP>(p, s[u]) - lse2);
-                    if (whole || (ok[half] && t <= row.hi && t > row.lo))
-                        sum[4 * half + u] += w;
-                }
+                    kop[s][i] = k[s].operand(i);
+            for (int x0 = 0; x0 < rows; x0 += 16) {
+                if (rows > 16)
+                    load_rows(x0);
+                const bool sees = ok[0] && ok[1] && t0 + 31 <= r.hi && t0 > r.lo;
+                const bool whole = __builtin_amdgcn_ballot_w64(!sees) == 0;
+                add_weights<D, 2, CAP>(p, kop, r, whole, ok, t0 + 4 * g, sum);
             }
         }
+        const float x = own_sum<8>(sum, lane);
+        if ((lane & 15) < 8)
+            w.store(seq, b, kv_head, t0 + own_token(lane), x);
     }
+}
+
+// Many rows: a workgroup's four waves hold 64 tokens each, their keys as operands, and go over
+// the rows together, 32 at a time through LDS, loaded while the 32 before
+// are computed; workgroups along the rows leave their sums in the workspace, which
+// mx4_weights_join_kernel adds in their order. Bound by the exponentials (a quarter of
+// the rate of other vector instructions, together as long as the product) and the product. The rows
+// shared through LDS are what carries it: with every wave reading rows of its own the L1
+// bound it, at twice the time with half the tokens a wave. Prompts of 2048 and 8192 tokens
+// (32 heads over 8, D = 128): 55 and 440 us.
+//
+// A row's 16-byte pieces lie in LDS at their number xor (row % 8), so that eight rows' reads of a
+// piece meet different banks.
+constexpr int kWeightRows = 32, kWeightTokens = 256;
+
+template <int D, bool CAP>
+__global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
+{
+    constexpr int N = 4, kPieces = D / 8; // 16-byte pieces of a row
+    constexpr int kPass = 256 / kPieces;  // rows copied by one load of each thread
+    __shared__ v4i rows_q[2][kWeightRows][kPieces];
+    __shared__ float rows_lse[2][kWeightRows];
+    __shared__ int rows_hi[2][kWeightRows], rows_lo[2][kWeightRows];
+    const AttnParams& p = w.a;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (sequence, kv head) innermost: the workgroups that read the same rows are apart by a multiple
+    // of 8 where there are as many, on one XCD
+    const unsigned units = p.seqs * p.kv_heads;
+    unsigned part = blockIdx.x / units;
+    const unsigned unit = blockIdx.x - part * units;
+    const int split = part % w.splits;
+    part /= w.splits;
+    const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
+    const Sequence seq(p, b);
+    const int first = part * kWeightTokens; // of the workgroup's tokens
+    const int t0 = first + 64 * wave;
+    float sum[4 * N] = {};
+    // the queries that see some of the tokens: positions first .. first + 255 + window - 1
+    const int pos0 = seq.len - seq.n;
+    const int i0 = p.causal ? max(first - pos0, 0) : 0;
+    const long long far =
+        p.window ? (long long)first + kWeightTokens - 1 + p.window - 1 - pos0 : seq.n - 1;
+    const long long see = (min((long long)seq.n, far + 1)) * p.group; // end of their rows
+    const int x_begin = max(i0 * p.group, split * w.chunk);
+    const int x_end = (int)min(see, split == w.splits - 1 ? see : (long long)(split + 1) * w.chunk);
+    if (first < seq.len && x_begin < x_end) {
+        const Mx4Page<D> lay(1 << p.log2p);
+        v4i kop[N][D / 32];
+        bool ok[N], all_ok = true;
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+        for (int s = 0; s < N; s++) {
+            const Sixteen x =
+                locate<D>(p, lay, p.table + b * p.s_table, kv_head, t0 + 16 * s, seq.len);
+            load_keys_in_order<D>(x, lay, lane, kop[s]);
+            ok[s] = x.ok;
+            all_ok &= x.ok;
+        }
+        // a thread carries piece tid % kPieces of row tid / kPieces of each kPass; the first
+        // 32 threads the rest of a row each
+        constexpr int kLoads = kWeightRows / kPass;
+        const int my_row = tid / kPieces, my_piece = tid % kPieces;
+        RowCursor copy[kLoads];
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1)
-            sum[j] += __shfl_xor(sum[j], o, 64);
-    // lane 16*g + j (j < 8) stores token 16 * (j / 4) + 4 * g + j % 4
-    const int j = lane & 15;
-    float x = sum[0];
+        for (int j = 0; j < kLoads; j++)
+            copy[j] = RowCursor(p, seq, kv_head, x_begin + j * kPass + my_row, kWeightRows,
+                                8 * my_piece);
+        RowCursor rest(p, seq, kv_head, x_begin + (tid & 31), kWeightRows, 0);
+        v4i held[kLoads];
+        auto fetch = [&](int x0, float& lse, int& hi, int& lo) {
 #pragma unroll
-    for (int i = 1; i < 8; i++)
-        x = j == i ? sum[i] : x;
-    const int t = t0 + 16 * (j / 4) + 4 * g + j % 4;
-    if (j < 8 && t < width) {
-        const float old =
-            w_in && t < seq.len ? w_in[b * si_seq + kv_head * si_head + t] : 0.0f;
-        w_out[b * so_seq + kv_head * so_head + t] = t < seq.len ? old + x : 0.0f;
+            for (int j = 0; j < kLoads; j++) {
+                const bool real = x0 + j * kPass + my_row < x_end;
+                held[j] = *(const v4i*)(p.q + (real ? copy[j].q : copy[j].q0));
+                copy[j].advance();
+            }
+            const bool real = x0 + (tid & 31) < x_end;
+            lse = p.lse[real ? rest.lse : rest.lse0];
+            hi = real ? min(rest.hi, rest.top) : -1;
+            lo = rest.lo;
+            rest.advance();
+        };
+        auto publish = [&](int buf, float lse, int hi, int lo) {
+#pragma unroll
+            for (int j = 0; j < kLoads; j++) {
+                const int r = j * kPass + my_row;
+                rows_q[buf][r][my_piece ^ (r & 7)] = held[j];
+            }
+            if (tid < kWeightRows) {
+                rows_lse[buf][tid] = lse * kLog2e;
+                rows_hi[buf][tid] = hi;
+                rows_lo[buf][tid] = lo;
+            }
+        };
+        float lse;
+        int hi, lo, buf = 0;
+        fetch(x_begin, lse, hi, lo);
+        publish(0, lse, hi, lo);
+        __syncthreads();
+        for (int x0 = x_begin; x0 < x_end; x0 += kWeightRows, buf ^= 1) {
+            const bool more = x0 + kWeightRows < x_end;
+            if (more)
+                fetch(x0 + kWeightRows, lse, hi, lo);
+#pragma unroll
+            for (int half = 0; half < kWeightRows; half += 16) {
+                const int r = half + (lane & 15);
+                WeightRows<D> rows;
+#pragma unroll
+                for (int m = 0; m < D / 32; m++)
+                    rows.q[m] = rows_q[buf][r][(4 * m + g) ^ (r & 7)];
+                rows.lse2 = rows_lse[buf][r];
+                rows.hi = rows_hi[buf][r];
+                rows.lo = rows_lo[buf][r];
+                const bool sees = all_ok && t0 + 63 <= rows.hi && t0 > rows.lo;
+                const bool whole = __builtin_amdgcn_ballot_w64(!sees) == 0;
+                add_weights<D, N, CAP>(p, kop, rows, whole, ok, t0 + 4 * g, sum);
+            }
+            if (more)
+                publish(buf ^ 1, lse, hi, lo);
+            __syncthreads();
+        }
     }
+    const float x = own_sum<4 * N>(sum, lane);
+    const int t = t0 + own_token(lane);
+    if (w.splits == 1)
+        w.store(seq, b, kv_head, t, x);
+    else if (t < w.width)
+        w.ws[((size_t)split * units + unit) * w.width + t] = x;
+}
+
+__global__ __launch_bounds__(256) void mx4_weights_join_kernel(WeightsParams w)
+{
+    const AttnParams& p = w.a;
+    const unsigned units = p.seqs * p.kv_heads;
+    const unsigned part = blockIdx.x / units, unit = blockIdx.x - part * units;
+    const int t = part * 256 + threadIdx.x;
+    if (t >= w.width)
+        return;
+    const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
+    const float* x = w.ws + (size_t)unit * w.width + t;
+    const size_t step = (size_t)units * w.width;
+    float sum = 0.0f;
+    for (int s0 = 0; s0 < w.splits; s0 += 8) { // eight loads at a time, added in their order
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            y[i] = s0 + i < w.splits ? x[(s0 + i) * step] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            sum += y[i];
+    }
+    w.store(Sequence(p, b), b, kv_head, t, sum);
 }
 
 // ---- host -------------------------------------------------------------------------------
@@ -887,6 +1192,43 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
     return r;
 }
 
+struct WeightsPlan {
+    bool few;
+    int chunk, splits;
+    long long grid;
+    size_t ws_bytes;
+};
+
+// Few rows: tokens in chunks of a multiple of 128, up to 8 workgroups a CU. Many: rows in
+// chunks of a multiple of 32, at least 128, for up to 6 workgroups a CU (a prompt of 8192 tokens,
+// 32 heads over 8: 440 us; with 4 a CU 645, with 8 490, as half of them see nothing).
+static WeightsPlan weights_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a, int width,
+                                int num_cu)
+{
+    WeightsPlan r{};
+    const long long units = (long long)a.seqs * c.kv_heads;
+    const long long max_q = a.q_starts ? std::min(std::max(a.max_q, 1), std::max(a.rows, 1)) : 1;
+    const long long rows = max_q * (a.heads / c.kv_heads);
+    r.few = rows <= 16;
+    r.splits = 1;
+    if (r.few) {
+        const long long most = std::max<long long>(1, 8ll * num_cu / units);
+        r.chunk = (int)(((width + most - 1) / most + 127) / 128 * 128);
+        r.grid = units * (((long long)width + r.chunk - 1) / r.chunk);
+        return r;
+    }
+    const long long blocks = ((long long)width + kWeightTokens - 1) / kWeightTokens;
+    const long long most = std::max<long long>(1, 6ll * num_cu / (units * blocks));
+    r.chunk = (int)std::min<long long>(((rows + most - 1) / most + kWeightRows - 1) / kWeightRows *
+                                           kWeightRows, 1 << 30);
+    r.chunk = std::max(r.chunk, 128);
+    r.splits = (int)((rows + r.chunk - 1) / r.chunk);
+    r.grid = units * blocks * r.splits;
+    if (r.splits > 1)
+        r.ws_bytes = (size_t)r.splits * units * width * 4;
+    return r;
+}
+
 template <int D, bool CAP>
 static void launch_rows(const AttnParams& p, const RowsPlan& r, unsigned grid, hipStream_t s)
 {
@@ -986,11 +1328,31 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
     return GA_OK;
 }
 
+ga_status ga_mx4_attention_weights_workspace_bytes(const ga_mx4_cache* cache,
+                                                   const ga_mx4_attention_args* args, int width,
+                                                   size_t* bytes)
+{
+    if (!bytes)
+        return fail(GA_ERR_ARG, "mx4 attention weights: null pointer");
+    if (const ga_status st = attention_check(cache, args, false))
+        return st;
+    if (width < 0)
+        return fail(GA_ERR_ARG, "mx4 attention weights: negative width");
+    *bytes = 0;
+    if (args->seqs == 0 || width == 0)
+        return GA_OK;
+    int num_cu = 0;
+    if (const ga_status st = device_cu_count(&num_cu))
+        return st;
+    *bytes = weights_plan(*cache, *args, width, num_cu).ws_bytes;
+    return GA_OK;
+}
+
 ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_attention_args* args,
                                    const float* w_in, long long stride_in_seq,
                                    long long stride_in_head, float* w_out,
                                    long long stride_out_seq, long long stride_out_head, int width,
-                                   void* stream)
+                                   void* workspace, size_t workspace_bytes, void* stream)
 {
     if (const ga_status st = attention_check(cache, args, true))
         return st;
@@ -1001,17 +1363,36 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
         return GA_OK;
     if (!w_out || !a.lens || (a.rows && !a.lse))
         return fail(GA_ERR_ARG, "mx4 attention weights: null pointer");
-    const long long blocks = ((long long)width + 127) / 128;
-    const long long grid = (long long)a.seqs * cache->kv_heads * blocks;
-    if (grid > 0x7FFFFFFFll)
+    int num_cu = 0;
+    if (const ga_status st = device_cu_count(&num_cu))
+        return st;
+    const WeightsPlan r = weights_plan(*cache, a, width, num_cu);
+    if (r.ws_bytes && (!workspace || workspace_bytes < r.ws_bytes))
+        return fail(GA_ERR_WORKSPACE, "mx4 attention weights: workspace holds %zu bytes, need %zu",
+                    workspace ? workspace_bytes : (size_t)0, r.ws_bytes);
+    if ((uintptr_t)workspace % 4)
+        return fail(GA_ERR_ARG, "mx4 attention weights: workspace must be 4-byte aligned");
+    if (r.grid > 0x7FFFFFFFll)
         return fail(GA_ERR_SHAPE, "mx4 attention weights: too many sequences for one call");
-    const AttnParams p = params_of(*cache, a);
+    const WeightsParams w{params_of(*cache, a), w_in,    w_out,    stride_in_seq,
+                          stride_in_head,       stride_out_seq, stride_out_head,
+                          width,                r.chunk, r.splits, (float*)workspace};
+    hipStream_t st = (hipStream_t)stream;
     with_dim_cap(cache->head_dim, a.softcap > 0.0f, [&](auto dim, auto cap) {
-        hipLaunchKernelGGL((mx4_weights_kernel<decltype(dim)::value, decltype(cap)::value>),
-                           dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, p, w_in,
-                           stride_in_seq, stride_in_head, w_out, stride_out_seq, stride_out_head,
-                           width, (int)blocks);
+        constexpr int D = decltype(dim)::value;
+        constexpr bool CAP = decltype(cap)::value;
+        if (r.few)
+            hipLaunchKernelGGL((mx4_weights_few_kernel<D, CAP>), dim3((unsigned)r.grid), dim3(256),
+                               0, st, w);
+        else
+            hipLaunchKernelGGL((mx4_weights_many_kernel<D, CAP>), dim3((unsigned)r.grid), dim3(256),
+                               0, st, w);
     });
+    if (r.splits > 1)
+        hipLaunchKernelGGL(mx4_weights_join_kernel,
+                           dim3((unsigned)((long long)a.seqs * cache->kv_heads *
+                                           (((long long)width + 255) / 256))),
+                           dim3(256), 0, st, w);
     GA_HIP_CHECK(hipGetLastError());
     return GA_OK;
 }

@@ -88,6 +88,14 @@ def _check(x, what, dtype, shape, device):
     return strides
 
 
+def _scratch(workspace, device):
+    if workspace is None:
+        return None, 0
+    if workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous on the cache's GPU")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _on(stream):
     """Allocations belong to the stream that the call runs on."""
     if stream is None:
@@ -195,11 +203,7 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
     sl = _check(lse, "lse", torch.float32, q.shape[:2], device)
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     a.stride_out_row, a.stride_out_head, a.stride_lse_row = so[0], so[1], sl[0]
-    ptr, size = None, 0
-    if workspace is not None:
-        if workspace.get_device() != device:
-            raise ValueError("workspace is on %s, not on the cache's GPU" % workspace.device)
-        ptr, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ptr, size = _scratch(workspace, device)
     check(lib().ga_mx4_attention(c, a, ptr, size, _stream_handle(stream)))
     return out, lse
 
@@ -221,7 +225,7 @@ def _weights(x, what, seqs, heads, device):
 
 def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, max_q=None,
                       max_len=None, scale=None, causal=True, window=0, softcap=0.0, width=None,
-                      out=None, stream=None):
+                      out=None, workspace=None, stream=None):
     """weights [sequences, kv heads, tokens] float32 (None: zeros) plus what the rows
     q give to each cached token: the sum of exp(score - lse) over the rows that see it
     and the query heads of the kv head. q, lse and the rest as of the attention()
@@ -235,17 +239,23 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
     if weights is not None:
         sw = _weights(weights, "weights", a.seqs, c.kv_heads, device)
         ptr = weights.data_ptr()
-    if out is None:
-        if width is None:
-            width = a.max_len if weights is None else weights.shape[2]
-        with _on(stream):
-            out = q.new_empty((a.seqs, c.kv_heads, width), dtype=torch.float32)
-    so = _weights(out, "out", a.seqs, c.kv_heads, device)
-    width = out.shape[2]
+    if width is None:
+        width = a.max_len if weights is None else weights.shape[2]
+    if out is not None:
+        width = out.shape[-1]
     if weights is not None and weights.shape[2] < width:
         raise ValueError("weights hold %d tokens, out %d" % (weights.shape[2], width))
+    need = ctypes.c_size_t(0)
+    check(lib().ga_mx4_attention_weights_workspace_bytes(c, a, width, need))
+    with _on(stream):
+        if out is None:
+            out = q.new_empty((a.seqs, c.kv_heads, width), dtype=torch.float32)
+        if workspace is None and need.value:
+            workspace = q.new_empty(need.value, dtype=torch.uint8)
+    so = _weights(out, "out", a.seqs, c.kv_heads, device)
+    ws, size = _scratch(workspace, device)
     check(lib().ga_mx4_attention_weights(c, a, ptr, sw[0], sw[1], out.data_ptr(), so[0], so[1],
-                                         width, _stream_handle(stream)))
+                                         width, ws, size, _stream_handle(stream)))
     return out
 
 

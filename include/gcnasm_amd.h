@@ -666,12 +666,16 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
  * in elements. Zero from the sequence's length on; tokens past `width` are left
  * out. w_in NULL counts as zeros, and may be w_out with the same strides. args: those
  * of the attention; lse is read, out is not looked at. Sums run in a fixed
- * order. */
+ * order. workspace: device scratch of the bytes that the call before says (0: none),
+ * as for ga_mx4_attention. */
+ga_status ga_mx4_attention_weights_workspace_bytes(const ga_mx4_cache* cache,
+                                                   const ga_mx4_attention_args* args, int width,
+                                                   size_t* bytes);
 ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_attention_args* args,
                                    const float* w_in, long long stride_in_seq,
                                    long long stride_in_head, float* w_out,
                                    long long stride_out_seq, long long stride_out_head, int width,
-                                   void* stream);
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* Eviction: of each sequence longer than `keep` (>= 1), every kv head keeps its last
  * `recent` (0 .. keep) tokens and of the others the keep - recent of largest

@@ -57,7 +57,7 @@ def test_caches_that_are_refused(change, status):
     assert l.ga_mx4_read(r(c), 0x1000, 1, 0x1000, 0x1000, 0, None) == status
     assert l.ga_mx4_attention(r(c), r(a), None, 0, None) == status
     assert l.ga_mx4_attention_workspace_bytes(r(c), r(a), r(need)) == status
-    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, 8, None) == status
+    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, 8, None, 0, None) == status
     assert l.ga_mx4_evict(r(c), r(e), None) == status
 
 
@@ -76,7 +76,7 @@ def test_attention_arguments_that_are_refused(change, status):
     c, a = cache(), attention(**change)
     r = ctypes.byref
     assert l.ga_mx4_attention(r(c), r(a), None, 0, None) == status
-    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, 8, None) == status
+    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, 8, None, 0, None) == status
     assert l.ga_last_error()
 
 
@@ -91,11 +91,14 @@ def test_other_arguments_that_are_refused():
                    dict(stride_out_head=4)):
         assert l.ga_mx4_attention(r(c), r(attention(**change)), None, 0, None) == _lib.GA_ERR_SHAPE
     # weights
-    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, None, 8, 8, 8, None) == _lib.GA_ERR_ARG
+    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, None, 8, 8, 8, None, 0, None) == _lib.GA_ERR_ARG
     assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, -1,
-                                      None) == _lib.GA_ERR_ARG
+                                      None, 0, None) == _lib.GA_ERR_ARG
     assert l.ga_mx4_attention_weights(r(c), r(attention(lse=None)), None, 0, 0, 0x1000, 8, 8, 8,
-                                      None) == _lib.GA_ERR_ARG
+                                      None, 0, None) == _lib.GA_ERR_ARG
+    assert l.ga_mx4_attention_weights_workspace_bytes(r(c), r(a), 8, None) == _lib.GA_ERR_ARG
+    assert l.ga_mx4_attention_weights_workspace_bytes(r(c), r(a), -1, ctypes.byref(
+        ctypes.c_size_t())) == _lib.GA_ERR_ARG
     # append and read
     ok = [r(c), 0x1000, 0x1000, 0, 1, 256, 128, 256, 128, 0x1000, 0, None]
     for at, bad, status in ((1, None, 1), (2, None, 1), (9, None, 1), (3, 2, 1), (4, -1, 1),
@@ -148,4 +151,4 @@ def test_nothing_to_do_is_no_error():
         assert l.ga_mx4_attention(r(c), r(attention(q=None, **kw)), None, 0, None) == 0
         assert l.ga_mx4_attention_workspace_bytes(r(c), r(attention(**kw)), r(need)) == 0
         assert need.value == 0
-    assert l.ga_mx4_attention_weights(r(c), r(attention()), None, 0, 0, None, 8, 8, 0, None) == 0
+    assert l.ga_mx4_attention_weights(r(c), r(attention()), None, 0, 0, None, 8, 8, 0, None, 0, None) == 0
