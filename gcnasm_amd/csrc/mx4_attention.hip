@@ -1,111 +1,12 @@
 // mx4_attention.hip -- attention over the MXFP4 key/value cache, and the weights it gives
 // to the cached tokens (layout and operand order: ga_mx4_cache.hpp).
-//
-// For row i (position len - n + i) of a sequence and the tokens t that it sees:
-//   x_t = scale q.k_t  (or softcap tanh(scale q.k_t / softcap)),  in powers of two:
-//   m = max x_t,  l = sum 2^(x_t - m),  out = sum 2^(x_t - m) v_t / l,  lse = (m + log2 l) ln 2
-// kept as running values over the tokens, so the scores are never stored.
 #include "ga_device.hpp"
 #include "ga_internal.hpp"
-#include "ga_mx4_cache.hpp"
+#include "ga_mx4_attention.hpp"
 
 #include <algorithm>
 
 namespace ga {
-
-typedef float v2f __attribute__((ext_vector_type(2)));
-typedef __bf16 v2bf16 __attribute__((ext_vector_type(2)));
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-struct AttnParams {
-    const uint16_t* q;
-    uint16_t* out;
-    float* lse;
-    const int *table, *lens, *q_starts;
-    const uint8_t* pages;
-    long long num_pages, stride_page;
-    long long sq_row, sq_head, so_row, so_head, sl_row, s_table;
-    int seqs, rows, heads, kv_heads, group, table_pages, log2p;
-    int causal, window;
-    float to_log2; // scores to powers of two: scale * log2(e), or softcap * log2(e)
-    float to_cap;  // scale / softcap
-    int row_blocks; // workgroups along a sequence's rows; each takes every row_blocks-th block
-    int splits, chunk; // workgroups along the tokens, tokens of each
-    float* ws;         // [splits][rows][heads] {m, l}, then [splits][rows][heads][D]
-};
-
-__host__ __device__ inline size_t stats_floats(int splits, int rows, int heads)
-{
-    return ((size_t)splits * rows * heads * 2 + 3) / 4 * 4;
-}
-
-// A sequence's rows and tokens; whatever the tables hold, inside the operands.
-struct Sequence {
-    int q0, n, len;
-    __device__ __forceinline__ Sequence(const AttnParams& p, int b)
-    {
-        q0 = b;
-        n = 1;
-        if (p.q_starts) {
-            q0 = min(max(p.q_starts[b], 0), p.rows);
-            n = min(max(p.q_starts[b + 1] - q0, 0), p.rows - q0);
-        }
-        const long long cap = (long long)p.table_pages << p.log2p;
-        len = (int)min((long long)max(p.lens[b], 0), min(cap, 0x7FFFFF00ll));
-    }
-};
-
-// Rows r0 .. r0 + count - 1 of a sequence's n * group (row r: query r / group, head
-// r % group) and what they see: tokens in (lo, hi] of each row, and over all.
-struct Block {
-    int r0, count;
-    int hi_min, hi_max, lo_min, lo_max;
-    __device__ __forceinline__ Block(const AttnParams& p, const Sequence& s, int first, int most)
-    {
-        r0 = first;
-        count = min(most, s.n * p.group - first);
-        const int i0 = first / p.group, i1 = (first + count - 1) / p.group;
-        hi_min = p.causal ? min(s.len - s.n + i0, s.len - 1) : s.len - 1;
-        hi_max = p.causal ? min(s.len - s.n + i1, s.len - 1) : s.len - 1;
-        lo_min = p.window ? max(s.len - s.n + i0 - p.window, -1) : -1;
-        lo_max = p.window ? max(s.len - s.n + i1 - p.window, -1) : -1;
-    }
-    // the tokens that some row sees: [begin, end), begin a multiple of 64
-    __device__ __forceinline__ int begin() const { return (lo_min + 1) & ~63; }
-    __device__ __forceinline__ int end() const { return hi_max + 1; }
-};
-
-struct Row {
-    bool real;
-    int head;      // query head
-    long long at;  // row of q and out
-    int hi, lo;    // sees tokens in (lo, hi]
-    __device__ __forceinline__ Row(const AttnParams& p, const Sequence& s, const Block& blk,
-                                   int kv_head, int r)
-    {
-        real = r < blk.count;
-        const int x = real ? blk.r0 + r : blk.r0;
-        const int i = x / p.group;
-        head = kv_head * p.group + (x - i * p.group);
-        at = s.q0 + i;
-        hi = !real ? -1 : (p.causal ? min(s.len - s.n + i, s.len - 1) : s.len - 1);
-        lo = p.window ? s.len - s.n + i - p.window : -1;
-    }
-};
-
-template <bool CAP>
-__device__ __forceinline__ float score_log2(const AttnParams& p, float qk)
-{
-    return CAP ? tanhf(qk * p.to_cap) * p.to_log2 : qk * p.to_log2;
-}
-
-__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
-{
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf16));
-}
 
 // A row's D elements as the second operand of D/32 products: lane 16*g + r the
 // elements g*D/4 .. (g+1)*D/4 - 1 of row r.
@@ -254,13 +155,6 @@ __device__ __forceinline__ void value_operands(const ValueCodes<D> (&v)[2], v4i&
     }
 }
 
-// Nonzero if one of a dword's four scale bytes is 253 or more: its values may pass bf16
-// (4 * 2^126), or are NaN.
-__device__ __forceinline__ uint32_t any_huge(uint32_t w)
-{
-    return ((w & 0x7F7F7F7Fu) + 0x03030303u) & w & 0x80808080u;
-}
-
 // 32 tokens of one kv head as a wave holds them.
 template <int D>
 struct Tile {
@@ -304,10 +198,6 @@ __device__ __forceinline__ void scores16(const KeyCodes<D>& k, const v4i (&q)[RT
 // until the waves' results are joined. The tokens are split over the waves and over
 // p.splits workgroups, whose results mx4_join_kernel joins.
 //
-// The running maximum is raised only when a score passes it by 2^8: until
-// then probabilities up to 2^8 stand in the same sums, which fp32 holds as exactly,
-// and neither the exchange between lanes nor the rescaling is needed.
-//
 // Probabilities enter the second product as two bf16 terms (16 bits of
 // significand together): one alone would add as much error as the output's own
 // rounding to bf16, and the matrix cores wait for memory here anyway.
@@ -318,7 +208,6 @@ __device__ __forceinline__ void scores16(const KeyCodes<D>& k, const v4i (&q)[RT
 // The scheduling barriers keep the operands of one product live at a time: without
 // them and with the rare path below inside the loop the registers left room for 2
 // waves a SIMD instead of 3 (134 us of 64 x 8192, 143 of 4 x 131072).
-constexpr float kRaise = 8.0f;
 
 // What the sums lack: the tokens with a scale byte of 253 or more, whose values
 // pass bf16 or are NaN. In a product 0 * infinity would reach rows that do not
@@ -1147,9 +1036,13 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
     return p;
 }
 
-// How a call is cut. Row blocks of 16 rows while a sequence has no more, else of
-// 32 (D = 256: always 16, two blocks' sums do not fit the registers). Tokens in
-// chunks of a multiple of 128, a tile for each of four waves:
+// How a call is cut. A kv head with more than 64 rows in a sequence goes to
+// mx4_prompt.hip (32768 tokens, 32 heads over 8, D = 128: 256 rows of each kv head 80 us
+// there and 86 here, 64 rows 41 and 39; 8 sequences of 8192 with 64 rows 68 and 59),
+// its tokens split for up to two workgroups a CU, at least 256 a split. Here row blocks
+// of 16 rows while a sequence has no more, else of 32 (D = 256: always 16, two
+// blocks' sums do not fit the registers), and tokens in chunks of a multiple of 128, a
+// tile for each of four waves:
 // - Few tokens stay in one workgroup, of eight waves past 128, which saves the
 //   join's launch: 1 x 513 tokens of 8 kv heads (D = 128) 8.6 us against 8.9 split,
 //   and 4 us less on the host; 768 tokens 9.5 against 8.9; D = 256 already at 300
@@ -1160,7 +1053,8 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 // - Many usually differ in length, and smaller chunks even that out: 64 sequences of
 //   2048 to 8192 tokens 97 us with up to 8 a CU, 103 with 4, 102 with 12.
 struct RowsPlan {
-    int tiles; // of 16 rows
+    bool prompt; // mx4_prompt.hip
+    int tiles;   // else: of 16 rows
     int waves;
     int row_blocks, splits, chunk;
     size_t ws_floats;
@@ -1172,19 +1066,28 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
     const int group = a.heads / c.kv_heads;
     const long long max_q = a.q_starts ? std::min<long long>(std::max(a.max_q, 1), a.rows) : 1;
     const long long rows = max_q * group;
+    r.prompt = rows > 64;
     r.tiles = rows <= 16 || c.head_dim == 256 ? 1 : 2;
-    r.row_blocks = (int)((rows + 16 * r.tiles - 1) / (16 * r.tiles));
+    const int block = r.prompt ? mx4_prompt_rows(c.head_dim) : 16 * r.tiles;
+    r.row_blocks = (int)((rows + block - 1) / block);
     long long span = std::min<long long>(a.max_len, (long long)a.table_pages * c.page_size);
     if (a.window > 0) // a row block's rows and the alignment of its first token
-        span = std::min<long long>(span, (long long)a.window + 16 * r.tiles / group + 64);
+        span = std::min<long long>(span, (long long)a.window + block / group + 64);
     span = std::max<long long>(span, 1);
     const long long units = (long long)a.seqs * c.kv_heads * r.row_blocks;
-    const int resident = c.head_dim == 64 ? 4 : (c.head_dim == 128 ? 3 : 2);
-    const bool one = r.tiles == 1 && units < 2 * num_cu && span * c.head_dim <= 640 * 128;
-    r.waves = one && span > 128 ? 8 : 4;
-    const long long most = one ? 1 : (long long)(units < num_cu ? resident : 8) * num_cu / units;
-    const long long want = std::max<long long>(1, most);
-    r.chunk = (int)(((span + want - 1) / want + 127) / 128 * 128);
+    if (r.prompt) {
+        const long long want = std::max<long long>(1, 2ll * num_cu / units);
+        r.chunk = (int)std::max<long long>((span + want - 1) / want, 256);
+        r.chunk = (r.chunk + 63) / 64 * 64;
+    } else {
+        const int resident = c.head_dim == 64 ? 4 : (c.head_dim == 128 ? 3 : 2);
+        const bool one = r.tiles == 1 && units < 2 * num_cu && span * c.head_dim <= 640 * 128;
+        r.waves = one && span > 128 ? 8 : 4;
+        const long long most =
+            one ? 1 : (long long)(units < num_cu ? resident : 8) * num_cu / units;
+        const long long want = std::max<long long>(1, most);
+        r.chunk = (int)(((span + want - 1) / want + 127) / 128 * 128);
+    }
     r.splits = (int)((span + r.chunk - 1) / r.chunk);
     if (r.splits > 1)
         r.ws_floats = stats_floats(r.splits, a.rows, a.heads) +
@@ -1316,7 +1219,10 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
     hipStream_t st = (hipStream_t)stream;
     with_dim_cap(cache->head_dim, a.softcap > 0.0f, [&](auto dim, auto cap) {
         constexpr int D = decltype(dim)::value;
-        launch_rows<D, decltype(cap)::value>(p, r, (unsigned)grid, st);
+        if (r.prompt)
+            launch_mx4_prompt(p, D, decltype(cap)::value, st);
+        else
+            launch_rows<D, decltype(cap)::value>(p, r, (unsigned)grid, st);
         const long long joins = (long long)a.rows * a.heads;
         if (r.splits > 4)
             hipLaunchKernelGGL((mx4_join_kernel<D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
