@@ -5,6 +5,8 @@
 #include "ga_mx4_cache.hpp"
 #include "ga_quant.hpp"
 
+#include <algorithm>
+
 namespace ga {
 
 struct CacheView {
@@ -108,7 +110,8 @@ __global__ __launch_bounds__(256) void mx4_append_kernel(
 }
 
 // ---- read back ---------------------------------------------------------------------
-// Eight elements of a token's key and value per lane; bound by the bytes written.
+// Eight elements of a token's key and value per lane; bound by the bytes written (8191 tokens of
+// 8 heads, D = 128, as bf16: 10 us).
 template <int D>
 __device__ __forceinline__ uint32_t value_codes8(const uint8_t* page, Mx4Page<D> lay, uint32_t t,
                                                  uint32_t d)
@@ -122,20 +125,36 @@ __device__ __forceinline__ uint32_t value_codes8(const uint8_t* page, Mx4Page<D>
         return *(const uint32_t*)(page + lay.v_quad(t / 4, d / kPer) + u + d % kPer / 2);
 }
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+// The converter's results are exact while neither code 0.5 nor 6 leaves the normal range; scale
+// bytes outside 2 .. 252 take fp4_value.
 template <int OUT>
 __device__ __forceinline__ void store_values8(void* dst, size_t at, uint32_t w, uint32_t scale)
 {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-        x[j] = fp4_value(w >> (4 * j) & 15u, scale);
+    const bool usual = scale - 2u <= 250u;
+    const float sc = __uint_as_float(scale << 23);
     if constexpr (OUT == GA_DTYPE_BF16) {
-        v4i o;
+        v4i o = fp4_oct_bf16(w, sc);
+        if (!usual) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            o[j] = (int)(f32_to_bf16(x[2 * j]) | (uint32_t)f32_to_bf16(x[2 * j + 1]) << 16);
+            for (int j = 0; j < 4; j++)
+                o[j] = (int)(f32_to_bf16(fp4_value(w >> (8 * j) & 15u, scale)) |
+                             (uint32_t)f32_to_bf16(fp4_value(w >> (8 * j + 4) & 15u, scale)) << 16);
+        }
         *(v4i*)((uint16_t*)dst + at) = o;
     } else {
+        float x[8];
+        static_for<4>([&](auto j) {
+            const v2f y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, j);
+            x[2 * j] = y[0];
+            x[2 * j + 1] = y[1];
+        });
+        if (!usual) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                x[j] = fp4_value(w >> (4 * j) & 15u, scale);
+        }
         *(v4f*)((float*)dst + at) = (v4f){x[0], x[1], x[2], x[3]};
         *(v4f*)((float*)dst + at + 4) = (v4f){x[4], x[5], x[6], x[7]};
     }
@@ -194,18 +213,26 @@ __device__ __forceinline__ uint32_t weight_key(float x)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The weight of a key (a zero without its sign, a NaN without its payload).
+__device__ __forceinline__ float key_weight(uint32_t key)
+{
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
 
 // One workgroup per sequence and kv head. The (keep - recent)-th largest key is
 // found by its digits (11, 11 and 10 bits, a histogram each), then every wave
-// goes over a stretch of the weights twice: once to count what is above
-// the key and equal to it, once to write the indices at the place that the
-// stretches before it leave. No atomics on anything but the histograms' counts,
-// so the result does not depend on an order. Five passes over weights that the first
-// one brings into the L2.
+// goes over its stretch of the weights twice: once to count what is above the key and
+// equal to it, once to write the indices at the place that the stretches before it
+// leave. No atomics on anything but the histograms' counts, so the result does
+// not depend on an order. Bound by latency: a lane keeps its keys in registers, up to
+// KEYS of them (65536 tokens), so that the weights are loaded once, all at the same time;
+// longer sequences (KEYS 0) read them from the L2 in each of the five passes.
+template <int KEYS>
 __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
 {
-    __shared__ int hist[kSelBins];
+    __shared__ v4i hist[kSelBins]; // four counts of a bin, of every fourth lane each
     __shared__ int wave_sum[kSelWaves], wave_gt[kSelWaves], wave_eq[kSelWaves];
     __shared__ int found_bin, found_left;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -236,6 +263,38 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
     }
     if (want == 0)
         return;
+    // each wave's stretch of the tokens: lane's are lo + lane, 64 apart
+    const int rows = (old + kSelThreads - 1) / kSelThreads;
+    const int lo = min(old, wave * rows * 64), hi = min(old, lo + rows * 64);
+    uint32_t held[KEYS ? KEYS : 1];
+    auto key_of = [&](int i) { // 0, which no weight has, past the stretch's end
+        const int j = lo + 64 * i + lane;
+        const uint32_t key = weight_key(w[j < hi ? j : 0]);
+        return j < hi ? key : 0u;
+    };
+    if constexpr (KEYS > 0) {
+        // a branch for 16 of them: loads under a branch are waited for inside it
+        constexpr int kGroup = KEYS < 16 ? KEYS : 16;
+#pragma unroll
+        for (int i0 = 0; i0 < KEYS; i0 += kGroup)
+            if (i0 < rows) {
+#pragma unroll
+                for (int i = i0; i < i0 + kGroup; i++)
+                    held[i] = key_of(i);
+            }
+    }
+    // f(token of the lane, its key) in the tokens' order
+    auto each = [&](auto&& f) {
+        if constexpr (KEYS > 0) {
+#pragma unroll
+            for (int i = 0; i < KEYS; i++)
+                if (i < rows) // a register's number has to be known: no loop over them
+                    f(lo + 64 * i + lane, held[i]);
+        } else {
+            for (int i = 0; i < rows; i++)
+                f(lo + 64 * i + lane, key_of(i));
+        }
+    };
     uint32_t key_at = 0;
     int left = want; // of the keys that share key_at's digits so far
     for (int pass = 0; pass < 3; pass++) {
@@ -243,17 +302,17 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
         const int bits = pass == 2 ? 10 : 11;
         const uint32_t fixed = pass == 0 ? 0u : ~0u << (shift + bits);
         for (int j = tid; j < kSelBins; j += kSelThreads)
-            hist[j] = 0;
+            hist[j] = (v4i){0, 0, 0, 0};
         __syncthreads();
-        for (int j = tid; j < old; j += kSelThreads) {
-            const uint32_t key = weight_key(w[j]);
-            if (((key ^ key_at) & fixed) == 0)
-                atomicAdd(&hist[key >> shift & ((1u << bits) - 1u)], 1);
-        }
+        each([&](int, uint32_t key) {
+            if (key != 0 && ((key ^ key_at) & fixed) == 0)
+                atomicAdd((int*)&hist[key >> shift & ((1u << bits) - 1u)] + (lane & 3), 1);
+        });
         __syncthreads();
-        // thread i holds bins hi = 2047 - 2i and hi - 1: keys above come first
-        const int hi = kSelBins - 1 - 2 * tid;
-        const int n1 = hist[hi], n0 = hist[hi - 1];
+        // thread i holds bins top = 2047 - 2i and top - 1: keys above come first
+        const int top = kSelBins - 1 - 2 * tid;
+        const v4i h1 = hist[top], h0 = hist[top - 1];
+        const int n1 = h1[0] + h1[1] + h1[2] + h1[3], n0 = h0[0] + h0[1] + h0[2] + h0[3];
         int sum = n1 + n0;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -263,28 +322,23 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
         if (lane == 63)
             wave_sum[wave] = sum;
         __syncthreads();
-        int before = sum - n1 - n0; // keys in bins above hi
+        int before = sum - n1 - n0; // keys in bins above top
         for (int i = 0; i < wave; i++)
             before += wave_sum[i];
         if (before < left && left <= before + n1 + n0) {
             const bool upper = left <= before + n1;
-            found_bin = upper ? hi : hi - 1;
+            found_bin = upper ? top : top - 1;
             found_left = left - (upper ? before : before + n1);
         }
         __syncthreads();
         key_at |= (uint32_t)found_bin << shift;
         left = found_left;
     }
-    // each wave's stretch of the tokens
-    const int per = (old + kSelThreads - 1) / kSelThreads * 64;
-    const int lo = min(old, wave * per), hi = min(old, lo + per);
     int gt = 0, eq = 0;
-    for (int j = lo; j < hi; j += 64) {
-        const uint32_t key = j + lane < hi ? weight_key(w[j + lane]) : 0u;
-        const bool in = j + lane < hi;
-        gt += __popcll(__builtin_amdgcn_ballot_w64(in && key > key_at));
-        eq += __popcll(__builtin_amdgcn_ballot_w64(in && key == key_at));
-    }
+    each([&](int, uint32_t key) {
+        gt += __popcll(__builtin_amdgcn_ballot_w64(key > key_at));
+        eq += __popcll(__builtin_amdgcn_ballot_w64(key == key_at));
+    });
     if (lane == 0) {
         wave_gt[wave] = gt;
         wave_eq[wave] = eq;
@@ -297,36 +351,34 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
     }
     int at = at_gt + min(at_eq, left);
     const uint64_t below = (1ull << lane) - 1ull;
-    for (int j = lo; j < hi; j += 64) {
-        const bool in = j + lane < hi;
-        const float x = in ? w[j + lane] : 0.0f;
-        const uint32_t key = weight_key(x);
-        const uint64_t eqs = __builtin_amdgcn_ballot_w64(in && key == key_at);
-        const bool stays = in && (key > key_at ||
-                                  (key == key_at && at_eq + __popcll(eqs & below) < left));
+    each([&](int j, uint32_t key) {
+        const uint64_t eqs = __builtin_amdgcn_ballot_w64(key == key_at);
+        const bool stays =
+            key > key_at || (key == key_at && at_eq + __popcll(eqs & below) < left);
         const uint64_t stay = __builtin_amdgcn_ballot_w64(stays);
         if (stays) {
             const int to = at + __popcll(stay & below);
-            kept[to] = j + lane;
-            nw[to] = x;
+            kept[to] = j;
+            nw[to] = key_weight(key);
         }
         at_eq += __popcll(eqs);
         at += __popcll(stay);
-    }
+    });
 }
 
 // ---- eviction: moving them ---------------------------------------------------------------
 // A workgroup moves 64 kept tokens of one head, at their new places in whole
-// quads of four, so that each lane writes a value's piece of four tokens at once;
-// the reads are as scattered as the kept tokens are. Bound by bytes.
+// quads of four, so that a lane writes a value's pieces of four tokens, or their scales, at
+// once; the reads are as scattered as the kept tokens are, and of a value's line only a
+// quarter is its own. Bound by bytes.
 constexpr int kMoveTokens = 64;
 
 template <int D>
 __global__ __launch_bounds__(256) void mx4_move_kernel(EvictArgs e, int blocks)
 {
-    constexpr int kPiece = D / 32; // code bytes of a token's value under one i
+    constexpr int kPiece = D / 32; // code bytes of a token's value under one i; scale bytes of a token
     __shared__ const uint8_t* src_page[kMoveTokens];
-    __shared__ uint8_t* dst_page[kMoveTokens];
+    __shared__ uint8_t* dst_page[kMoveTokens / 4]; // of a quad
     __shared__ int src_at[kMoveTokens];
     const Mx4Page<D> lay(e.c.page_size());
     const int unit = blockIdx.x / blocks, first = (blockIdx.x - unit * blocks) * kMoveTokens;
@@ -338,58 +390,97 @@ __global__ __launch_bounds__(256) void mx4_move_kernel(EvictArgs e, int blocks)
     if (threadIdx.x < kMoveTokens) {
         const int i = threadIdx.x;
         const uint8_t* sp = nullptr;
-        uint8_t* dp = nullptr;
         int at = 0;
         if (i < n) {
             const int t = e.a.kept[(size_t)unit * e.a.keep + first + i];
-            const int j = (first + i) >> e.c.log2p;
-            const long long to = j < e.a.dst_pages ? e.a.dst_table[b * e.a.stride_dst_table + j]
-                                                   : -1;
             const long long from = e.a.table[b * e.a.stride_table + (t >> e.c.log2p)];
-            if (e.c.in_cache(from) && e.c.in_cache(to)) {
+            if (e.c.in_cache(from))
                 sp = e.c.page(from, head, lay.bytes());
-                dp = e.c.page(to, head, lay.bytes());
-                at = t & mask;
-            }
+            at = t & mask;
         }
         src_page[i] = sp;
-        dst_page[i] = dp;
         src_at[i] = at;
+        if (i % 4 == 0) {
+            const int j = (first + i) >> e.c.log2p;
+            const long long to =
+                i < n && j < e.a.dst_pages ? e.a.dst_table[b * e.a.stride_dst_table + j] : -1;
+            dst_page[i / 4] = e.c.in_cache(to) ? e.c.page(to, head, lay.bytes()) : nullptr;
+        }
     }
     __syncthreads();
-    // keys: 16 bytes a lane
+    // keys: 16 bytes a lane, then their scales; a token without a source becomes zeros
     for (int x = threadIdx.x; x < kMoveTokens * (D / 32); x += 256) {
         const int i = x / (D / 32), o = x % (D / 32) * 16;
+        uint8_t* dst = dst_page[i / 4];
+        if (!dst || i >= n)
+            continue;
+        v4i w = (v4i){0, 0, 0, 0};
         if (src_page[i])
-            *(v4i*)(dst_page[i] + lay.k_row((first + i) & mask) + o) =
-                *(const v4i*)(src_page[i] + lay.k_row(src_at[i]) + o);
+            w = *(const v4i*)(src_page[i] + lay.k_row(src_at[i]) + o);
+        *(v4i*)(dst + lay.k_row((first + i) & mask) + o) = w;
     }
-    // values: the four tokens of a quad, each kPiece bytes
+    // values: the four tokens of a quad (those past the last become zeros)
     for (int x = threadIdx.x; x < kMoveTokens / 4 * 16; x += 256) {
         const int quad = x / 16, i = x % 16;
+        uint8_t* dst = dst_page[quad];
+        if (!dst)
+            continue;
+        dst += lay.v_quad(((first + 4 * quad) & mask) / 4, i);
+        uint32_t w[4 * kPiece / 4] = {};
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int j = quad * 4 + u, to = (first + j) & mask;
+            const int j = quad * 4 + u;
             if (!src_page[j])
                 continue;
             const uint8_t* s = src_page[j] + lay.v_quad(src_at[j] / 4, i) + src_at[j] % 4 * kPiece;
-            uint8_t* d = dst_page[j] + lay.v_quad(to / 4, i) + to % 4 * kPiece;
-            if constexpr (kPiece == 2)
-                *(uint16_t*)d = *(const uint16_t*)s;
-            else if constexpr (kPiece == 4)
-                *(uint32_t*)d = *(const uint32_t*)s;
-            else
-                *(uint2*)d = *(const uint2*)s;
+            if constexpr (kPiece == 2) {
+                w[u / 2] |= (uint32_t) * (const uint16_t*)s << (u % 2 * 16);
+            } else if constexpr (kPiece == 4) {
+                w[u] = *(const uint32_t*)s;
+            } else {
+                const uint2 y = *(const uint2*)s;
+                w[2 * u] = y.x;
+                w[2 * u + 1] = y.y;
+            }
+        }
+        if constexpr (kPiece == 2) {
+            *(uint2*)dst = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int o = 0; o < kPiece; o += 4)
+                *(v4i*)(dst + 4 * o) =
+                    (v4i){(int)w[o], (int)w[o + 1], (int)w[o + 2], (int)w[o + 3]};
         }
     }
-    // scales
-    for (int x = threadIdx.x; x < kMoveTokens * kPiece; x += 256) {
-        const int i = x / kPiece, blk = x % kPiece, to = (first + i) & mask;
-        if (!src_page[i])
-            continue;
-        dst_page[i][lay.k_scale(to) + blk] = src_page[i][lay.k_scale(src_at[i]) + blk];
-        dst_page[i][lay.v_scale(to / 4, blk) + to % 4] =
-            src_page[i][lay.v_scale(src_at[i] / 4, blk) + src_at[i] % 4];
+    // scales: of a token's key, and of a block of a quad's values
+    for (int x = threadIdx.x; x < kMoveTokens + kMoveTokens / 4 * kPiece; x += 256) {
+        if (x < kMoveTokens) {
+            uint8_t* dst = dst_page[x / 4];
+            if (!dst || x >= n)
+                continue;
+            dst += lay.k_scale((first + x) & mask);
+            const uint8_t* s = src_page[x] ? src_page[x] + lay.k_scale(src_at[x]) : nullptr;
+            if constexpr (kPiece == 2)
+                *(uint16_t*)dst = s ? *(const uint16_t*)s : 0;
+            else if constexpr (kPiece == 4)
+                *(uint32_t*)dst = s ? *(const uint32_t*)s : 0;
+            else
+                *(uint2*)dst = s ? *(const uint2*)s : make_uint2(0, 0);
+        } else {
+            const int quad = (x - kMoveTokens) / kPiece, blk = (x - kMoveTokens) % kPiece;
+            uint8_t* dst = dst_page[quad];
+            if (!dst)
+                continue;
+            uint32_t w = 0;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int j = quad * 4 + u;
+                if (src_page[j])
+                    w |= (uint32_t)src_page[j][lay.v_scale(src_at[j] / 4, blk) + src_at[j] % 4]
+                         << (8 * u);
+            }
+            *(uint32_t*)(dst + lay.v_scale(((first + 4 * quad) & mask) / 4, blk)) = w;
+        }
     }
 }
 
@@ -528,7 +619,7 @@ ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args,
         return fail(GA_ERR_ARG, "mx4_evict: keep must be positive and recent 0 .. keep");
     if (a.seqs < 0 || a.table_pages < 0 || a.dst_pages < 0 || a.width < 0 || a.new_width < a.keep)
         return fail(GA_ERR_ARG, "mx4_evict: negative size, or new_width below keep");
-    if ((long long)a.dst_pages * cache->page_size < min(a.keep, a.width))
+    if ((long long)a.dst_pages * cache->page_size < std::min(a.keep, a.width))
         return fail(GA_ERR_SHAPE, "mx4_evict: dst_table's pages hold fewer than keep tokens");
     if (a.seqs == 0)
         return GA_OK;
@@ -540,8 +631,17 @@ ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args,
     if (units * blocks > 0x7FFFFFFFll)
         return fail(GA_ERR_SHAPE, "mx4_evict: too many sequences for one call");
     const EvictArgs e{a, view_of(*cache)};
-    hipLaunchKernelGGL(mx4_select_kernel, dim3((unsigned)units), dim3(kSelThreads), 0,
-                       (hipStream_t)stream, e);
+    // the most tokens that may be looked at decide whether a lane can hold its share
+    const long long most = std::min<long long>((long long)a.table_pages * cache->page_size, a.width);
+    if (most <= 8ll * kSelThreads)
+        hipLaunchKernelGGL((mx4_select_kernel<8>), dim3((unsigned)units), dim3(kSelThreads), 0,
+                           (hipStream_t)stream, e);
+    else if (most <= 64ll * kSelThreads)
+        hipLaunchKernelGGL((mx4_select_kernel<64>), dim3((unsigned)units), dim3(kSelThreads), 0,
+                           (hipStream_t)stream, e);
+    else
+        hipLaunchKernelGGL((mx4_select_kernel<0>), dim3((unsigned)units), dim3(kSelThreads), 0,
+                           (hipStream_t)stream, e);
     with_dim(cache->head_dim, [&](auto dim) {
         hipLaunchKernelGGL((mx4_move_kernel<decltype(dim)::value>), dim3((unsigned)(units * blocks)),
                            dim3(256), 0, (hipStream_t)stream, e, blocks);

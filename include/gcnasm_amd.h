@@ -689,8 +689,8 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
  *               zeros behind them
  * The pages of dst_table that a sequence needs (ceil(new_len / P)) must be pages
  * that no table holds for tokens in use, and new_weights and new_lens no part of
- * weights and lens. Kept tokens of a page outside the cache keep whatever the
- * new page held. */
+ * weights and lens. A kept token of a page outside the cache becomes zeros, as do the
+ * places behind the last one up to a multiple of four. */
 typedef struct ga_mx4_evict_args {
     const int* table;
     const int* lens;
