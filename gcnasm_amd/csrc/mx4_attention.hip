@@ -608,17 +608,15 @@ struct WeightsParams {
     int splits;       // workgroups along the rows (many)
     float* ws;        // their sums, [splits][seqs][kv heads][width]
 
+    // the weight so far of token t < len of a sequence
+    __device__ __forceinline__ float before(int b, int head, int t) const
+    {
+        return w_in ? w_in[b * si_seq + head * si_head + t] : 0.0f;
+    }
     __device__ __forceinline__ void store(const Sequence& s, int b, int head, int t, float x) const
     {
-        if (t >= width)
-            return;
-        float y = 0.0f;
-        if (t < s.len) {
-            y = x;
-            if (w_in)
-                y += w_in[b * si_seq + head * si_head + t];
-        }
-        w_out[b * so_seq + head * so_head + t] = y;
+        if (t < width)
+            w_out[b * so_seq + head * so_head + t] = t < s.len ? x + before(b, head, t) : 0.0f;
     }
 };
 
@@ -670,7 +668,6 @@ struct RowCursor {
     long long q_step, q_wrap, lse_step, lse_wrap; // of a step, and if the head wraps besides
     int in, d_in, group;                          // head of the kv head's
     int hi, lo, top, d_hi, wrap_hi, d_lo, wrap_lo;
-    RowCursor() = default;
     __device__ __forceinline__ RowCursor(const AttnParams& p, const Sequence& s, int kv_head, int x,
                                          int step, int offset)
     {
@@ -781,7 +778,9 @@ __global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
         load_rows(0);
     KeyCodes<D> k[2], ahead[2];
     bool ok[2], ok_ahead[2];
+    float old = 0.0f, old_ahead = 0.0f; // weight so far of this lane's token
     auto load_keys = [&](int t0) {
+        old_ahead = w.before(b, kv_head, min(t0 + own_token(lane), last - 1));
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const Sixteen x = locate<D>(p, lay, table, kv_head, t0 + 16 * s, last);
@@ -799,6 +798,7 @@ __global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
                 k[s] = ahead[s];
                 ok[s] = ok_ahead[s];
             }
+            old = old_ahead;
             load_keys(t0 + 128); // past the end: the last tokens again, not used
             v4i kop[2][D / 32];
 #pragma unroll
@@ -815,32 +815,35 @@ __global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
             }
         }
         const float x = own_sum<8>(sum, lane);
-        if ((lane & 15) < 8)
-            w.store(seq, b, kv_head, t0 + own_token(lane), x);
+        const int t = t0 + own_token(lane);
+        if ((lane & 15) < 8 && t < w.width)
+            w.w_out[b * w.so_seq + kv_head * w.so_head + t] = t < seq.len ? old + x : 0.0f;
     }
 }
 
-// Many rows: a workgroup's four waves hold 64 tokens each, their keys as operands, and go over
+// Many rows: a workgroup's four waves hold 32 tokens each, their keys as operands, and go over
 // the rows together, 32 at a time through LDS, loaded while the 32 before
 // are computed; workgroups along the rows leave their sums in the workspace, which
-// mx4_weights_join_kernel adds in their order. Bound by the exponentials (a quarter of
-// the rate of other vector instructions, together as long as the product) and the product. The rows
-// shared through LDS are what carries it: with every wave reading rows of its own the L1
-// bound it, at twice the time with half the tokens a wave. Prompts of 2048 and 8192 tokens
-// (32 heads over 8, D = 128): 55 and 440 us.
+// mx4_weights_join_kernel adds in their order. Bound by issuing the exponentials (a
+// quarter of the rate of other vector instructions, together as long as the product) and the product.
+// Prompts of 2048 and 8192 tokens (32 heads over 8, D = 128): 46 and 403 us. With
+// 64 tokens a wave, whose operands leave room for two waves a SIMD instead of four,
+// 54 and 410; with every wave reading rows of its own, the L1 bound it: 67 and 510.
 //
 // A row's 16-byte pieces lie in LDS at their number xor (row % 8), so that eight rows' reads of a
 // piece meet different banks.
-constexpr int kWeightRows = 32, kWeightTokens = 256;
+constexpr int kWeightRows = 32, kWeightTiles = 2, kWeightTokens = 64 * kWeightTiles;
 
 template <int D, bool CAP>
 __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
 {
-    constexpr int N = 4, kPieces = D / 8; // 16-byte pieces of a row
+    constexpr int N = kWeightTiles;
+    constexpr int kPieces = D / 8;        // 16-byte pieces of a row
     constexpr int kPass = 256 / kPieces;  // rows copied by one load of each thread
     __shared__ v4i rows_q[2][kWeightRows][kPieces];
     __shared__ float rows_lse[2][kWeightRows];
     __shared__ int rows_hi[2][kWeightRows], rows_lo[2][kWeightRows];
+    __shared__ long long rows_at[2][kWeightRows]; // where q has them
     const AttnParams& p = w.a;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -854,7 +857,7 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
     const int kv_head = unit % p.kv_heads, b = unit / p.kv_heads;
     const Sequence seq(p, b);
     const int first = part * kWeightTokens; // of the workgroup's tokens
-    const int t0 = first + 64 * wave;
+    const int t0 = first + 16 * N * wave;
     float sum[4 * N] = {};
     // the queries that see some of the tokens: positions first .. first + 255 + window - 1
     const int pos0 = seq.len - seq.n;
@@ -877,50 +880,50 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
             all_ok &= x.ok;
         }
         // a thread carries piece tid % kPieces of row tid / kPieces of each kPass; the first
-        // 32 threads the rest of a row each
+        // 32 threads know a row each, and say where the others find it, a round before
         constexpr int kLoads = kWeightRows / kPass;
         const int my_row = tid / kPieces, my_piece = tid % kPieces;
-        RowCursor copy[kLoads];
-#pragma unroll
-        for (int j = 0; j < kLoads; j++)
-            copy[j] = RowCursor(p, seq, kv_head, x_begin + j * kPass + my_row, kWeightRows,
-                                8 * my_piece);
-        RowCursor rest(p, seq, kv_head, x_begin + (tid & 31), kWeightRows, 0);
+        const bool teller = tid < kWeightRows;
+        RowCursor at(p, seq, kv_head, x_begin + (tid & (kWeightRows - 1)), kWeightRows, 0);
         v4i held[kLoads];
-        auto fetch = [&](int x0, float& lse, int& hi, int& lo) {
-#pragma unroll
-            for (int j = 0; j < kLoads; j++) {
-                const bool real = x0 + j * kPass + my_row < x_end;
-                held[j] = *(const v4i*)(p.q + (real ? copy[j].q : copy[j].q0));
-                copy[j].advance();
-            }
-            const bool real = x0 + (tid & 31) < x_end;
-            lse = p.lse[real ? rest.lse : rest.lse0];
-            hi = real ? min(rest.hi, rest.top) : -1;
-            lo = rest.lo;
-            rest.advance();
+        float lse;
+        int hi, lo;
+        auto tell = [&](int x0, int buf) {
+            if (teller)
+                rows_at[buf][tid] = x0 + tid < x_end ? at.q : at.q0;
         };
-        auto publish = [&](int buf, float lse, int hi, int lo) {
+        auto fetch = [&](int x0, int buf) {
+#pragma unroll
+            for (int j = 0; j < kLoads; j++)
+                held[j] = *(const v4i*)(p.q + rows_at[buf][j * kPass + my_row] + 8 * my_piece);
+            const bool real = x0 + (tid & (kWeightRows - 1)) < x_end;
+            lse = p.lse[real ? at.lse : at.lse0];
+            hi = real ? min(at.hi, at.top) : -1;
+            lo = at.lo;
+            at.advance();
+        };
+        auto publish = [&](int buf) {
 #pragma unroll
             for (int j = 0; j < kLoads; j++) {
                 const int r = j * kPass + my_row;
                 rows_q[buf][r][my_piece ^ (r & 7)] = held[j];
             }
-            if (tid < kWeightRows) {
+            if (teller) {
                 rows_lse[buf][tid] = lse * kLog2e;
                 rows_hi[buf][tid] = hi;
                 rows_lo[buf][tid] = lo;
             }
         };
-        float lse;
-        int hi, lo, buf = 0;
-        fetch(x_begin, lse, hi, lo);
-        publish(0, lse, hi, lo);
+        int buf = 0;
+        tell(x_begin, 0);
+        __syncthreads();
+        fetch(x_begin, 0);
+        publish(0);
+        tell(x_begin + kWeightRows, 1);
         __syncthreads();
         for (int x0 = x_begin; x0 < x_end; x0 += kWeightRows, buf ^= 1) {
-            const bool more = x0 + kWeightRows < x_end;
-            if (more)
-                fetch(x0 + kWeightRows, lse, hi, lo);
+            // past the end: the sequence's first row, not used
+            fetch(x0 + kWeightRows, buf ^ 1);
 #pragma unroll
             for (int half = 0; half < kWeightRows; half += 16) {
                 const int r = half + (lane & 15);
@@ -931,17 +934,19 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
                 rows.lse2 = rows_lse[buf][r];
                 rows.hi = rows_hi[buf][r];
                 rows.lo = rows_lo[buf][r];
-                const bool sees = all_ok && t0 + 63 <= rows.hi && t0 > rows.lo;
+                const bool sees = all_ok && t0 + 16 * N - 1 <= rows.hi && t0 > rows.lo;
                 const bool whole = __builtin_amdgcn_ballot_w64(!sees) == 0;
                 add_weights<D, N, CAP>(p, kop, rows, whole, ok, t0 + 4 * g, sum);
             }
-            if (more)
-                publish(buf ^ 1, lse, hi, lo);
+            publish(buf ^ 1);
+            tell(x0 + 2 * kWeightRows, buf);
             __syncthreads();
         }
     }
     const float x = own_sum<4 * N>(sum, lane);
     const int t = t0 + own_token(lane);
+    if ((lane & 15) >= 4 * N)
+        return;
     if (w.splits == 1)
         w.store(seq, b, kv_head, t, x);
     else if (t < w.width)
@@ -1102,9 +1107,11 @@ struct WeightsPlan {
     size_t ws_bytes;
 };
 
-// Few rows: tokens in chunks of a multiple of 128, up to 8 workgroups a CU. Many: rows in
-// chunks of a multiple of 32, at least 128, for up to 6 workgroups a CU (a prompt of 8192 tokens,
-// 32 heads over 8: 440 us; with 4 a CU 645, with 8 490, as half of them see nothing).
+// Few rows: tokens in chunks of a multiple of 128, up to 4 workgroups a CU, as many as it
+// holds (32 sequences of 4096: 21 us, 24 with 8). Many: rows in chunks of a multiple of 32, at
+// least 128, for up to 10 workgroups a CU, of which a prompt leaves half with nothing
+// to see (8192 tokens, 32 heads over 8: 403 us, with 4 a CU 532, with 8, whose
+// two chunks of the rows fall together with the halves, 532, with 16 418).
 static WeightsPlan weights_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a, int width,
                                 int num_cu)
 {
@@ -1115,13 +1122,13 @@ static WeightsPlan weights_plan(const ga_mx4_cache& c, const ga_mx4_attention_ar
     r.few = rows <= 16;
     r.splits = 1;
     if (r.few) {
-        const long long most = std::max<long long>(1, 8ll * num_cu / units);
+        const long long most = std::max<long long>(1, 4ll * num_cu / units);
         r.chunk = (int)(((width + most - 1) / most + 127) / 128 * 128);
         r.grid = units * (((long long)width + r.chunk - 1) / r.chunk);
         return r;
     }
     const long long blocks = ((long long)width + kWeightTokens - 1) / kWeightTokens;
-    const long long most = std::max<long long>(1, 6ll * num_cu / (units * blocks));
+    const long long most = std::max<long long>(1, 10ll * num_cu / (units * blocks));
     r.chunk = (int)std::min<long long>(((rows + most - 1) / most + kWeightRows - 1) / kWeightRows *
                                            kWeightRows, 1 << 30);
     r.chunk = std::max(r.chunk, 128);
