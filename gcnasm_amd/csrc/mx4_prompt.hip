@@ -86,24 +86,48 @@ struct PromptThread {
     struct Ids {
         int k, v;
     };
+    // what is left of the ids once the codes are on their way, so that the next ids' loads can
+    // take their registers
+    struct Seen {
+        uint64_t away; // tokens t0 + lane whose page is outside the cache
+        bool v;        // the quads' page is inside
+    };
+    // BIG: pages of 64 tokens or more, so that all 64 are in one and addresses are a scalar
+    // and what stays the same; t0 is a multiple of 64. Past the end: of the last token.
+    template <bool BIG>
     __device__ __forceinline__ Ids ids(const AttnParams& p, const int* table, int t0, int end) const
     {
+        if (BIG)
+            return {table[min(t0, end - 1) >> p.log2p], 0};
         return {table[min(t0 + lane, end - 1) >> p.log2p],
                 table[min(t0 + 4 * quad, end - 1) >> p.log2p]};
     }
-    __device__ __forceinline__ const uint8_t* page(const AttnParams& p, Mx4Page<D> lay, int head,
-                                                   int id) const
-    {
-        const bool ok = id >= 0 && id < p.num_pages;
-        return p.pages + (ok ? id : 0) * p.stride_page + (size_t)head * lay.bytes();
-    }
-    __device__ __forceinline__ void load(const AttnParams& p, Mx4Page<D> lay, int head, int t0,
-                                         Ids id, PromptCodes<D>& c) const
+    // pages: the kv head's bytes of the first page
+    template <bool BIG>
+    __device__ __forceinline__ Seen load(const AttnParams& p, Mx4Page<D> lay, const uint8_t* pages,
+                                         int t0, Ids id, PromptCodes<D>& c) const
     {
         const uint32_t mask = (1u << p.log2p) - 1u;
-        const uint8_t* kp = page(p, lay, head, id.k);
-        const uint32_t t = (uint32_t)(t0 + lane) & mask;
-        const uint8_t* src = kp + lay.k_row(t) + wave * (S::kPer * 4);
+        const uint8_t *kp, *vp;  // the pages of the key and of the values
+        uint32_t in = 0;         // where the 64 tokens start in the page
+        uint32_t t = lane, at = quad; // the key and the quads from there
+        Seen seen;
+        if (BIG) {
+            const int page = __builtin_amdgcn_readfirstlane(id.k);
+            const bool ok = page >= 0 && page < p.num_pages;
+            kp = vp = pages + (ok ? page : 0) * p.stride_page;
+            in = (uint32_t)t0 & mask;
+            seen = {ok ? 0 : ~0ull, ok};
+        } else {
+            const bool ok_k = id.k >= 0 && id.k < p.num_pages;
+            const bool ok_v = id.v >= 0 && id.v < p.num_pages;
+            kp = pages + (ok_k ? id.k : 0) * p.stride_page;
+            vp = pages + (ok_v ? id.v : 0) * p.stride_page;
+            t &= mask;
+            at &= mask / 4;
+            seen = {__builtin_amdgcn_ballot_w64(!ok_k), ok_v};
+        }
+        const uint8_t* src = kp + in * (D / 2) + (lay.k_row(t) + wave * (S::kPer * 4));
         if constexpr (S::kPer == 2) {
             const uint2 x = *(const uint2*)src;
             c.k[0] = x.x;
@@ -117,58 +141,49 @@ struct PromptThread {
                     c.k[4 * j + a] = (uint32_t)x[a];
             }
         }
-        const uint8_t* sc = kp + lay.k_scale(t);
+        const uint8_t* sc = kp + in * (D / 32) + (lay.k_scale(t) + wave * S::kPer / 4);
         if constexpr (S::kPer == 8)
-            c.k_scale = *(const uint16_t*)(sc + 2 * wave);
+            c.k_scale = *(const uint16_t*)sc;
         else
-            c.k_scale = sc[wave * S::kPer / 4];
-        const uint8_t* vp = page(p, lay, head, id.v);
+            c.k_scale = *sc;
+        const uint8_t* vs = vp + in * (D / 2) + lay.v_quad(at, i);
+        const uint8_t* vsc = vp + in * (D / 32) + lay.v_scale(at, i * (D / 16) / 32);
 #pragma unroll
         for (int q = 0; q < 2; q++) { // quads quad and quad + 2 are of the same 16 tokens
-            const uint32_t at = ((uint32_t)(t0 + 4 * quad) & mask) / 4 + 2 * q;
-            const uint8_t* vs = vp + lay.v_quad(at, i);
             if constexpr (D == 64) {
-                const uint2 x = *(const uint2*)vs;
+                const uint2 x = *(const uint2*)(vs + 4 * D * q);
                 c.v[q][0] = x.x;
                 c.v[q][1] = x.y;
             } else if constexpr (D == 128) {
-                const v4i x = *(const v4i*)vs;
+                const v4i x = *(const v4i*)(vs + 4 * D * q);
 #pragma unroll
                 for (int a = 0; a < 4; a++)
                     c.v[q][a] = (uint32_t)x[a];
             } else {
 #pragma unroll
                 for (int a = 0; a < 4; a++)
-                    c.v[q][a] = *(const uint32_t*)(vs + 8 * a + 4 * part);
+                    c.v[q][a] = *(const uint32_t*)(vs + 4 * D * q + 8 * a + 4 * part);
             }
-            c.v_scale[q] = *(const uint32_t*)(vp + lay.v_scale(at, i * (D / 16) / 32));
+            c.v_scale[q] = *(const uint32_t*)(vsc + D / 4 * q);
         }
+        return seen;
     }
-    // codes -> operands in LDS; t0, id: as they were loaded
-    __device__ __forceinline__ void turn(const AttnParams& p, PromptLds<D>& lds, int buf, int t0,
-                                         int end, Ids id, PromptCodes<D>& c) const
+    // codes -> operands in LDS; t0, seen: as they were loaded
+    __device__ __forceinline__ void turn(PromptLds<D>& lds, int buf, int t0, int end, Seen seen,
+                                         PromptCodes<D>& c) const
     {
 #pragma unroll
         for (int j = 0; j < S::kPer; j++)
             lds.k[buf][wave * S::kPer + j][lane] =
                 fp4_oct_bf16(c.k[j], j >= 4 ? e8m0_of<1>(c.k_scale) : e8m0_of<0>(c.k_scale));
-        const bool ok = id.v >= 0 && id.v < p.num_pages;
-        const int t = t0 + 4 * quad;
-        if (!ok || t + 12 > end) { // tokens that no row sees: scales that make finite values
+        if (t0 + 64 > end || seen.away) { // tokens that no row sees: scales that make finite values
+            const int t = t0 + 4 * quad;
 #pragma unroll
             for (int q = 0; q < 2; q++) {
-                const int left = ok ? min(max(end - t - 8 * q, 0), 4) : 0;
+                const int left = seen.v ? min(max(end - t - 8 * q, 0), 4) : 0;
                 c.v_scale[q] &= left == 4 ? ~0u : (1u << (8 * left)) - 1u;
             }
         }
-        uint32_t x[2][4];
-#pragma unroll
-        for (int q = 0; q < 2; q++)
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                x[q][u] = D == 64 ? c.v[q][u / 2] >> (8 * part + 16 * (u % 2))
-                                  : (D == 128 ? c.v[q][u % S::kWords] >> (16 * part)
-                                              : c.v[q][u % S::kWords]);
         if (any_huge(c.v_scale[0]) | any_huge(c.v_scale[1])) {
             // values past bf16, or NaN: left to the end
             lds.left_out = 1;
@@ -178,15 +193,28 @@ struct PromptThread {
                 for (int u = 0; u < 4; u++)
                     if ((c.v_scale[q] >> (8 * u) & 0xFFu) >= 253u) {
                         c.v_scale[q] &= ~(0xFFu << (8 * u));
-                        x[q][u] = 0;
+                        c.v[q][D == 64 ? u / 2 : u] &= D == 64 ? 0xFFFFu << (16 - u % 2 * 16) : 0;
                     }
         }
+        if (D == 256 || part == 0)
+            turn_values<0>(lds, buf, c);
+        else
+            turn_values<D == 256 ? 0 : 1>(lds, buf, c);
+    }
+    // PART: which half of the bytes in the words
+    template <int PART>
+    __device__ __forceinline__ void turn_values(PromptLds<D>& lds, int buf,
+                                                const PromptCodes<D>& c) const
+    {
         static_for<S::kBytes>([&](auto byte) {
             constexpr int B = decltype(byte)::value;
             uint32_t y[2][4];
-            static_for<4>([&](auto u) {
-                y[0][u] = fp4_pair_bf16<B>(x[0][u], e8m0_of<u>(c.v_scale[0]));
-                y[1][u] = fp4_pair_bf16<B>(x[1][u], e8m0_of<u>(c.v_scale[1]));
+            static_for<4>([&](auto token) {
+                constexpr int U = decltype(token)::value;
+                constexpr int W = D == 64 ? U / 2 : U;
+                constexpr int AT = D == 64 ? U % 2 * 2 + PART : (D == 128 ? 2 * PART + B : B);
+                y[0][U] = fp4_pair_bf16<AT>(c.v[0][W], e8m0_of<U>(c.v_scale[0]));
+                y[1][U] = fp4_pair_bf16<AT>(c.v[1][W], e8m0_of<U>(c.v_scale[1]));
             });
             v4i even, odd;
 #pragma unroll
@@ -265,7 +293,8 @@ __device__ __forceinline__ void add_left_out(const AttnParams& p, Mx4Page<D> lay
     }
 }
 
-template <int D, bool CAP>
+// BIG: pages of 64 tokens or more.
+template <int D, bool CAP, bool BIG>
 __global__ __launch_bounds__(64 * PromptShape<D>::kWaves, D == 256 ? 1 : (D == 64 ? 3 : 2))
 void mx4_prompt_kernel(AttnParams p)
 {
@@ -313,8 +342,8 @@ void mx4_prompt_kernel(AttnParams p)
             lds.left_out = 0;
         __syncthreads();
 
-        // id: the page of token t0 + lane
-        auto step = [&](int t0, int buf, int id) {
+        // away: the tokens from t0 on in pages outside the cache, which are hidden too
+        auto step = [&](int t0, int buf, uint64_t away) {
             // operands are read kDepth products ahead: left to itself the compiler reads each
             // one right before its product and waits
             constexpr int kDepth = 4;
@@ -341,9 +370,7 @@ void mx4_prompt_kernel(AttnParams p)
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            // tokens in pages outside the cache are hidden too
-            const uint64_t away = __builtin_amdgcn_ballot_w64(id < 0 || id >= p.num_pages);
-            const bool whole = t0 > mine.lo_max && t0 + 63 <= mine.hi_min && away == 0;
+            const bool whole = t0 > mine.lo_max && t0 + 63 <= mine.hi_min && (BIG || away == 0);
             if (CAP || !whole) {
 #pragma unroll
                 for (int half = 0; half < 2; half++)
@@ -360,7 +387,7 @@ void mx4_prompt_kernel(AttnParams p)
                         const int at = 32 * half + 8 * (r / 4) + r % 4; // + 4 * h
                         s[half][r] = at > hi || at <= lo ? -INFINITY : s[half][r];
                     }
-                if (away) {
+                if (!BIG && away) {
 #pragma unroll
                     for (int half = 0; half < 2; half++) {
                         const uint32_t w = (uint32_t)(away >> (32 * half)) >> (4 * h);
@@ -440,28 +467,32 @@ void mx4_prompt_kernel(AttnParams p)
         };
 
         if (begin < end) {
+            // Past the end the last tokens are read again and turned into zeros that no row
+            // sees: under a branch the loads' registers are copied where it ends, and the copies
+            // wait for the loads.
             PromptCodes<D> codes;
-            typename PromptThread<D>::Ids id = me.ids(p, table, begin, end);
-            me.load(p, lay, kv_head, begin, id, codes);
-            me.turn(p, lds, 0, begin, end, id, codes);
-            int now = id.k;
-            id = me.ids(p, table, begin + 64, end);
-            me.load(p, lay, kv_head, begin + 64, id, codes);
-            auto id_next = me.ids(p, table, begin + 128, end);
+            const uint8_t* pages = p.pages + (size_t)kv_head * lay.bytes();
+            auto ids = [&](int t0) { return me.template ids<BIG>(p, table, t0, end); };
+            auto load = [&](int t0, typename PromptThread<D>::Ids id) {
+                return me.template load<BIG>(p, lay, pages, t0, id, codes);
+            };
+            auto id = ids(begin);
+            auto seen = load(begin, id);
+            me.turn(lds, 0, begin, end, seen, codes);
+            uint64_t next_away = seen.away;
+            id = ids(begin + 64);
+            seen = load(begin + 64, id);
+            id = ids(begin + 128);
             __syncthreads();
             int buf = 0;
             for (int t0 = begin; t0 < end; t0 += 64, buf ^= 1) {
-                const int of_tile = now;
-                if (t0 + 64 < end) {
-                    me.turn(p, lds, buf ^ 1, t0 + 64, end, id, codes);
-                    now = id.k;
-                    // past the end: the last tokens again, not used
-                    id = id_next;
-                    me.load(p, lay, kv_head, t0 + 128, id, codes);
-                    id_next = me.ids(p, table, t0 + 192, end);
-                }
-                if (busy && t0 <= mine.hi_max && t0 + 63 > mine.lo_min)
-                    step(t0, buf, of_tile);
+                me.turn(lds, buf ^ 1, t0 + 64, end, seen, codes);
+                const uint64_t away = next_away;
+                next_away = seen.away;
+                seen = load(t0 + 128, id);
+                id = ids(t0 + 192);
+                if (busy && t0 <= mine.hi_max && t0 + 63 > mine.lo_min && !(BIG && away))
+                    step(t0, buf, away);
                 barrier_lds();
             }
             if (lds.left_out) // the operands are not read any more
@@ -511,8 +542,8 @@ int mx4_prompt_rows(int head_dim)
                           : (head_dim == 128 ? PromptShape<128>::kRows : PromptShape<256>::kRows);
 }
 
-template <int D>
-static void launch_prompt(AttnParams p, bool capped, hipStream_t stream)
+template <int D, bool CAP>
+static void launch_prompt(AttnParams p, hipStream_t stream)
 {
     // the kernel takes the maximum before the scale: its sign goes to the queries
     if (p.to_log2 < 0.0f) {
@@ -521,20 +552,20 @@ static void launch_prompt(AttnParams p, bool capped, hipStream_t stream)
     }
     const dim3 grid((unsigned)((long long)p.seqs * p.kv_heads * p.row_blocks * p.splits));
     const dim3 block(64 * PromptShape<D>::kWaves);
-    if (capped)
-        hipLaunchKernelGGL((mx4_prompt_kernel<D, true>), grid, block, 0, stream, p);
+    if (p.log2p >= 6)
+        hipLaunchKernelGGL((mx4_prompt_kernel<D, CAP, true>), grid, block, 0, stream, p);
     else
-        hipLaunchKernelGGL((mx4_prompt_kernel<D, false>), grid, block, 0, stream, p);
+        hipLaunchKernelGGL((mx4_prompt_kernel<D, CAP, false>), grid, block, 0, stream, p);
 }
 
 void launch_mx4_prompt(const AttnParams& p, int head_dim, bool capped, hipStream_t stream)
 {
     if (head_dim == 64)
-        launch_prompt<64>(p, capped, stream);
+        capped ? launch_prompt<64, true>(p, stream) : launch_prompt<64, false>(p, stream);
     else if (head_dim == 128)
-        launch_prompt<128>(p, capped, stream);
+        capped ? launch_prompt<128, true>(p, stream) : launch_prompt<128, false>(p, stream);
     else
-        launch_prompt<256>(p, capped, stream);
+        capped ? launch_prompt<256, true>(p, stream) : launch_prompt<256, false>(p, stream);
 }
 
 } // namespace ga
