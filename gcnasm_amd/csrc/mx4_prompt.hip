@@ -16,10 +16,11 @@ __device__ __forceinline__ v16f mfma_bf16_32x32x16(v4i a, v4i b, v16f c)
 }
 
 // Probabilities enter the second product in bf16, and where one is more than kShare of its
-// lane's sum so far a second bf16 term follows: there its rounding would show in the
-// output beside the output's own, elsewhere the many roundings even out. Always
-// a second term would make the second product twice as long.
-constexpr float kShare = 1.0f / 32;
+// lane's sum so far a second bf16 term follows: there its rounding, up to 2^-8 of it, would show
+// in the output beside the output's own, elsewhere the many roundings even out (of 16 equal
+// ones to a tenth of 2^-8). Always a second term would make the second product twice
+// as long; at a 32nd the two measured below are 603 and 637 us.
+constexpr float kShare = 1.0f / 16;
 
 // A wave has 32 rows, a workgroup four waves; both products give a row to a lane pair (l, l + 32):
 //   scores  S[token][row] = K Q^T, 32 tokens x 32 rows a product,
@@ -30,14 +31,16 @@ constexpr float kShare = 1.0f / 32;
 // the products of the 64 before: K as [d/8][token][8], V as [8 tokens][d/2 x parity][8 tokens],
 // which a lane reads 16 bytes at a time, neighbours side by side.
 //
-// Bound by issuing vector instructions: of a wave's 64 tokens at D = 128 about 130 (32 of
-// them exponentials, at a quarter of the rate) make probabilities and 110 operands, beside 32 products of
-// 32 cycles. A prompt of 8192 tokens (32 heads over 8, D = 128) 640 us, 0.86
-// PFLOP/s, where a large bf16 product reaches 1.39; pieces of 500 to 1000 rows over up to 8191 tokens
-// (64 heads over 8, D = 64) 685 us. Four waves rather than eight, whose barrier
-// the products of all wait at: 2048 tokens 82 us against 116. Operands read a few
-// products ahead instead of as the compiler places them: 642 against 677 at 8192.
-// D = 64 held to the registers of three waves a SIMD: 685 against 806.
+// Bound by what the chip's power allows more than by any unit: at D = 128 matrix
+// instructions are under way for half of the cycles and vector instructions for half, at
+// 1.7 of 2.4 GHz, and neither fewer exponentials nor fewer operand reads make it faster. A
+// prompt of 8192 tokens (32 heads over 8, D = 128, pages of 64) 571 us, 0.96 PFLOP/s, where a large
+// bf16 product reaches 1.39; pieces of 500 to 1000 rows over up to 8191 tokens (64 heads over 8,
+// D = 64, pages of 16) 609 us. Tried beside it: eight waves, whose barrier the products of all
+// wait at (2048 tokens 82 us with four, 116 with eight); operands read as the compiler places
+// them and not a few products ahead (677 us where that took 642); their turning between the products, a
+// piece each (593, 616); D = 64 without the limit of registers that holds three waves a
+// SIMD (806 us where that took 685).
 template <int D>
 struct PromptShape {
     static constexpr int kWaves = 4;
