@@ -604,7 +604,7 @@ struct WeightsParams {
     const float* w_in;
     float* w_out;
     long long si_seq, si_head, so_seq, so_head;
-    int width, chunk; // chunk: tokens of a workgroup (few rows), or rows (many)
+    int width, chunk; // chunk: tokens of a workgroup (few rows)
     int splits;       // workgroups along the rows (many)
     float* ws;        // their sums, [splits][seqs][kv heads][width]
 
@@ -826,13 +826,14 @@ __global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
 // are computed; workgroups along the rows leave their sums in the workspace, which
 // mx4_weights_join_kernel adds in their order. Bound by issuing the exponentials (a
 // quarter of the rate of other vector instructions, together as long as the product) and the product.
-// Prompts of 2048 and 8192 tokens (32 heads over 8, D = 128): 46 and 403 us. With
-// 64 tokens a wave, whose operands leave room for two waves a SIMD instead of four,
-// 54 and 410; with every wave reading rows of its own, the L1 bound it: 67 and 510.
+// Prompts of 2048 and 8192 tokens (32 heads over 8, D = 128): 39 and 342 us. Where
+// those took 46 and 403, 64 tokens a wave, whose operands leave room for two waves a SIMD instead
+// of four, took 54 and 410, and every wave reading rows of its own, bound by the L1, 67 and 510.
 //
 // A row's 16-byte pieces lie in LDS at their number xor (row % 8), so that eight rows' reads of a
 // piece meet different banks.
 constexpr int kWeightRows = 32, kWeightTiles = 2, kWeightTokens = 64 * kWeightTiles;
+constexpr int kWeightChunk = 128; // rows of a workgroup, at least
 
 template <int D, bool CAP>
 __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
@@ -865,8 +866,11 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
     const long long far =
         p.window ? (long long)first + kWeightTokens - 1 + p.window - 1 - pos0 : seq.n - 1;
     const long long see = (min((long long)seq.n, far + 1)) * p.group; // end of their rows
-    const int x_begin = max(i0 * p.group, split * w.chunk);
-    const int x_end = (int)min(see, split == w.splits - 1 ? see : (long long)(split + 1) * w.chunk);
+    const long long x_first = (long long)i0 * p.group;
+    const int even = (int)((see - x_first + w.splits - 1) / w.splits);
+    const int chunk = max((even + kWeightRows - 1) / kWeightRows * kWeightRows, kWeightChunk);
+    const int x_begin = (int)min(see, x_first + (long long)split * chunk);
+    const int x_end = (int)min(see, (long long)x_begin + chunk);
     if (first < seq.len && x_begin < x_end) {
         const Mx4Page<D> lay(1 << p.log2p);
         v4i kop[N][D / 32];
@@ -1108,10 +1112,11 @@ struct WeightsPlan {
 };
 
 // Few rows: tokens in chunks of a multiple of 128, up to 4 workgroups a CU, as many as it
-// holds (32 sequences of 4096: 21 us, 24 with 8). Many: rows in chunks of a multiple of 32, at
-// least 128, for up to 10 workgroups a CU, of which a prompt leaves half with nothing
-// to see (8192 tokens, 32 heads over 8: 403 us, with 4 a CU 532, with 8, whose
-// two chunks of the rows fall together with the halves, 532, with 16 418).
+// holds (32 sequences of 4096: 21 us, 24 with 8). Many: up to 4 workgroups a CU of at least
+// 128 rows each, or up to 8 of 256 (a prompt of 8192 tokens, 32 heads over 8: 342 us, 384 with 4
+// a CU, 339 with 16; of 2048: 39, 40 and 46; of 1024: 19, and 24 with 8 of 128). Each block of
+// tokens divides the rows that see it: divided alike for all, half of a prompt's
+// workgroups have nothing to do and the others differ most (412 and 47 us).
 static WeightsPlan weights_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a, int width,
                                 int num_cu)
 {
@@ -1128,11 +1133,11 @@ static WeightsPlan weights_plan(const ga_mx4_cache& c, const ga_mx4_attention_ar
         return r;
     }
     const long long blocks = ((long long)width + kWeightTokens - 1) / kWeightTokens;
-    const long long most = std::max<long long>(1, 10ll * num_cu / (units * blocks));
-    r.chunk = (int)std::min<long long>(((rows + most - 1) / most + kWeightRows - 1) / kWeightRows *
-                                           kWeightRows, 1 << 30);
-    r.chunk = std::max(r.chunk, 128);
-    r.splits = (int)((rows + r.chunk - 1) / r.chunk);
+    const auto splits = [&](int per_cu, int least) {
+        const long long most = std::max<long long>(1, (long long)per_cu * num_cu / (units * blocks));
+        return (int)std::min<long long>(most, (rows + least - 1) / least);
+    };
+    r.splits = std::max(splits(4, kWeightChunk), splits(8, 2 * kWeightChunk));
     r.grid = units * blocks * r.splits;
     if (r.splits > 1)
         r.ws_bytes = (size_t)r.splits * units * width * 4;
