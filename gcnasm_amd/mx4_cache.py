@@ -96,10 +96,13 @@ def _scratch(workspace, device):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(stream):
     """Allocations belong to the stream that the call runs on."""
     if stream is None:
-        return contextlib.nullcontext()
+        return _HERE
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream)
     return torch.cuda.stream(stream)
@@ -192,15 +195,19 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
                          softcap)
     need = ctypes.c_size_t(0)
     check(lib().ga_mx4_attention_workspace_bytes(c, a, need))
+    heads, dim = a.heads, c.head_dim
+    so, sl = (heads * dim, dim), (heads,)
+    if out is not None:
+        so = _check(out, "out", torch.bfloat16, q.shape, device)
+    if lse is not None:
+        sl = _check(lse, "lse", torch.float32, q.shape[:2], device)
     with _on(stream):
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if lse is None:
-            lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+            lse = q.new_empty((a.rows, heads), dtype=torch.float32)
         if workspace is None and need.value:
             workspace = q.new_empty(need.value, dtype=torch.uint8)
-    so = _check(out, "out", torch.bfloat16, q.shape, device)
-    sl = _check(lse, "lse", torch.float32, q.shape[:2], device)
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     a.stride_out_row, a.stride_out_head, a.stride_lse_row = so[0], so[1], sl[0]
     ptr, size = _scratch(workspace, device)
@@ -247,12 +254,14 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
         raise ValueError("weights hold %d tokens, out %d" % (weights.shape[2], width))
     need = ctypes.c_size_t(0)
     check(lib().ga_mx4_attention_weights_workspace_bytes(c, a, width, need))
+    so = (c.kv_heads * width, width)
+    if out is not None:
+        so = _weights(out, "out", a.seqs, c.kv_heads, device)
     with _on(stream):
         if out is None:
             out = q.new_empty((a.seqs, c.kv_heads, width), dtype=torch.float32)
         if workspace is None and need.value:
             workspace = q.new_empty(need.value, dtype=torch.uint8)
-    so = _weights(out, "out", a.seqs, c.kv_heads, device)
     ws, size = _scratch(workspace, device)
     check(lib().ga_mx4_attention_weights(c, a, ptr, sw[0], sw[1], out.data_ptr(), so[0], so[1],
                                          width, ws, size, _stream_handle(stream)))
@@ -281,15 +290,18 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
     sw = _weights(weights, "weights", seqs, c.kv_heads, device)
     if keep <= 0 or not 0 <= recent <= keep:
         raise ValueError("keep must be positive and recent 0 .. keep")
+    sn, new_width = (c.kv_heads * keep, keep), keep
+    if new_weights is not None:
+        sn = _weights(new_weights, "new_weights", seqs, c.kv_heads, device)
+        new_width = new_weights.shape[2]
     with _on(stream):
         kept = lens.new_empty((seqs, c.kv_heads, keep))
         new_lens = torch.empty_like(lens)
         if new_weights is None:
             new_weights = weights.new_empty((seqs, c.kv_heads, keep))
-    sn = _weights(new_weights, "new_weights", seqs, c.kv_heads, device)
     a = _lib.Mx4EvictArgs(
         table.data_ptr(), lens.data_ptr(), dst_table.data_ptr(), weights.data_ptr(),
         kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(), st[0], sd[0], sw[0], sw[1],
-        sn[0], sn[1], seqs, pages, dst_pages, weights.shape[2], new_weights.shape[2], keep, recent)
+        sn[0], sn[1], seqs, pages, dst_pages, weights.shape[2], new_width, keep, recent)
     check(lib().ga_mx4_evict(c, a, _stream_handle(stream)))
     return kept, new_lens, new_weights
