@@ -28,13 +28,17 @@ struct Sixteen {
     bool ok;
 };
 template <int D>
-__device__ __forceinline__ Sixteen locate(const AttnParams& p, Mx4Page<D> lay, const int* table,
-                                          int head, int t, int end)
+__device__ __forceinline__ Sixteen locate(const AttnParams& p, Mx4Page<D> lay, int head, int t, int id)
 {
-    const int id = table[min(t, end - 1) >> p.log2p];
     const bool ok = id >= 0 && id < p.num_pages;
     return {p.pages + (ok ? id : 0) * p.stride_page + (size_t)head * lay.bytes(),
             (uint32_t)t & ((1u << p.log2p) - 1u), ok};
+}
+template <int D>
+__device__ __forceinline__ Sixteen locate(const AttnParams& p, Mx4Page<D> lay, const int* table,
+                                          int head, int t, int end)
+{
+    return locate<D>(p, lay, head, t, table[min(t, end - 1) >> p.log2p]);
 }
 
 // A lane's codes and scales of 16 tokens' keys (row lane % 16), or values.
@@ -161,12 +165,19 @@ struct Tile {
     KeyCodes<D> k[2];
     ValueCodes<D> v[2];
     bool ok[2];
-    __device__ __forceinline__ void load(const AttnParams& p, Mx4Page<D> lay, const int* table,
-                                         int head, int t0, int end, int lane)
+    // the pages of its halves, in even and odd lanes
+    static __device__ __forceinline__ int ids(const AttnParams& p, const int* table, int t0, int end,
+                                              int lane)
+    {
+        return table[min(t0 + 16 * (lane & 1), end - 1) >> p.log2p];
+    }
+    __device__ __forceinline__ void load(const AttnParams& p, Mx4Page<D> lay, int head, int t0,
+                                         int ids, int lane)
     {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const Sixteen x = locate<D>(p, lay, table, head, t0 + 16 * s, end);
+            const Sixteen x =
+                locate<D>(p, lay, head, t0 + 16 * s, __builtin_amdgcn_readlane(ids, s));
             k[s].load(x, lay, lane);
             v[s].load(x, lay, lane);
             ok[s] = x.ok;
@@ -203,11 +214,14 @@ __device__ __forceinline__ void scores16(const KeyCodes<D>& k, const v4i (&q)[RT
 // rounding to bf16, and the matrix cores wait for memory here anyway.
 //
 // Bound by reading the cache: 4 x 131072 tokens (64 heads over 8, D = 128, 570 MB)
-// 114 us with the join, 5.0 TB/s, where a copy reaches 5.16; 64 sequences of 2048 to 8192
-// tokens (361 MB) 97 us, where every workgroup's first loads and the waves' join show.
-// The scheduling barriers keep the operands of one product live at a time: without
-// them and with the rare path below inside the loop the registers left room for 2
-// waves a SIMD instead of 3 (134 us of 64 x 8192, 143 of 4 x 131072).
+// 113 us with the join, 5.0 TB/s, where a copy reaches 5.16; 64 sequences of 2048 to 8192
+// tokens (361 MB) 85 us, 32 of up to 4096 with 8 kv heads (90 MB) 30, where the first loads, the
+// waves' join and the lengths' differences show. The pages' numbers are read a tile
+// before the codes and those a tile before their use: read where they are needed,
+// each tile waited for its page and the codes before it (100 and 36 us). The scheduling
+// barriers keep the operands of one product live at a time: without them and with the rare
+// path below inside the loop the registers left room for 2 waves a SIMD instead of 3
+// (64 x 8192: 134 us at the time, and 97 with 3).
 
 // What the sums lack: the tokens with a scale byte of 253 or more, whose values
 // pass bf16 or are NaN. In a product 0 * infinity would reach rows that do not
@@ -264,7 +278,8 @@ __device__ __forceinline__ void add_huge(const AttnParams& p, Mx4Page<D> lay, co
 }
 
 template <int D, int RT, bool CAP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void mx4_rows_kernel(AttnParams p)
+__global__ __launch_bounds__(64 * WAVES, (D == 64 ? 5 : (D == 128 ? 4 : 3)) - RT)
+void mx4_rows_kernel(AttnParams p)
 {
     constexpr int NT = D / 16; // output tiles of 16 elements
     constexpr int kRows = 16 * RT;
@@ -403,11 +418,18 @@ __global__ __launch_bounds__(64 * WAVES) void mx4_rows_kernel(AttnParams p)
             });
         };
         if (int t0 = begin + 32 * wave; t0 < end) {
+            // the next tile's codes and the pages of the one after are on their way beside a
+            // tile's work; past the end the last tokens' again, not used
+            constexpr int kStep = 32 * WAVES;
             Tile<D> cur;
-            cur.load(p, lay, table, kv_head, t0, end, lane);
-            for (; t0 < end; t0 += 32 * WAVES) {
-                Tile<D> ahead; // past the end: the last tokens again, not used
-                ahead.load(p, lay, table, kv_head, t0 + 32 * WAVES, end, lane);
+            int ids = Tile<D>::ids(p, table, t0, end, lane);
+            const int next = Tile<D>::ids(p, table, t0 + kStep, end, lane);
+            cur.load(p, lay, kv_head, t0, ids, lane);
+            ids = next;
+            for (; t0 < end; t0 += kStep) {
+                Tile<D> ahead;
+                ahead.load(p, lay, kv_head, t0 + kStep, ids, lane);
+                ids = Tile<D>::ids(p, table, t0 + 2 * kStep, end, lane);
                 step(cur, t0);
                 cur = ahead;
             }
@@ -1053,14 +1075,13 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 // blocks' sums do not fit the registers), and tokens in chunks of a multiple of 128, a
 // tile for each of four waves:
 // - Few tokens stay in one workgroup, of eight waves past 128, which saves the
-//   join's launch: 1 x 513 tokens of 8 kv heads (D = 128) 8.6 us against 8.9 split,
+//   join's launch: 1 x 513 tokens of 8 kv heads (D = 128) 8.7 us against 8.9 split,
 //   and 4 us less on the host; 768 tokens 9.5 against 8.9; D = 256 already at 300
 //   tokens 10.5 against 10.7, at 520 12.4 against 10.9.
-// - Few sequences and heads get as many workgroups as the CUs hold at a time
-//   (4, 3, 2 of D = 64, 128, 256 by registers), so that all end together: 4 x
-//   131072 tokens 114 us, 4 a CU 141, 6 a CU 120.
-// - Many usually differ in length, and smaller chunks even that out: 64 sequences of
-//   2048 to 8192 tokens 97 us with up to 8 a CU, 103 with 4, 102 with 12.
+// - Else up to two workgroups a CU, against 4 and 6 in one run: 64 sequences of 2048 to 8192 tokens
+//   (64 heads over 8) 87 us, 92 and 96; 32 of up to 4096 31, 30 and 33; 16 of 4000 with 4
+//   rows each (32 heads over 8) 23, 28 and 30, with 8 rows (64 heads over 8) 49, 55 and 69; 4 of
+//   131072 121, 127 and 122.
 struct RowsPlan {
     bool prompt; // mx4_prompt.hip
     int tiles;   // else: of 16 rows
@@ -1089,11 +1110,10 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
         r.chunk = (int)std::max<long long>((span + want - 1) / want, 256);
         r.chunk = (r.chunk + 63) / 64 * 64;
     } else {
-        const int resident = c.head_dim == 64 ? 4 : (c.head_dim == 128 ? 3 : 2);
         const bool one = r.tiles == 1 && units < 2 * num_cu && span * c.head_dim <= 640 * 128;
         r.waves = one && span > 128 ? 8 : 4;
         const long long most =
-            one ? 1 : (long long)(units < num_cu ? resident : 8) * num_cu / units;
+            one ? 1 : 2ll * num_cu / units;
         const long long want = std::max<long long>(1, most);
         r.chunk = (int)(((span + want - 1) / want + 127) / 128 * 128);
     }
