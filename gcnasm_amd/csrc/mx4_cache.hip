@@ -35,7 +35,8 @@ static CacheView view_of(const ga_mx4_cache& c)
 // ---- append -----------------------------------------------------------------------
 // A lane quantises EPL elements of a token's key and the same ones of its value,
 // 32 / EPL lanes a block: both loads are in flight before the first maximum is
-// taken. Bound by bytes: the input once, 17/32 of a byte per element out.
+// taken. Bound by bytes: the input once, 17/32 of a byte per element out (8191 tokens of
+// 8 heads, D = 128, from bf16, 42 MB: 12 us).
 template <int D, int EPL>
 __device__ __forceinline__ void store_value_codes(uint8_t* page, Mx4Page<D> lay, uint32_t t,
                                                   uint32_t d, uint32_t w)
@@ -228,7 +229,9 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
 // leave. No atomics on anything but the histograms' counts, so the result does
 // not depend on an order. Bound by latency: a lane keeps its keys in registers, up to
 // KEYS of them (65536 tokens), so that the weights are loaded once, all at the same time;
-// longer sequences (KEYS 0) read them from the L2 in each of the five passes.
+// longer sequences (KEYS 0) read them from the L2 in each of the five passes. One sequence of
+// 5000 tokens (8 heads) 10 us; 16 of 16384 to 32768 31 us, on half of the CUs by then bound by the
+// five passes' instructions (eight counts a bin instead of four: 33).
 template <int KEYS>
 __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
 {
@@ -370,7 +373,8 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
 // A workgroup moves 64 kept tokens of one head, at their new places in whole
 // quads of four, so that a lane writes a value's pieces of four tokens, or their scales, at
 // once; the reads are as scattered as the kept tokens are, and of a value's line only a
-// quarter is its own. Bound by bytes.
+// quarter is its own. Bound by those lines: 16 sequences' 2048 tokens of 8 heads (D = 128) 34 us,
+// 36 MB written and about 130 MB of lines touched.
 constexpr int kMoveTokens = 64;
 
 template <int D>
