@@ -230,8 +230,9 @@ constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
 // not depend on an order. Bound by latency: a lane keeps its keys in registers, up to
 // KEYS of them (65536 tokens), so that the weights are loaded once, all at the same time;
 // longer sequences (KEYS 0) read them from the L2 in each of the five passes. One sequence of
-// 5000 tokens (8 heads) 10 us; 16 of 16384 to 32768 31 us, on half of the CUs by then bound by the
-// five passes' instructions (eight counts a bin instead of four: 33).
+// 5000 tokens (8 heads) 10 us; 16 of 16384 to 32768 26 us, on half of the CUs by then bound by the
+// five passes' instructions (with a branch around each count 31; eight counts a bin instead
+// of four 33).
 template <int KEYS>
 __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
 {
@@ -300,16 +301,19 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
     };
     uint32_t key_at = 0;
     int left = want; // of the keys that share key_at's digits so far
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-        const int bits = pass == 2 ? 10 : 11;
-        const uint32_t fixed = pass == 0 ? 0u : ~0u << (shift + bits);
+    static_for<3>([&](auto digit) {
+        constexpr int kPass = decltype(digit)::value;
+        constexpr int shift = kPass == 0 ? 21 : (kPass == 1 ? 10 : 0);
+        constexpr int bits = kPass == 2 ? 10 : 11;
+        constexpr uint32_t fixed = kPass == 0 ? 0u : ~0u << (shift + bits < 32 ? shift + bits : 0);
         for (int j = tid; j < kSelBins; j += kSelThreads)
             hist[j] = (v4i){0, 0, 0, 0};
         __syncthreads();
+        // without a branch a key, which costs more than to count a 0; the zeros past the
+        // stretch's end are below every key and never reached
         each([&](int, uint32_t key) {
-            if (key != 0 && ((key ^ key_at) & fixed) == 0)
-                atomicAdd((int*)&hist[key >> shift & ((1u << bits) - 1u)] + (lane & 3), 1);
+            atomicAdd((int*)&hist[key >> shift & ((1u << bits) - 1u)] + (lane & 3),
+                      ((key ^ key_at) & fixed) == 0 ? 1 : 0);
         });
         __syncthreads();
         // thread i holds bins top = 2047 - 2i and top - 1: keys above come first
@@ -326,8 +330,9 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
             wave_sum[wave] = sum;
         __syncthreads();
         int before = sum - n1 - n0; // keys in bins above top
-        for (int i = 0; i < wave; i++)
-            before += wave_sum[i];
+#pragma unroll
+        for (int i = 0; i < kSelWaves; i++)
+            before += i < wave ? wave_sum[i] : 0;
         if (before < left && left <= before + n1 + n0) {
             const bool upper = left <= before + n1;
             found_bin = upper ? top : top - 1;
@@ -336,7 +341,7 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
         __syncthreads();
         key_at |= (uint32_t)found_bin << shift;
         left = found_left;
-    }
+    });
     int gt = 0, eq = 0;
     each([&](int, uint32_t key) {
         gt += __popcll(__builtin_amdgcn_ballot_w64(key > key_at));
@@ -348,9 +353,10 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
     }
     __syncthreads();
     int at_gt = 0, at_eq = 0;
-    for (int i = 0; i < wave; i++) {
-        at_gt += wave_gt[i];
-        at_eq += wave_eq[i];
+#pragma unroll
+    for (int i = 0; i < kSelWaves; i++) {
+        at_gt += i < wave ? wave_gt[i] : 0;
+        at_eq += i < wave ? wave_eq[i] : 0;
     }
     int at = at_gt + min(at_eq, left);
     const uint64_t below = (1ull << lane) - 1ull;
