@@ -51,7 +51,17 @@ def new_cache(num_pages, kv_heads, head_dim, page_size=64, device="cuda"):
 
 
 # The checks below run on every call, of which a decode step makes several for each
-# layer: they ask a tensor for as little as they can.
+# layer: they ask a tensor for as little as they can. The current device and its stream come
+# from torch's own functions beneath the public ones where this version has them (0.1 us each
+# instead of 0.3).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(stream, device):
+    if stream is None and _current_stream is not None:
+        return _current_stream(device)
+    return _stream_handle(stream)
 
 
 def _cache(cache, head_dim):
@@ -66,7 +76,7 @@ def _cache(cache, head_dim):
         raise ValueError("the heads of a page must be contiguous (strides %s)"
                          % (tuple(cache.stride()),))
     device = cache.get_device()
-    if device < 0 or device != torch.cuda.current_device():
+    if device < 0 or device != _current_device():
         raise ValueError("the cache is on %s, not on the current GPU" % cache.device)
     return _lib.Mx4Cache(cache.data_ptr(), pages, stride if pages > 1 else heads * size, heads,
                          head_dim, page), device
@@ -130,7 +140,7 @@ def append(cache, k, v, slots, scale_rule=_lib.GA_MX_SCALE_FLOOR_448, stream=Non
     sk = _check(k, "k", k.dtype, shape, device)
     sv = _check(v, "v", k.dtype, shape, device)
     check(lib().ga_mx4_append(c, k.data_ptr(), v.data_ptr(), kind, tokens, sk[0], sk[1], sv[0],
-                              sv[1], slots.data_ptr(), scale_rule, _stream_handle(stream)))
+                              sv[1], slots.data_ptr(), scale_rule, _stream(stream, device)))
 
 
 def read(cache, slots, head_dim, dtype=torch.bfloat16, stream=None):
@@ -146,7 +156,7 @@ def read(cache, slots, head_dim, dtype=torch.bfloat16, stream=None):
         k = cache.new_empty((tokens, c.kv_heads, head_dim), dtype=dtype)
         v = torch.empty_like(k)
     check(lib().ga_mx4_read(c, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(), kind,
-                            _stream_handle(stream)))
+                            _stream(stream, device)))
     return k, v
 
 
@@ -211,7 +221,7 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     a.stride_out_row, a.stride_out_head, a.stride_lse_row = so[0], so[1], sl[0]
     ptr, size = _scratch(workspace, device)
-    check(lib().ga_mx4_attention(c, a, ptr, size, _stream_handle(stream)))
+    check(lib().ga_mx4_attention(c, a, ptr, size, _stream(stream, device)))
     return out, lse
 
 
@@ -264,7 +274,7 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
             workspace = q.new_empty(need.value, dtype=torch.uint8)
     ws, size = _scratch(workspace, device)
     check(lib().ga_mx4_attention_weights(c, a, ptr, sw[0], sw[1], out.data_ptr(), so[0], so[1],
-                                         width, ws, size, _stream_handle(stream)))
+                                         width, ws, size, _stream(stream, device)))
     return out
 
 
@@ -303,5 +313,5 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
         table.data_ptr(), lens.data_ptr(), dst_table.data_ptr(), weights.data_ptr(),
         kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(), st[0], sd[0], sw[0], sw[1],
         sn[0], sn[1], seqs, pages, dst_pages, weights.shape[2], new_width, keep, recent)
-    check(lib().ga_mx4_evict(c, a, _stream_handle(stream)))
+    check(lib().ga_mx4_evict(c, a, _stream(stream, device)))
     return kept, new_lens, new_weights
