@@ -96,7 +96,8 @@ struct PromptThread {
         bool v;        // the quads' page is inside
     };
     // BIG: pages of 64 tokens or more, so that all 64 are in one and addresses are a scalar
-    // and what stays the same; t0 is a multiple of 64. Past the end: of the last token.
+    // and what stays the same; else smaller pages, which start where the 64 do. t0 is a multiple
+    // of 64. Past the end: of the last token.
     template <bool BIG>
     __device__ __forceinline__ Ids ids(const AttnParams& p, const int* table, int t0, int end) const
     {
@@ -296,8 +297,9 @@ __device__ __forceinline__ void add_left_out(const AttnParams& p, Mx4Page<D> lay
     }
 }
 
-// BIG: pages of 64 tokens or more, whose addresses are scalars. The two measured above, with
-// pages of 64: 566 us and without it 575, 582 and 610; D = 256 gains nothing and does without.
+// BIG: pages of 64 tokens or more, which hold a tile whole, so that its address is a scalar. The two
+// measured above with pages of 64: 566 us and as with smaller pages 575, 582 and 610 (D = 256:
+// alike).
 template <int D, bool CAP, bool BIG>
 __global__ __launch_bounds__(64 * PromptShape<D>::kWaves, D == 256 ? 1 : (D == 64 ? 3 : 2))
 void mx4_prompt_kernel(AttnParams p)
@@ -556,13 +558,10 @@ static void launch_prompt(AttnParams p, hipStream_t stream)
     }
     const dim3 grid((unsigned)((long long)p.seqs * p.kv_heads * p.row_blocks * p.splits));
     const dim3 block(64 * PromptShape<D>::kWaves);
-    if constexpr (D < 256) {
-        if (p.log2p >= 6) {
-            hipLaunchKernelGGL((mx4_prompt_kernel<D, CAP, true>), grid, block, 0, stream, p);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((mx4_prompt_kernel<D, CAP, false>), grid, block, 0, stream, p);
+    if (p.log2p >= 6)
+        hipLaunchKernelGGL((mx4_prompt_kernel<D, CAP, true>), grid, block, 0, stream, p);
+    else
+        hipLaunchKernelGGL((mx4_prompt_kernel<D, CAP, false>), grid, block, 0, stream, p);
 }
 
 void launch_mx4_prompt(const AttnParams& p, int head_dim, bool capped, hipStream_t stream)
