@@ -34,7 +34,8 @@ constexpr float kShare = 1.0f / 16;
 // Bound by what the chip's power allows more than by any unit: at D = 128 matrix
 // instructions are under way for half of the cycles and vector instructions for half, at
 // 1.7 of 2.4 GHz, and neither fewer exponentials nor fewer operand reads make it faster. A
-// prompt of 8192 tokens (32 heads over 8, D = 128, pages of 64) 591 us, 0.93 PFLOP/s, where a large
+// prompt of 8192 tokens (32 heads over 8, D = 128, pages of 64) 566 to 596 us
+// from card to card, 0.92 to 0.97 PFLOP/s, where a large
 // bf16 product reaches 1.39; pieces of 500 to 1000 rows over up to 8191 tokens (64 heads over 8,
 // D = 64, pages of 16) 609 us. Tried beside it: eight waves, whose barrier the products of all
 // wait at (2048 tokens 82 us with four, 116 with eight); operands read as the compiler places
