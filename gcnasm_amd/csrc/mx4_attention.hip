@@ -1073,7 +1073,7 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 // How a call is cut. A kv head with more than 64 rows in a sequence goes to
 // mx4_prompt.hip (32768 tokens, 32 heads over 8, D = 128: 256 rows of each kv head 80 us
 // there and 86 here, 64 rows 41 and 39; 8 sequences of 8192 with 64 rows 68 and 59),
-// its tokens split for up to two workgroups a CU, at least 256 a split. Here row blocks
+// its tokens split as prompt_chunk says. Here row blocks
 // of 16 rows while a sequence has no more, else of 32 (D = 256: always 16, two
 // blocks' sums do not fit the registers), and tokens in chunks of a multiple of 128, a
 // tile for each of four waves:
@@ -1093,6 +1093,33 @@ struct RowsPlan {
     size_t ws_floats;
 };
 
+// Tokens of a split for many rows: the cut with the least time by what was measured, in us. 64 tokens
+// take a workgroup alone on its CU 1.1, 1.5, 2.6 (D = 64, 128, 256), two on a CU, of which D = 256
+// has no room, 0.85 and 1.15 each; splits cost a launch, and their sums are written and
+// read at 2.5 TB/s. 32 heads over 8, D = 128: 1000 tokens 36 us, 55 in two splits, 500 21 and 29;
+// 700 rows over 8000 154 us in two splits, 190 in one; 300 rows 86 in three, 94 in six, 189 in one;
+// 100 rows 54 in eight, 188 in one.
+static int prompt_chunk(int head_dim, long long span, long long units, int num_cu, double rows)
+{
+    const double alone = head_dim == 64 ? 1.1 : (head_dim == 128 ? 1.5 : 2.6);
+    const double shared = head_dim == 64 ? 0.85 : (head_dim == 128 ? 1.15 : 2.6);
+    const long long tiles = (span + 63) / 64;
+    const long long most = std::min<long long>(tiles, std::max<long long>(1, 2ll * num_cu / units));
+    long long best = tiles;
+    double least = 0.0;
+    for (long long s = 1; s <= most; s++) {
+        const long long n = (tiles + s - 1) / s; // of a split
+        const long long per_cu = (units * s + num_cu - 1) / num_cu;
+        const double time = n * (per_cu == 1 ? alone : shared * per_cu) +
+                            (s == 1 ? 0.0 : 6.0 + s * rows * head_dim * 8 / 2.5e6);
+        if (s == 1 || time < least) {
+            least = time;
+            best = n;
+        }
+    }
+    return (int)std::min<long long>(best * 64, 1 << 30);
+}
+
 static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a, int num_cu)
 {
     RowsPlan r{};
@@ -1109,9 +1136,7 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
     span = std::max<long long>(span, 1);
     const long long units = (long long)a.seqs * c.kv_heads * r.row_blocks;
     if (r.prompt) {
-        const long long want = std::max<long long>(1, 2ll * num_cu / units);
-        r.chunk = (int)std::max<long long>((span + want - 1) / want, 256);
-        r.chunk = (r.chunk + 63) / 64 * 64;
+        r.chunk = prompt_chunk(c.head_dim, span, units, num_cu, (double)a.rows * a.heads);
     } else {
         const bool one = r.tiles == 1 && units < 2 * num_cu && span * c.head_dim <= 640 * 128;
         r.waves = one && span > 128 ? 8 : 4;
