@@ -537,13 +537,15 @@ void mx4_rows_kernel(AttnParams p)
 // The splits of a row joined: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s. A
 // workgroup of WAVES waves a row, each wave every WAVES-th split, then the waves in
 // order: the same order on every call. Bound by its launch, and with many splits by
-// the latency of reading their sums, so eight are read at a time.
+// the latency of reading their sums, so eight are read at a time: about 4 us for a few splits. WAVES: 1
+// up to 4 splits, 4 up to 64, then 16 (one row of two heads over 96025 tokens, D = 64, 376
+// splits: 16 us in all, 23 with 4).
 template <int D, int WAVES>
-__global__ __launch_bounds__(256) void mx4_join_kernel(AttnParams p)
+__global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void mx4_join_kernel(AttnParams p)
 {
     constexpr int E = D / 64; // elements of a lane
-    constexpr int kRows = 4 / WAVES;
-    __shared__ float part_acc[4][D], part_sum[4];
+    constexpr int kRows = WAVES > 4 ? 1 : 4 / WAVES;
+    __shared__ float part_acc[kRows * WAVES][D], part_sum[kRows * WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long unit = (long long)blockIdx.x * kRows + wave / WAVES;
     const bool real = unit < (long long)p.rows * p.heads;
@@ -792,8 +794,24 @@ __global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
     const Mx4Page<D> lay(1 << p.log2p);
     const int* table = p.table + b * p.s_table;
     const int rows = seq.n * p.group;
-    const int begin = part * w.chunk + 32 * wave, end = min((part + 1) * w.chunk, w.width);
+    const int end = min((part + 1) * w.chunk, w.width);
     const int last = min(end, seq.len); // of the tokens that have keys
+    // a window leaves most tokens behind: their weights stay, without a look at their keys (23
+    // sequences of up to 41289 tokens, 20 heads over 4, window 6: 11 us for 77)
+    int begin = part * w.chunk;
+    if (p.window) {
+        const long long seen = (long long)seq.len - seq.n - p.window + 1; // the first
+        const int behind = (int)(min(max(seen, (long long)begin), (long long)last) - begin);
+        const int skip = behind > 0 ? behind / 128 * 128 : 0;
+        const float* in = w.w_in ? w.w_in + b * w.si_seq + kv_head * w.si_head : nullptr;
+        float* out = w.w_out + b * w.so_seq + kv_head * w.so_head;
+        if (in != out)
+#pragma unroll 4
+            for (int t = begin + (int)threadIdx.x; t < begin + skip; t += 256)
+                out[t] = in ? in[t] : 0.0f;
+        begin += skip;
+    }
+    begin += 32 * wave;
     WeightRows<D> r;
     auto load_rows = [&](int x0) {
         const int x = x0 + (lane & 15);
@@ -1284,7 +1302,10 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
         else
             launch_rows<D, decltype(cap)::value>(p, r, (unsigned)grid, st);
         const long long joins = (long long)a.rows * a.heads;
-        if (r.splits > 4)
+        if (r.splits > 64)
+            hipLaunchKernelGGL((mx4_join_kernel<D, 16>), dim3((unsigned)joins), dim3(1024), 0, st,
+                               p);
+        else if (r.splits > 4)
             hipLaunchKernelGGL((mx4_join_kernel<D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
         else if (r.splits > 1)
             hipLaunchKernelGGL((mx4_join_kernel<D, 1>), dim3((unsigned)((joins + 3) / 4)), dim3(256),

@@ -122,3 +122,45 @@ def test_weights_of_many_rows_over_ragged_sequences(dev, rows, D):
             tol = want * (2.0 ** -14 + n[b] * 2 * 2.0 ** -23) + 1e-30
             assert (np.abs(got[b, :, :length] - want) <= tol).all()
             assert (got[b, :, length:] == 0).all()
+
+
+@pytest.mark.parametrize("D,hq,h,length", [(64, 2, 1, 20011), (128, 1, 1, 9001), (256, 2, 1, 17000)])
+def test_many_splits_of_one_row(dev, D, hq, h, length):
+    print("splits", D, hq, h, length, flush=True)
+    s = Setup(dev, [length, 1], [1, 1], hq, h, D, 64, seed=16)
+    parts = s.expected()
+    for lens, b in ((s.lens_d[:1], 0), (s.lens_d[1:], 1)):  # alone, so that it is cut the most
+        s1 = mc.attention(s.q[b:b + 1], s.cache, s.table_d[b:b + 1], lens, max_len=length)
+        o, l, _, ot, lt = parts[b]
+        assert (np.abs(host(s1[0].float()) - o) <= ot).all()
+        assert (np.abs(host(s1[1]) - l) <= lt).all()
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("window", [1, 6, 128, 700, 5000])
+def test_weights_of_few_rows_with_a_window(dev, rows, window):
+    print("weights with a window", rows, window, flush=True)
+    lens, n = [3001, 640, 130, 5, 0], [rows, rows, 0, rows, rows]
+    s = Setup(dev, lens, n, 4, 2, 128, 32, seed=17)
+    parts = s.expected(window=window)
+    lse = torch.from_numpy(np.concatenate([p[1] for p in parts]).astype(np.float32)).to(dev)
+    width = 3020
+    before = torch.rand((5, 2, width), device=dev)
+    old = host(before).astype(np.float64)
+    kw = dict(q_starts=s.starts_d, max_q=rows, max_len=3001, window=window)
+    args = (s.q, s.cache, s.table_d, s.lens_d, lse)
+    got = mc.attention_weights(*args, before, **kw)
+    for b, length in enumerate(lens):
+        want = parts[b][2] + old[b, :, :length]
+        # as of many rows, and the sum's rounding to fp32
+        tol = parts[b][2] * (2.0 ** -14 + 2 * rows * 2.0 ** -23) + want * 2.0 ** -22 + 1e-30
+        assert (np.abs(host(got)[b, :, :length] - want) <= tol).all()
+        assert (host(got)[b, :, length:] == 0).all()
+    base = mc.attention_weights(*args, None, width=width, **kw)
+    for b, length in enumerate(lens):
+        want = parts[b][2]
+        tol = want * (2.0 ** -14 + 2 * rows * 2.0 ** -23) + 1e-30
+        assert (np.abs(host(base)[b, :, :length] - want) <= tol).all()
+    place = before.clone()
+    assert mc.attention_weights(*args, place, out=place, **kw) is place
+    assert torch.equal(place, got)
