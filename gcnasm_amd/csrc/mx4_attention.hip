@@ -1102,7 +1102,10 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 // - Else up to two workgroups a CU, against 4 and 6 in one run: 64 sequences of 2048 to 8192 tokens
 //   (64 heads over 8) 87 us, 92 and 96; 32 of up to 4096 31, 30 and 33; 16 of 4000 with 4
 //   rows each (32 heads over 8) 23, 28 and 30, with 8 rows (64 heads over 8) 49, 55 and 69; 4 of
-//   131072 121, 127 and 122.
+//   131072 121, 127 and 122. Four of D = 64, which a CU holds: 53 of up to 99211 (one kv head)
+//   79, 91 with two.
+// - At least 256 tokens a split (8 of 2000: 13 us, with 128 16) and at most 128 splits, whose join
+//   grows: 131072 tokens of one kv head 19 us, with 64 24, with 512 28.
 struct RowsPlan {
     bool prompt; // mx4_prompt.hip
     int tiles;   // else: of 16 rows
@@ -1158,10 +1161,11 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
     } else {
         const bool one = r.tiles == 1 && units < 2 * num_cu && span * c.head_dim <= 640 * 128;
         r.waves = one && span > 128 ? 8 : 4;
-        const long long most =
-            one ? 1 : 2ll * num_cu / units;
-        const long long want = std::max<long long>(1, most);
+        const long long room = (c.head_dim == 64 && r.tiles == 1 ? 4ll : 2ll) * num_cu / units;
+        const long long want = one ? 1 : std::min<long long>(std::max<long long>(1, room), 128);
         r.chunk = (int)(((span + want - 1) / want + 127) / 128 * 128);
+        if (want > 1)
+            r.chunk = std::max(r.chunk, 256);
     }
     r.splits = (int)((span + r.chunk - 1) / r.chunk);
     if (r.splits > 1)
