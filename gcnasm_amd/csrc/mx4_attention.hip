@@ -538,8 +538,8 @@ void mx4_rows_kernel(AttnParams p)
 // workgroup of WAVES waves a row, each wave every WAVES-th split, then the waves in
 // order: the same order on every call. Bound by its launch, and with many splits by
 // the latency of reading their sums, so eight are read at a time: about 4 us for a few splits. WAVES: 1
-// up to 4 splits, 4 up to 64, then 16 (one row of two heads over 96025 tokens, D = 64, 376
-// splits: 16 us in all, 23 with 4).
+// up to 4 splits, 4 up to 64, then 16 (30000 tokens of two kv heads in 118 splits, the whole call: 13.2 us,
+// 14.6 with 4).
 template <int D, int WAVES>
 __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void mx4_join_kernel(AttnParams p)
 {
