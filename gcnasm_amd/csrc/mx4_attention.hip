@@ -214,8 +214,8 @@ __device__ __forceinline__ void scores16(const KeyCodes<D>& k, const v4i (&q)[RT
 // rounding to bf16, and the matrix cores wait for memory here anyway.
 //
 // Bound by reading the cache: 4 x 131072 tokens (64 heads over 8, D = 128, 570 MB)
-// 113 us with the join, 5.0 TB/s, where a copy reaches 5.16; 64 sequences of 2048 to 8192
-// tokens (361 MB) 85 us, 32 of up to 4096 with 8 kv heads (90 MB) 30, where the first loads, the
+// 105 to 113 us by card with the join, 5.0 to 5.4 TB/s, where a copy reaches 5.16; 64 sequences of
+// 2048 to 8192 tokens (361 MB) 79 to 85 us, 32 of up to 4096 with 8 kv heads (90 MB) 30, where the first loads, the
 // waves' join and the lengths' differences show. The pages' numbers are read a tile
 // before the codes and those a tile before their use: read where they are needed,
 // each tile waited for its page and the codes before it (100 and 36 us). The scheduling
