@@ -15,12 +15,30 @@ __device__ __forceinline__ v16f mfma_bf16_32x32x16(v4i a, v4i b, v16f c)
                                                    __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// Probabilities enter the second product in bf16, and where one is more than kShare of its
-// lane's sum so far a second bf16 term follows: there its rounding, up to 2^-8 of it, would show
-// in the output beside the output's own, elsewhere the many roundings even out (of 16 equal
-// ones to a tenth of 2^-8). Always a second term would make the second product twice
-// as long; at a 32nd the two measured below are 603 and 637 us.
+// Probabilities enter the second product in bf16, each off by up to 2^-8 of it. The output is
+// divided by the sum of what entered, so that what their roundings have in common leaves no trace
+// (512 equal scores below a larger one, values of 1.5: 1.492 divided by the sum of the unrounded
+// ones, which stays the one that lse is taken of). What is left of an output element is at most
+// 2^-8 of sum p |v - out|. Of random values it is, with the output's own rounding, 1.12, 1.21 and
+// 1.25 times that rounding's root mean square (2048 tokens, D = 64, 128, 256), and more tokens do
+// not lower it. Where a probability is more than kShare of its lane's sum so far a second bf16 term
+// follows, 16 bits together: few tokens carry such a row. A second term for all of them would take
+// the rest away and makes the second product twice as long: the two measured below 740 and
+// 747 us where this took 596 and 648, and without the rounded ones' sum 576 and 610.
 constexpr float kShare = 1.0f / 16;
+
+// sum[i] + the four bf16 of a lane's two dwords, on the matrix cores: a lane's four are a column of
+// their own, so a NaN stays in its row. v_dot2_f32_bf16, which the vector units take along with the
+// rest of the softmax, made D = 64 take 678 us for this one's 648; a product of 16 columns would
+// add up rows r and r + 16 in one, and 0 * NaN reach the other.
+__device__ __forceinline__ v4f add_four(int a, int b, v4f sum)
+{
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(
+        __builtin_bit_cast(v4s, (v2i){0x3F803F80, 0x3F803F80}),
+        __builtin_bit_cast(v4s, (v2i){a, b}), sum, 0, 0, 0);
+}
 
 // A wave has 32 rows, a workgroup four waves; both products give a row to a lane pair (l, l + 32):
 //   scores  S[token][row] = K Q^T, 32 tokens x 32 rows a product,
@@ -34,10 +52,10 @@ constexpr float kShare = 1.0f / 16;
 // Bound by what the chip's power allows more than by any unit: at D = 128 matrix
 // instructions are under way for half of the cycles and vector instructions for half, at
 // 1.7 of 2.4 GHz, and neither fewer exponentials nor fewer operand reads make it faster. A
-// prompt of 8192 tokens (32 heads over 8, D = 128, pages of 64) 566 to 596 us
-// from card to card, 0.92 to 0.97 PFLOP/s, where a large
+// prompt of 8192 tokens (32 heads over 8, D = 128, pages of 64) 590 to 606 us
+// from card to card, 0.91 to 0.93 PFLOP/s, where a large
 // bf16 product reaches 1.39; pieces of 500 to 1000 rows over up to 8191 tokens (64 heads over 8,
-// D = 64, pages of 16) 609 us. Tried beside it: eight waves, whose barrier the products of all
+// D = 64, pages of 16) 650 us. Tried beside it: eight waves, whose barrier the products of all
 // wait at (2048 tokens 82 us with four, 116 with eight); operands read as the compiler places
 // them and not a few products ahead (677 us where that took 642); their turning between the products, a
 // piece each (593, 616); D = 64 without the limit of registers that holds three waves a
@@ -244,14 +262,15 @@ __device__ __forceinline__ int out_element(int tile, int reg, int h)
     return r % 16 * (D / 16) + 2 * tile + r / 16;
 }
 
-// The tokens that turn() left out, added in fp32 by each row that sees them: score and values
+// The tokens that turn() left out, added in fp32 by each row that sees them, times `share` for the
+// sum that the output is divided by: score and values
 // straight from the codes, in the order of the tokens. Rare. The sums go through
 // LDS (mem: a float for each of the lane's, 64 apart), half of them at a time, so
 // that this takes no registers of the loop's.
 template <int D, bool CAP>
 __device__ __forceinline__ void add_left_out(const AttnParams& p, Mx4Page<D> lay, const int* table,
                                               int head, int begin, int end, const Row& row, int h,
-                                              float base, float* mem,
+                                              float base, float share, float* mem,
                                               v16f (&acc)[D / 32])
 {
     constexpr int kHalf = D / 64; // tiles
@@ -281,7 +300,7 @@ __device__ __forceinline__ void add_left_out(const AttnParams& p, Mx4Page<D> lay
                          fp4_value(page[lay.k_row(in) + d / 2] >> (d % 2 * 4) & 15u,
                                    page[lay.k_scale(in) + d / 32]),
                          s);
-            const float w = exp2_of(score_log2<CAP>(p, p.q_sign ? -s : s) - base);
+            const float w = exp2_of(score_log2<CAP>(p, p.q_sign ? -s : s) - base) * share;
 #pragma unroll 1
             for (int x = 0; x < kHalf * 16; x++) {
                 const int d = out_element<D>(half * kHalf + x / 16, x % 16, h);
@@ -344,7 +363,8 @@ void mx4_prompt_kernel(AttnParams p)
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 acc[t][r] = 0.0f;
-        float m = -INFINITY, base = 0.0f, l = 0.0f;
+        float m = -INFINITY, base = 0.0f;
+        float l = 0.0f, entered = 0.0f; // sums of the probabilities, and of their bf16 terms
         if (threadIdx.x == 0)
             lds.left_out = 0;
         __syncthreads();
@@ -420,6 +440,7 @@ void mx4_prompt_kernel(AttnParams p)
                 m = t;
                 base = t == -INFINITY ? 0.0f : t;
                 l *= f;
+                entered *= f;
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -429,10 +450,19 @@ void mx4_prompt_kernel(AttnParams p)
 #pragma unroll
             for (int half = 0; half < 2; half++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
+                for (int r = 0; r < 16; r++)
                     s[half][r] = exp2_of(fmaf(s[half][r], by, -base));
-                    l += s[half][r];
-                }
+            // four sums of eight, then into l: one running sum of thousands of equal numbers rounds
+            // alike at every step
+            float part[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                part[i] = s[i / 2][8 * (i % 2)];
+#pragma unroll
+                for (int r = 1; r < 8; r++)
+                    part[i] += s[i / 2][8 * (i % 2) + r];
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
             v4i pr[2][2];
             auto add = [&]() {
                 auto read = [&](int n) {
@@ -451,6 +481,13 @@ void mx4_prompt_kernel(AttnParams p)
                         a[n % kDepth] = read(n + kDepth);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                v4f sum[2] = {(v4f){0, 0, 0, 0}, (v4f){0, 0, 0, 0}};
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    sum[i % 2] = add_four(pr[i / 4][i / 2 % 2][i % 2 * 2],
+                                          pr[i / 4][i / 2 % 2][i % 2 * 2 + 1], sum[i % 2]);
+                entered += sum[0][0] + sum[1][0];
+                __builtin_amdgcn_sched_barrier(0);
             };
 #pragma unroll
             for (int half = 0; half < 2; half++)
@@ -502,15 +539,16 @@ void mx4_prompt_kernel(AttnParams p)
                     step(t0, buf, away);
                 barrier_lds();
             }
-            if (lds.left_out) // the operands are not read any more
-                add_left_out<D, CAP>(p, lay, table, kv_head, begin, end, row, h, base,
-                                      (float*)&lds + wave * (D / 64 * 16 * 64) + lane, acc);
         }
-
         l += __shfl_xor(l, 32, 64);
+        entered += __shfl_xor(entered, 32, 64);
+        if (begin < end && lds.left_out) // the operands are not read any more
+            add_left_out<D, CAP>(p, lay, table, kv_head, begin, end, row, h, base,
+                                 l == 0.0f ? 1.0f : entered / l,
+                                 (float*)&lds + wave * (D / 64 * 16 * 64) + lane, acc);
         if (!row.real) {
         } else if (p.splits == 1) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / entered;
             uint16_t* out = p.out + row.at * p.so_row + row.head * p.so_head;
 #pragma unroll
             for (int r = 0; r < 8; r++) {
@@ -531,12 +569,13 @@ void mx4_prompt_kernel(AttnParams p)
                 *(float2*)(p.ws + at * 2) = make_float2(m, l);
             if (m != -INFINITY || l != 0.0f) { // else nothing seen: the sums are not read
                 float* dst = p.ws + stats_floats(p.splits, p.rows, p.heads) + at * D;
+                const float f = l / entered; // the join divides by l
 #pragma unroll
                 for (int r = 0; r < 8; r++)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         *(float2*)(dst + out_element<D>(t, r, h)) =
-                            make_float2(acc[t][r], acc[t][r + 8]);
+                            make_float2(acc[t][r] * f, acc[t][r + 8] * f);
             }
         }
         __syncthreads(); // lds.left_out is read before the next block of rows clears it
