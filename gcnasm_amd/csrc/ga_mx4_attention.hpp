@@ -8,6 +8,7 @@
 #pragma once
 
 #include "ga_mx4_cache.hpp"
+#include "ga_mx4_positions.hpp"
 
 namespace ga {
 
@@ -56,23 +57,20 @@ struct Sequence {
 };
 
 // Rows r0 .. r0 + count - 1 of a sequence's n * group (row r: query r / group, head
-// r % group) and what they see: tokens in (lo, hi] of each row, and over all.
-struct Block {
+// r % group) and what they see.
+struct Block : Seen {
     int r0, count;
-    int hi_min, hi_max, lo_min, lo_max;
     __device__ __forceinline__ Block(const AttnParams& p, const Sequence& s, int first, int most)
+        : Block(p, s, first, min(most, s.n * p.group - first), 0)
     {
-        r0 = first;
-        count = min(most, s.n * p.group - first);
-        const int i0 = first / p.group, i1 = (first + count - 1) / p.group;
-        hi_min = p.causal ? min(s.len - s.n + i0, s.len - 1) : s.len - 1;
-        hi_max = p.causal ? min(s.len - s.n + i1, s.len - 1) : s.len - 1;
-        lo_min = p.window ? max(s.len - s.n + i0 - p.window, -1) : -1;
-        lo_max = p.window ? max(s.len - s.n + i1 - p.window, -1) : -1;
     }
-    // the tokens that some row sees: [begin, end), begin a multiple of 64
-    __device__ __forceinline__ int begin() const { return (lo_min + 1) & ~63; }
-    __device__ __forceinline__ int end() const { return hi_max + 1; }
+
+private:
+    __device__ __forceinline__ Block(const AttnParams& p, const Sequence& s, int first, int rows, int)
+        : Seen(s.len, s.n, first / p.group, (first + rows - 1) / p.group, p.causal, p.window),
+          r0(first), count(rows)
+    {
+    }
 };
 
 struct Row {
@@ -88,8 +86,8 @@ struct Row {
         const int i = x / p.group;
         head = kv_head * p.group + (x - i * p.group);
         at = s.q0 + i;
-        hi = !real ? -1 : (p.causal ? min(s.len - s.n + i, s.len - 1) : s.len - 1);
-        lo = p.window ? s.len - s.n + i - p.window : -1;
+        hi = real ? last_seen(s.len - s.n + i, s.len, p.causal) : -1;
+        lo = before_first(s.len - s.n + i, p.window);
     }
 };
 

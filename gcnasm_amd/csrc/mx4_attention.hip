@@ -691,7 +691,8 @@ struct RowCursor {
     long long q0, lse0;                           // of the sequence's first row
     long long q_step, q_wrap, lse_step, lse_wrap; // of a step, and if the head wraps besides
     int in, d_in, group;                          // head of the kv head's
-    int hi, lo, top, d_hi, wrap_hi, d_lo, wrap_lo;
+    int pos, d_pos;                               // position; if not causal the last token
+    int top, wrap_pos;
     __device__ __forceinline__ RowCursor(const AttnParams& p, const Sequence& s, int kv_head, int x,
                                          int step, int offset)
     {
@@ -709,12 +710,9 @@ struct RowCursor {
         lse_step = di * p.sl_row + d_in;
         lse_wrap = p.sl_row - group;
         top = s.len - 1;
-        hi = p.causal ? s.len - s.n + i : top;
-        d_hi = p.causal ? di : 0;
-        wrap_hi = p.causal ? 1 : 0;
-        lo = p.window ? s.len - s.n + i - p.window : -1;
-        d_lo = p.window ? di : 0;
-        wrap_lo = p.window ? 1 : 0;
+        pos = p.causal ? s.len - s.n + i : top;
+        d_pos = p.causal ? di : 0;
+        wrap_pos = p.causal ? 1 : 0;
     }
     // the lane's operands; real: the row is one of the sequence's (which has one), otherwise
     // the first row is read, for nothing
@@ -726,8 +724,8 @@ struct RowCursor {
         for (int m = 0; m < D / 32; m++)
             r.q[m] = *(const v4i*)(src + 8 * m);
         r.lse2 = p.lse[real ? lse : lse0] * kLog2e;
-        r.hi = real ? min(hi, top) : -1;
-        r.lo = lo;
+        r.hi = real ? min(pos, top) : -1;
+        r.lo = before_first(pos, p.window);
     }
     __device__ __forceinline__ void advance()
     {
@@ -736,8 +734,7 @@ struct RowCursor {
         in -= wrap ? group : 0;
         q += q_step + (wrap ? q_wrap : 0);
         lse += lse_step + (wrap ? lse_wrap : 0);
-        hi += d_hi + (wrap ? wrap_hi : 0);
-        lo += d_lo + (wrap ? wrap_lo : 0);
+        pos += d_pos + (wrap ? wrap_pos : 0);
     }
 };
 
@@ -879,7 +876,8 @@ constexpr int kWeightRows = 32, kWeightTiles = 2, kWeightTokens = 64 * kWeightTi
 constexpr int kWeightChunk = 128; // rows of a workgroup, at least
 
 template <int D, bool CAP>
-__global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
+__global__ __launch_bounds__(256, D == 64 ? 5 : (D == 128 ? 4 : 2))
+void mx4_weights_many_kernel(WeightsParams w)
 {
     constexpr int N = kWeightTiles;
     constexpr int kPieces = D / 8;        // 16-byte pieces of a row
@@ -905,11 +903,11 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
     float sum[4 * N] = {};
     // the queries that see some of the tokens: positions first .. first + 255 + window - 1
     const int pos0 = seq.len - seq.n;
-    const int i0 = p.causal ? max(first - pos0, 0) : 0;
+    const long long i0 = p.causal ? max((long long)first - pos0, 0ll) : 0;
     const long long far =
         p.window ? (long long)first + kWeightTokens - 1 + p.window - 1 - pos0 : seq.n - 1;
     const long long see = (min((long long)seq.n, far + 1)) * p.group; // end of their rows
-    const long long x_first = (long long)i0 * p.group;
+    const long long x_first = i0 * p.group;
     const int even = (int)((see - x_first + w.splits - 1) / w.splits);
     const int chunk = max((even + kWeightRows - 1) / kWeightRows * kWeightRows, kWeightChunk);
     const int x_begin = (int)min(see, x_first + (long long)split * chunk);
@@ -934,7 +932,7 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
         RowCursor at(p, seq, kv_head, x_begin + (tid & (kWeightRows - 1)), kWeightRows, 0);
         v4i held[kLoads];
         float lse;
-        int hi, lo;
+        int pos;
         auto tell = [&](int x0, int buf) {
             if (teller)
                 rows_at[buf][tid] = x0 + tid < x_end ? at.q : at.q0;
@@ -945,8 +943,7 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
                 held[j] = *(const v4i*)(p.q + rows_at[buf][j * kPass + my_row] + 8 * my_piece);
             const bool real = x0 + (tid & (kWeightRows - 1)) < x_end;
             lse = p.lse[real ? at.lse : at.lse0];
-            hi = real ? min(at.hi, at.top) : -1;
-            lo = at.lo;
+            pos = real ? at.pos : -1;
             at.advance();
         };
         auto publish = [&](int buf) {
@@ -957,8 +954,8 @@ __global__ __launch_bounds__(256) void mx4_weights_many_kernel(WeightsParams w)
             }
             if (teller) {
                 rows_lse[buf][tid] = lse * kLog2e;
-                rows_hi[buf][tid] = hi;
-                rows_lo[buf][tid] = lo;
+                rows_hi[buf][tid] = min(pos, at.top);
+                rows_lo[buf][tid] = before_first(pos, p.window);
             }
         };
         int buf = 0;

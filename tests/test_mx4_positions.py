@@ -1,0 +1,68 @@
+"""Which tokens of the MXFP4 cache a row sees (ga_mx4_positions.hpp), as the kernels compute it in 32
+bits, against the definition in 64 (CPU only): windows up to the largest int, more rows than tokens."""
+import os
+import subprocess
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gcnasm_amd",
+                    "csrc")
+
+CHECK = r"""
+#include "ga_mx4_positions.hpp"
+#include <stdio.h>
+#include <algorithm>
+typedef long long ll;
+int main()
+{
+    const int lens[] = {0, 1, 3, 63, 64, 65, 500, 1 << 20, 0x7FFFF000};
+    const int rows[] = {1, 2, 5, 9, 64, 700, 1 << 20};
+    const int windows[] = {0, 1, 6, 64, 499, 1 << 30, 0x7FFFFFF0, 0x7FFFFFFE, 0x7FFFFFFF};
+    ll bad = 0, checked = 0;
+    for (int len : lens)
+        for (int n : rows)
+            for (int w : windows)
+                for (int causal = w ? 1 : 0; causal < 2; causal++) {
+                    const ll step = n > 1000 ? n / 7 : 1;
+                    for (ll i0 = 0; i0 < n; i0 += step) {
+                        const ll i1 = std::min<ll>(i0 + 15, n - 1);
+                        const ga::Seen s(len, n, (int)i0, (int)i1, causal, w);
+                        ll first = 1ll << 40, last = -1; // that some row of the block sees
+                        for (ll i = i0; i <= i1; i++) {
+                            const ll pos = (ll)len - n + i;
+                            const ll hi = causal ? std::min<ll>(pos, len - 1) : len - 1;
+                            const ll lo = w ? std::max<ll>(pos - w, -1) : -1;
+                            const int got_hi = ga::last_seen((int)pos, len, causal);
+                            const int got_lo = ga::before_first((int)pos, w);
+                            if (hi > lo && hi >= 0) {
+                                bad += got_hi != hi || got_lo != lo;
+                                first = std::min(first, lo + 1);
+                                last = std::max(last, hi);
+                                bad += s.hi_min > hi || s.hi_max < hi || s.lo_min > lo ||
+                                       s.lo_max < lo;
+                            } else { // sees nothing
+                                bad += got_hi > got_lo && got_hi >= 0;
+                                bad += s.hi_min >= 0 && s.hi_min > s.lo_max && len > 0;
+                            }
+                            checked++;
+                        }
+                        // the tokens gone over are inside the sequence and hold all that is seen
+                        bad += s.begin() < 0 || s.begin() % 64 || s.end() > len;
+                        if (last >= 0)
+                            bad += s.begin() > first || s.end() <= last;
+                        else
+                            bad += s.begin() < s.end();
+                    }
+                }
+    printf("%lld of %lld\n", bad, checked);
+    return 0;
+}
+"""
+
+
+def test_what_rows_see(tmp_path):
+    src = tmp_path / "positions.cpp"
+    src.write_text(CHECK)
+    exe = str(tmp_path / "positions")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", CSRC, "-o", exe, str(src)], check=True)
+    out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()
+    assert out[0] == "0" and int(out[2]) > 20000, out
