@@ -160,6 +160,9 @@ def read(cache, slots, head_dim, dtype=torch.bfloat16, stream=None):
     return k, v
 
 
+_INT_MAX = 0x7FFFFFFF
+
+
 def _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window, softcap):
     if q.dim() != 3:
         raise ValueError("q must be [rows, heads, D], is %s" % (tuple(q.shape),))
@@ -175,11 +178,16 @@ def _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window
     if q_starts is not None:
         _check(q_starts, "q_starts", torch.int32, (seqs + 1,), device)
         starts = q_starts.data_ptr()
-    if max_len is None:
-        max_len = min(pages * c.page_size, 0x7FFFFFFF)
+    # what passes an int is more than any sequence has; ctypes would take its low 32 bits
+    if max_q is None or max_q > _INT_MAX:
+        max_q = rows
+    if max_len is None or max_len > _INT_MAX:
+        max_len = min(pages * c.page_size, _INT_MAX)
+    if window > _INT_MAX:
+        window = _INT_MAX
     return c, device, _lib.Mx4AttentionArgs(
         q.data_ptr(), None, None, table.data_ptr(), lens.data_ptr(), starts, sq[0], sq[1], 0, 0, 0,
-        st[0], seqs, rows, heads, pages, rows if max_q is None else max_q, max_len,
+        st[0], seqs, rows, heads, pages, max_q, max_len,
         1 if causal else 0, window, dim ** -0.5 if scale is None else scale, softcap)
 
 

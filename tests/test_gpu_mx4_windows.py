@@ -1,5 +1,7 @@
-"""Windows over the MXFP4 cache so large that they hide nothing, up to the largest int, as
+"""Windows over the MXFP4 cache so large that they hide nothing, up to and past the largest int, as
 "no limit" is written, with fewer tokens than rows among them: what no window gives."""
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -9,7 +11,7 @@ from test_gpu_mx4_cache import Setup, host
 
 pytestmark = pytest.mark.gpu
 
-WINDOWS = [1 << 30, 2 ** 31 - 2, 2 ** 31 - 1]
+WINDOWS = [1 << 30, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, sys.maxsize]
 SHAPES = [([3, 7], [9, 7], 4, 2, 128, 16), ([3, 0, 1], [5, 4, 1], 4, 2, 64, 16),
           ([700, 3, 129], [1, 1, 1], 6, 2, 256, 32), ([300, 20, 5], [250, 60, 70], 4, 2, 128, 64),
           ([130, 40], [129, 100], 2, 1, 64, 16), ([90], [100], 4, 2, 256, 64)]
@@ -32,3 +34,11 @@ def test_windows_without_an_end(dev, lens, rows, hq, h, D, P):
             tol = want * (2.0 ** -14 + rows[b] * hq * 2.0 ** -23) + 1e-30
             assert (np.abs(got[b, :, :length] - want) <= tol).all()
             assert (got[b, :, length:] == 0).all()
+
+
+def test_bounds_past_an_int(dev):
+    """max_q and max_len only choose the launch, whatever they are."""
+    s = Setup(dev, [300, 20], [30, 7], 4, 2, 128, 64, seed=32)
+    parts = s.expected()
+    for bound in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1):
+        s.check(*mc.attention(s.q, s.cache, s.table_d, s.lens_d, s.starts_d, bound, bound), parts)
