@@ -52,7 +52,7 @@ struct Sequence {
             n = min(max(p.q_starts[b + 1] - q0, 0), p.rows - q0);
         }
         const long long cap = (long long)p.table_pages << p.log2p;
-        len = (int)min((long long)max(p.lens[b], 0), min(cap, 0x7FFFFF00ll));
+        len = (int)min((long long)max(p.lens[b], 0), min(cap, (long long)GA_MX4_MAX_TOKENS));
     }
 };
 

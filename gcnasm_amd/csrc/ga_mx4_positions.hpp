@@ -36,4 +36,16 @@ struct Seen {
     GA_HOST_DEVICE int end() const { return hi_max + 1; }
 };
 
+// One of `parts` alike stretches of n tokens, [lo, hi): `rows` times 64, the last time maybe fewer.
+struct Stretch {
+    int lo, hi, rows;
+    GA_HOST_DEVICE Stretch(int n, int part, int parts)
+    {
+        const int most = (n + 64 * parts - 1) / (64 * parts) * 64;
+        lo = part * most < n ? part * most : n;
+        hi = n - lo < most ? n : lo + most;
+        rows = (hi - lo + 63) / 64;
+    }
+};
+
 } // namespace ga

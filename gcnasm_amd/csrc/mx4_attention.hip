@@ -791,7 +791,7 @@ __global__ __launch_bounds__(256) void mx4_weights_few_kernel(WeightsParams w)
     const Mx4Page<D> lay(1 << p.log2p);
     const int* table = p.table + b * p.s_table;
     const int rows = seq.n * p.group;
-    const int end = min((part + 1) * w.chunk, w.width);
+    const int end = (int)min((part + 1ll) * w.chunk, (long long)w.width);
     const int last = min(end, seq.len); // of the tokens that have keys
     // a window leaves most tokens behind: their weights stay, without a look at their keys (23
     // sequences of up to 41289 tokens, 20 heads over 4, window 6: 11 us for 77)
@@ -1041,7 +1041,8 @@ static ga_status attention_check(const ga_mx4_cache* c, const ga_mx4_attention_a
     if (!a->q_starts && a->rows != a->seqs)
         return fail(GA_ERR_SHAPE, "mx4 attention: %d rows of %d sequences need q_starts", a->rows,
                     a->seqs);
-    if ((long long)a->rows * a->heads > 0x7FFFFFFFll)
+    // a row's number and the step to the next block of rows together stay below 2^31
+    if ((long long)a->rows * a->heads > 0x3FFFFF00ll)
         return fail(GA_ERR_SHAPE, "mx4 attention: too many rows for one call");
     if (!pointers || a->seqs == 0 || a->rows == 0)
         return GA_OK;
@@ -1151,7 +1152,7 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
     long long span = std::min<long long>(a.max_len, (long long)a.table_pages * c.page_size);
     if (a.window > 0) // a row block's rows and the alignment of its first token
         span = std::min<long long>(span, (long long)a.window + block / group + 64);
-    span = std::max<long long>(span, 1);
+    span = std::min<long long>(std::max<long long>(span, 1), GA_MX4_MAX_TOKENS);
     const long long units = (long long)a.seqs * c.kv_heads * r.row_blocks;
     if (r.prompt) {
         r.chunk = prompt_chunk(c.head_dim, span, units, num_cu, (double)a.rows * a.heads);
@@ -1326,6 +1327,8 @@ ga_status ga_mx4_attention_weights_workspace_bytes(const ga_mx4_cache* cache,
         return st;
     if (width < 0)
         return fail(GA_ERR_ARG, "mx4 attention weights: negative width");
+    if (width > GA_MX4_MAX_TOKENS)
+        return fail(GA_ERR_SHAPE, "mx4 attention weights: too many tokens for one call");
     *bytes = 0;
     if (args->seqs == 0 || width == 0)
         return GA_OK;
@@ -1347,6 +1350,8 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
     const ga_mx4_attention_args& a = *args;
     if (width < 0)
         return fail(GA_ERR_ARG, "mx4 attention weights: negative width");
+    if (width > GA_MX4_MAX_TOKENS)
+        return fail(GA_ERR_SHAPE, "mx4 attention weights: too many tokens for one call");
     if (a.seqs == 0 || width == 0)
         return GA_OK;
     if (!w_out || !a.lens || (a.rows && !a.lse))

@@ -3,6 +3,7 @@
 #include "ga_device.hpp"
 #include "ga_internal.hpp"
 #include "ga_mx4_cache.hpp"
+#include "ga_mx4_positions.hpp"
 #include "ga_quant.hpp"
 
 #include <algorithm>
@@ -268,8 +269,8 @@ __global__ __launch_bounds__(kSelThreads) void mx4_select_kernel(EvictArgs e)
     if (want == 0)
         return;
     // each wave's stretch of the tokens: lane's are lo + lane, 64 apart
-    const int rows = (old + kSelThreads - 1) / kSelThreads;
-    const int lo = min(old, wave * rows * 64), hi = min(old, lo + rows * 64);
+    const Stretch part(old, wave, kSelWaves);
+    const int lo = part.lo, hi = part.hi, rows = part.rows;
     uint32_t held[KEYS ? KEYS : 1];
     auto key_of = [&](int i) { // 0, which no weight has, past the stretch's end
         const int j = lo + 64 * i + lane;
@@ -629,6 +630,8 @@ ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args,
         return fail(GA_ERR_ARG, "mx4_evict: keep must be positive and recent 0 .. keep");
     if (a.seqs < 0 || a.table_pages < 0 || a.dst_pages < 0 || a.width < 0 || a.new_width < a.keep)
         return fail(GA_ERR_ARG, "mx4_evict: negative size, or new_width below keep");
+    if (a.width > GA_MX4_MAX_TOKENS || a.new_width > GA_MX4_MAX_TOKENS)
+        return fail(GA_ERR_SHAPE, "mx4_evict: too many tokens for one call");
     if ((long long)a.dst_pages * cache->page_size < std::min(a.keep, a.width))
         return fail(GA_ERR_SHAPE, "mx4_evict: dst_table's pages hold fewer than keep tokens");
     if (a.seqs == 0)

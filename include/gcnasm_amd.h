@@ -599,6 +599,10 @@ typedef struct ga_mx4_cache {
     int page_size;
 } ga_mx4_cache;
 
+/* The most tokens of a sequence that the calls below look at, and the widest weights
+ * they take: positions, a few tiles past them included, stay below 2^31. */
+#define GA_MX4_MAX_TOKENS 0x7FFFF000
+
 /* Bytes of one kv head's page (0: no such page). */
 size_t ga_mx4_page_bytes(int page_size, int head_dim);
 
@@ -626,7 +630,7 @@ ga_status ga_mx4_read(const ga_mx4_cache* cache, const long long* slots, int tok
  *   table    [seqs, table_pages] page numbers, rows stride_table apart; tokens of
  *            a page outside the cache count as hidden
  *   lens     [seqs] tokens of each sequence, this step's rows among them (at most
- *            table_pages * P are used)
+ *            table_pages * P and GA_MX4_MAX_TOKENS are used)
  *   q_starts [seqs + 1] first row of each sequence (q_starts[seqs] = rows), or
  *            NULL: row b is sequence b's only one
  *   max_q, max_len  bounds of a sequence's rows and tokens, for the launch
@@ -663,8 +667,8 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
 /* What each cached token has been given: w_out[b, h, t] = w_in[b, h, t] + the
  * sum of exp(score - lse) over the rows that see token t and the query heads of
  * kv head h, fp32 [seqs, kv_heads, width], tokens contiguous, the other strides
- * in elements. Zero from the sequence's length on; tokens past `width` are left
- * out. w_in NULL counts as zeros, and may be w_out with the same strides. args: those
+ * in elements. Zero from the sequence's length on; tokens past `width` (at most
+ * GA_MX4_MAX_TOKENS) are left out. w_in NULL counts as zeros, and may be w_out with the same strides. args: those
  * of the attention; lse is read, out is not looked at. Sums run in a fixed
  * order. workspace: device scratch of the bytes that the call before says (0: none),
  * as for ga_mx4_attention. */
@@ -682,7 +686,8 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
  * weight (equal ones: the lowest index first; NaN counts as largest), in their
  * order, moved to the pages of dst_table; a sequence of at most `keep` is moved
  * whole.
- *   weights     [seqs, kv_heads, width] fp32, width >= every length
+ *   weights     [seqs, kv_heads, width] fp32, width >= every length; width and
+ *               new_width at most GA_MX4_MAX_TOKENS
  *   kept        [seqs, kv_heads, keep] the kept tokens' indices, -1 behind them
  *   new_lens    [seqs]
  *   new_weights [seqs, kv_heads, new_width >= keep] the kept tokens' weights,

@@ -1,7 +1,10 @@
 """Which tokens of the MXFP4 cache a row sees (ga_mx4_positions.hpp), as the kernels compute it in 32
 bits, against the definition in 64 (CPU only): windows up to the largest int, more rows than tokens."""
+import ctypes
 import os
 import subprocess
+
+from gcnasm_amd import _lib
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gcnasm_amd",
                     "csrc")
@@ -52,6 +55,19 @@ int main()
                             bad += s.begin() < s.end();
                     }
                 }
+    // eviction: 16 waves' stretches of the tokens follow each other and end with the last one
+    for (int n : {1, 2, 63, 64, 65, 1023, 1024, 1025, 8192, 8193, 65536, 65537, 100001, 0x7FFFEFFF,
+                  0x7FFFF000}) {
+        int at = 0;
+        for (int part = 0; part < 16; part++) {
+            const ga::Stretch s(n, part, 16);
+            bad += s.lo != at || s.hi < s.lo || s.hi > n || s.rows != (s.hi - s.lo + 63) / 64;
+            bad += s.rows > (n + 1023ll) / 1024;
+            bad += s.rows && s.lo + 64ll * (s.rows - 1) + 63 > 0x7FFFFFFF;
+            at = s.hi;
+        }
+        bad += at != n;
+    }
     printf("%lld of %lld\n", bad, checked);
     return 0;
 }
@@ -66,3 +82,31 @@ def test_what_rows_see(tmp_path):
                     "-I", CSRC, "-o", exe, str(src)], check=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()
     assert out[0] == "0" and int(out[2]) > 20000, out
+
+
+def test_sizes_that_pass_the_positions_are_refused():
+    """More tokens or rows than 32 bits can step over, before any device call."""
+    l, r = _lib.lib(), ctypes.byref
+    most, bad = 0x7FFFF000, 0x7FFFF001
+    c = _lib.Mx4Cache(0x10000, 8, 2 * 8704, 2, 128, 64)
+    a = _lib.Mx4AttentionArgs()
+    e = _lib.Mx4EvictArgs()
+    for n in ("q", "out", "lse", "table", "lens", "q_starts"):
+        setattr(a, n, 0x10000)
+    a.stride_q_row = a.stride_out_row = 4 * 128
+    a.stride_q_head = a.stride_out_head = 128
+    a.seqs, a.rows, a.heads, a.table_pages, a.max_q, a.max_len, a.causal = 3, 3, 4, 5, 1, 100, 1
+    need = ctypes.c_size_t()
+    assert l.ga_mx4_attention_weights_workspace_bytes(r(c), r(a), bad, r(need)) == _lib.GA_ERR_SHAPE
+    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, bad, None, 0,
+                                      None) == _lib.GA_ERR_SHAPE
+    a.rows = 0x3FFFFF00 // 4 + 1
+    assert l.ga_mx4_attention(r(c), r(a), None, 0, None) == _lib.GA_ERR_SHAPE
+    assert l.ga_mx4_attention_workspace_bytes(r(c), r(a), r(need)) == _lib.GA_ERR_SHAPE
+    for n in ("table", "lens", "dst_table", "weights", "kept", "new_lens", "new_weights"):
+        setattr(e, n, 0x10000)
+    for e.width, e.new_width in ((bad, 100), (200, bad)):
+        e.seqs, e.table_pages, e.dst_pages, e.keep, e.recent = 2, 4, 2, 100, 10
+        assert l.ga_mx4_evict(r(c), r(e), None) == _lib.GA_ERR_SHAPE
+    header = open(os.path.join(CSRC, "..", "..", "include", "gcnasm_amd.h")).read()
+    assert "#define GA_MX4_MAX_TOKENS 0x%X" % most in header
