@@ -268,6 +268,8 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
         width = a.max_len if weights is None else weights.shape[2]
     if out is not None:
         width = out.shape[-1]
+    if width > _INT_MAX:
+        raise ValueError("width %d is more than a call takes" % width)
     if weights is not None and weights.shape[2] < width:
         raise ValueError("weights hold %d tokens, out %d" % (weights.shape[2], width))
     need = ctypes.c_size_t(0)
@@ -306,8 +308,8 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
     st = _check(table, "table", torch.int32, (seqs, pages), device)
     sd = _check(dst_table, "dst_table", torch.int32, (seqs, dst_pages), device)
     sw = _weights(weights, "weights", seqs, c.kv_heads, device)
-    if keep <= 0 or not 0 <= recent <= keep:
-        raise ValueError("keep must be positive and recent 0 .. keep")
+    if not 0 < keep <= _INT_MAX or not 0 <= recent <= keep:
+        raise ValueError("keep must be positive (and an int) and recent 0 .. keep")
     sn, new_width = (c.kv_heads * keep, keep), keep
     if new_weights is not None:
         sn = _weights(new_weights, "new_weights", seqs, c.kv_heads, device)

@@ -42,3 +42,13 @@ def test_bounds_past_an_int(dev):
     parts = s.expected()
     for bound in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1):
         s.check(*mc.attention(s.q, s.cache, s.table_d, s.lens_d, s.starts_d, bound, bound), parts)
+
+
+def test_sizes_past_an_int_are_refused(dev):
+    s = Setup(dev, [20, 30], [1, 1], 4, 2, 128, 16, seed=33)
+    w = torch.zeros((2, 2, 30), device=dev)
+    lse = torch.zeros((2, 4), device=dev)
+    with pytest.raises(ValueError):
+        mc.attention_weights(s.q, s.cache, s.table_d, s.lens_d, lse, width=2 ** 32 + 5)
+    with pytest.raises(ValueError):
+        mc.evict(s.cache, s.table_d, s.lens_d, w, 2 ** 32 + 5, 1, s.table_d, 128)
