@@ -22,6 +22,12 @@ ga_status hip_fail(hipError_t e, const char* what);
             return ::ga::hip_fail(e_, #call);               \
     } while (0)
 
+// Workgroups of so many threads that one launch along x takes: HIP refuses 2^32 threads and more.
+constexpr long long most_workgroups(int threads)
+{
+    return 0xFFFFFFFFll / threads < 0x7FFFFFFFll ? 0xFFFFFFFFll / threads : 0x7FFFFFFFll;
+}
+
 // One compiled MX kernel: the manifest row plus its launcher.
 // ws: the split-K workspace, or (wsh set) found through the device slot wsh at
 // kernel entry, where a slot shorter than the layout makes the kernel write nothing.

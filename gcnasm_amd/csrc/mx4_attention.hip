@@ -1107,7 +1107,7 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 struct RowsPlan {
     bool prompt; // mx4_prompt.hip
     int tiles;   // else: of 16 rows
-    int waves;
+    int waves, threads; // of a workgroup
     int row_blocks, splits, chunk;
     size_t ws_floats;
 };
@@ -1166,6 +1166,14 @@ static RowsPlan rows_plan(const ga_mx4_cache& c, const ga_mx4_attention_args& a,
             r.chunk = std::max(r.chunk, 256);
     }
     r.splits = (int)((span + r.chunk - 1) / r.chunk);
+    // what one launch takes: without splits if their join would be too large; each workgroup
+    // goes over its share of a sequence's row blocks
+    r.threads = r.prompt ? 256 : 64 * r.waves;
+    if (r.splits > 1 && ((long long)a.rows * a.heads + 3) / 4 > most_workgroups(256))
+        r.splits = 1;
+    const long long others = (long long)a.seqs * c.kv_heads * r.splits;
+    r.row_blocks =
+        (int)std::min<long long>(r.row_blocks, std::max(1ll, most_workgroups(r.threads) / others));
     if (r.splits > 1)
         r.ws_floats = stats_floats(r.splits, a.rows, a.heads) +
                       (size_t)r.splits * a.rows * a.heads * c.head_dim;
@@ -1289,8 +1297,8 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
     if ((uintptr_t)workspace % 16)
         return fail(GA_ERR_ARG, "mx4 attention: workspace must be 16-byte aligned");
     const long long grid = (long long)a.seqs * cache->kv_heads * r.row_blocks * r.splits;
-    if (grid > 0x7FFFFFFFll)
-        return fail(GA_ERR_SHAPE, "mx4 attention: too many rows for one call");
+    if (grid > most_workgroups(r.threads))
+        return fail(GA_ERR_SHAPE, "mx4 attention: too many sequences for one call");
     AttnParams p = params_of(*cache, a);
     p.row_blocks = r.row_blocks;
     p.splits = r.splits;
@@ -1304,10 +1312,10 @@ ga_status ga_mx4_attention(const ga_mx4_cache* cache, const ga_mx4_attention_arg
         else
             launch_rows<D, decltype(cap)::value>(p, r, (unsigned)grid, st);
         const long long joins = (long long)a.rows * a.heads;
-        if (r.splits > 64)
+        if (r.splits > 64 && joins <= most_workgroups(1024))
             hipLaunchKernelGGL((mx4_join_kernel<D, 16>), dim3((unsigned)joins), dim3(1024), 0, st,
                                p);
-        else if (r.splits > 4)
+        else if (r.splits > 4 && joins <= most_workgroups(256))
             hipLaunchKernelGGL((mx4_join_kernel<D, 4>), dim3((unsigned)joins), dim3(256), 0, st, p);
         else if (r.splits > 1)
             hipLaunchKernelGGL((mx4_join_kernel<D, 1>), dim3((unsigned)((joins + 3) / 4)), dim3(256),
@@ -1365,8 +1373,9 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
                     workspace ? workspace_bytes : (size_t)0, r.ws_bytes);
     if ((uintptr_t)workspace % 4)
         return fail(GA_ERR_ARG, "mx4 attention weights: workspace must be 4-byte aligned");
-    if (r.grid > 0x7FFFFFFFll)
-        return fail(GA_ERR_SHAPE, "mx4 attention weights: too many sequences for one call");
+    if (r.grid > most_workgroups(256))
+        return fail(GA_ERR_SHAPE, "mx4 attention weights: too many sequences or tokens for one "
+                                  "call");
     const WeightsParams w{params_of(*cache, a), w_in,    w_out,    stride_in_seq,
                           stride_in_head,       stride_out_seq, stride_out_head,
                           width,                r.chunk, r.splits, (float*)workspace};

@@ -567,7 +567,7 @@ ga_status ga_mx4_append(const ga_mx4_cache* cache, const void* k, const void* v,
                       aligned_rows(v, stride_v_row, stride_v_head, 8, 16);
     const long long rows = (long long)tokens * cache->kv_heads;
     const long long blocks = (rows * (cache->head_dim / (wide ? 8 : 4)) + 255) / 256;
-    if (rows > 0x7FFFFFFFll || blocks > 0x7FFFFFFFll)
+    if (rows > 0x7FFFFFFFll || blocks > most_workgroups(256))
         return fail(GA_ERR_SHAPE, "mx4_append: too many tokens for one call");
     with_dim(cache->head_dim, [&](auto dim) {
         constexpr int D = decltype(dim)::value;
@@ -602,7 +602,7 @@ ga_status ga_mx4_read(const ga_mx4_cache* cache, const long long* slots, int tok
         return fail(GA_ERR_ARG, "mx4_read: k and v must be 16-byte aligned, nothing null");
     const long long rows = (long long)tokens * cache->kv_heads;
     const long long blocks = (rows * (cache->head_dim / 8) + 255) / 256;
-    if (rows > 0x7FFFFFFFll || blocks > 0x7FFFFFFFll)
+    if (rows > 0x7FFFFFFFll || blocks > most_workgroups(256))
         return fail(GA_ERR_SHAPE, "mx4_read: too many tokens for one call");
     with_dim(cache->head_dim, [&](auto dim) {
         constexpr int D = decltype(dim)::value;
@@ -641,7 +641,7 @@ ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args,
         return fail(GA_ERR_ARG, "mx4_evict: null pointer");
     const long long units = (long long)a.seqs * cache->kv_heads;
     const int blocks = (a.keep + kMoveTokens - 1) / kMoveTokens;
-    if (units * blocks > 0x7FFFFFFFll)
+    if (units > most_workgroups(kSelThreads) || units * blocks > most_workgroups(256))
         return fail(GA_ERR_SHAPE, "mx4_evict: too many sequences for one call");
     const EvictArgs e{a, view_of(*cache)};
     // the most tokens that may be looked at decide whether a lane can hold its share

@@ -110,3 +110,21 @@ def test_sizes_that_pass_the_positions_are_refused():
         assert l.ga_mx4_evict(r(c), r(e), None) == _lib.GA_ERR_SHAPE
     header = open(os.path.join(CSRC, "..", "..", "include", "gcnasm_amd.h")).read()
     assert "#define GA_MX4_MAX_TOKENS 0x%X" % most in header
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """A launch takes fewer than 2^32 threads; what asks for more is refused before it."""
+    l, r = _lib.lib(), ctypes.byref
+    c = _lib.Mx4Cache(0x10000, 8, 16 * 8704, 16, 128, 64)
+    # 2^24 tokens of 16 heads, 16 lanes a row of bf16, 32 of fp32: 2^32 and 2^33 threads
+    for kind, tokens in ((1, 1 << 24), (0, 1 << 23)):
+        assert l.ga_mx4_append(r(c), 0x1000, 0x1000, kind, tokens, 2048, 128, 2048, 128, 0x1000, 0,
+                               None) == _lib.GA_ERR_SHAPE
+    assert l.ga_mx4_read(r(c), 0x1000, 1 << 24, 0x1000, 0x1000, 0, None) == _lib.GA_ERR_SHAPE
+    e = _lib.Mx4EvictArgs()
+    for n in ("table", "lens", "dst_table", "weights", "kept", "new_lens", "new_weights"):
+        setattr(e, n, 0x10000)
+    # 1024 threads for each sequence's head to select; 256 for each 64 tokens of one to move
+    for e.seqs, e.keep in ((1 << 18, 1), (1 << 10, 1 << 16)):
+        e.table_pages, e.dst_pages, e.width, e.new_width = 4, 1 << 10, 200, e.keep
+        assert l.ga_mx4_evict(r(c), r(e), None) == _lib.GA_ERR_SHAPE
