@@ -1362,7 +1362,8 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
         return fail(GA_ERR_SHAPE, "mx4 attention weights: too many tokens for one call");
     if (a.seqs == 0 || width == 0)
         return GA_OK;
-    if (!w_out || !a.lens || (a.rows && !a.lse))
+    // without rows the kernels still look the tokens' pages up
+    if (!w_out || !a.lens || (!a.table && a.table_pages) || (a.rows && !a.lse))
         return fail(GA_ERR_ARG, "mx4 attention weights: null pointer");
     int num_cu = 0;
     if (const ga_status st = device_cu_count(&num_cu))

@@ -128,3 +128,15 @@ def test_launches_of_too_many_threads_are_refused():
     for e.seqs, e.keep in ((1 << 18, 1), (1 << 10, 1 << 16)):
         e.table_pages, e.dst_pages, e.width, e.new_width = 4, 1 << 10, 200, e.keep
         assert l.ga_mx4_evict(r(c), r(e), None) == _lib.GA_ERR_SHAPE
+
+
+def test_weights_of_no_rows_need_a_table():
+    """Without rows the weights' kernel still goes over the tokens: a table that is not there is
+    refused."""
+    l, r = _lib.lib(), ctypes.byref
+    c = _lib.Mx4Cache(0x10000, 8, 2 * 8704, 2, 128, 64)
+    a = _lib.Mx4AttentionArgs()
+    a.lens, a.q_starts = 0x10000, 0x10000
+    a.seqs, a.rows, a.heads, a.table_pages, a.max_q, a.max_len, a.causal = 3, 0, 4, 5, 1, 100, 1
+    assert l.ga_mx4_attention_weights(r(c), r(a), None, 0, 0, 0x1000, 8, 8, 8, None, 0,
+                                      None) == _lib.GA_ERR_ARG
