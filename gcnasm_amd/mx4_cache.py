@@ -255,7 +255,8 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
     q give to each cached token: the sum of exp(score - lse) over the rows that see it
     and the query heads of the kv head. q, lse and the rest as of the attention()
     call. -> out, float32 [sequences, kv heads, width] (width: weights', or
-    max_len), zeros from a sequence's length on; out may be weights."""
+    max_len), zeros from a sequence's length on; out may be weights. workspace: a tensor of
+    at least attention_weights_workspace_bytes."""
     c, device, a = _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window,
                          softcap)
     a.stride_lse_row = _check(lse, "lse", torch.float32, q.shape[:2], device)[0]
@@ -288,8 +289,19 @@ def attention_weights(q, cache, table, lens, lse, weights=None, q_starts=None, m
     return out
 
 
+def attention_weights_workspace_bytes(q, cache, table, lens, width, q_starts=None, max_q=None,
+                                      max_len=None, causal=True, window=0):
+    """Bytes of scratch that attention_weights() takes for these sizes; width as its out has it."""
+    c, _, a = _args(q, cache, table, lens, q_starts, max_q, max_len, None, causal, window, 0.0)
+    if width > _INT_MAX:
+        raise ValueError("width %d is more than a call takes" % width)
+    need = ctypes.c_size_t(0)
+    check(lib().ga_mx4_attention_weights_workspace_bytes(c, a, width, need))
+    return need.value
+
+
 def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_weights=None,
-          stream=None):
+          stream=None, kept=None, new_lens=None):
     """Keeps, of each sequence and kv head, the last `recent` tokens and of the
     others the keep - recent with the most weight (equal ones: the lowest index
     first), moved in their order to the pages of dst_table, int32 [sequences, at least
@@ -297,7 +309,8 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
 
     -> (kept int32 [sequences, kv heads, keep], -1 behind a shorter sequence;
     new_lens int32 [sequences]; new_weights float32 [sequences, kv heads, keep, or
-    the width of the new_weights given], zeros behind). The pages of dst_table must
+    the width of the new_weights given], zeros behind). kept (contiguous), new_lens and
+    new_weights can be given to write to. The pages of dst_table must
     be pages that no table holds for tokens in use; those of `table` are free
     for others once the call has run on its stream."""
     c, device = _cache(cache, head_dim)
@@ -314,9 +327,17 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
     if new_weights is not None:
         sn = _weights(new_weights, "new_weights", seqs, c.kv_heads, device)
         new_width = new_weights.shape[2]
+    if kept is not None:
+        _check(kept, "kept", torch.int32, (seqs, c.kv_heads, keep), device)
+        if not kept.is_contiguous():
+            raise ValueError("kept must be contiguous (strides %s)" % (tuple(kept.stride()),))
+    if new_lens is not None:
+        _check(new_lens, "new_lens", torch.int32, (seqs,), device)
     with _on(stream):
-        kept = lens.new_empty((seqs, c.kv_heads, keep))
-        new_lens = torch.empty_like(lens)
+        if kept is None:
+            kept = lens.new_empty((seqs, c.kv_heads, keep))
+        if new_lens is None:
+            new_lens = torch.empty_like(lens)
         if new_weights is None:
             new_weights = weights.new_empty((seqs, c.kv_heads, keep))
     a = _lib.Mx4EvictArgs(
