@@ -8,6 +8,9 @@ rows attend to it (attention), and what each token is given is added up
 cache is thinned: the latest `recent` tokens and those with the most weight move to
 fresh pages (evict) and the old pages are free again.
 
+append() quantises by its default rule here; scale_rule=GA_MX_SCALE_OCP loses less
+(values 0.12 of their root mean square instead of 0.20).
+
     python examples/mx4_cache_serving.py --seqs 16 --prompt 2000 --steps 300
 
 The host knows every length (a sequence of more than `keep` tokens has `keep` of them

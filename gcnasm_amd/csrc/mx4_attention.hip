@@ -901,7 +901,8 @@ void mx4_weights_many_kernel(WeightsParams w)
     const int first = part * kWeightTokens; // of the workgroup's tokens
     const int t0 = first + 16 * N * wave;
     float sum[4 * N] = {};
-    // the queries that see some of the tokens: positions first .. first + 255 + window - 1
+    // the queries that see some of the tokens: positions first .. first + kWeightTokens - 1 +
+    // window - 1
     const int pos0 = seq.len - seq.n;
     const long long i0 = p.causal ? max((long long)first - pos0, 0ll) : 0;
     const long long far =
@@ -1088,7 +1089,8 @@ static AttnParams params_of(const ga_mx4_cache& c, const ga_mx4_attention_args& 
 
 // How a call is cut. A kv head with more than 64 rows in a sequence goes to
 // mx4_prompt.hip (32768 tokens, 32 heads over 8, D = 128: 256 rows of each kv head 80 us
-// there and 86 here, 64 rows 41 and 39; 8 sequences of 8192 with 64 rows 68 and 59),
+// there and 86 here, 64 rows 41 and 39; 8 sequences of 8192 with 64 rows 68 and 59; the times
+// there of before it added up the rounded probabilities, 3 to 4 % more since),
 // its tokens split as prompt_chunk says. Here row blocks
 // of 16 rows while a sequence has no more, else of 32 (D = 256: always 16, two
 // blocks' sums do not fit the registers), and tokens in chunks of a multiple of 128, a
@@ -1115,7 +1117,8 @@ struct RowsPlan {
 // Tokens of a split for many rows: the cut with the least time by what was measured, in us. 64 tokens
 // take a workgroup alone on its CU 1.1, 1.5, 2.6 (D = 64, 128, 256), two on a CU, of which D = 256
 // has no room, 0.85 and 1.15 each; splits cost a launch, and their sums are written and
-// read at 2.5 TB/s. 32 heads over 8, D = 128: 1000 tokens 36 us, 55 in two splits, 500 21 and 29;
+// read at 2.5 TB/s. (Before the rounded probabilities were added up, which takes all cuts alike 3 to
+// 7 % more.) 32 heads over 8, D = 128: 1000 tokens 36 us, 55 in two splits, 500 21 and 29;
 // 700 rows over 8000 154 us in two splits, 190 in one; 300 rows 86 in three, 94 in six, 189 in one;
 // 100 rows 54 in eight, 188 in one.
 static int prompt_chunk(int head_dim, long long span, long long units, int num_cu, double rows)

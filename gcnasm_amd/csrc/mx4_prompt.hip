@@ -49,13 +49,14 @@ __device__ __forceinline__ v4f add_four(int a, int b, v4f sum)
 // the products of the 64 before: K as [d/8][token][8], V as [8 tokens][d/2 x parity][8 tokens],
 // which a lane reads 16 bytes at a time, neighbours side by side.
 //
-// Bound by what the chip's power allows more than by any unit: at D = 128 matrix
-// instructions are under way for half of the cycles and vector instructions for half, at
-// 1.7 of 2.4 GHz, and neither fewer exponentials nor fewer operand reads make it faster. A
-// prompt of 8192 tokens (32 heads over 8, D = 128, pages of 64) 590 to 606 us
-// from card to card, 0.91 to 0.93 PFLOP/s, where a large
+// Bound by no unit alone: a wave's products and its softmax follow each other, and the two (D =
+// 64: three) waves of a SIMD that the registers leave room for do not fill the gaps. At D = 128
+// matrix instructions are under way for 47 % of the cycles and vector instructions for 52, at 2.15
+// of 2.4 GHz; at D = 64 for 25 and 51 %, at 2.4 GHz. A prompt of 8192 tokens (32 heads over 8, D = 128,
+// pages of 64) 580 to 606 us from card to card, 0.91 to 0.95 PFLOP/s, where a large
 // bf16 product reaches 1.39; pieces of 500 to 1000 rows over up to 8191 tokens (64 heads over 8,
-// D = 64, pages of 16) 650 us. Tried beside it: eight waves, whose barrier the products of all
+// D = 64, pages of 16) 650 us; 4096 tokens at D = 256 (16 heads over 4) 204 us. Capped scores take
+// a tanhf each: 918 us for the first. Tried beside it, with the times of then: eight waves, whose barrier the products of all
 // wait at (2048 tokens 82 us with four, 116 with eight); operands read as the compiler places
 // them and not a few products ahead (677 us where that took 642); their turning between the products, a
 // piece each (593, 616); D = 64 without the limit of registers that holds three waves a
@@ -318,8 +319,8 @@ __device__ __forceinline__ void add_left_out(const AttnParams& p, Mx4Page<D> lay
 }
 
 // BIG: pages of 64 tokens or more, which hold a tile whole, so that its address is a scalar. The two
-// measured above with pages of 64: 566 us and as with smaller pages 575, 582 and 610 (D = 256:
-// alike).
+// measured above: with pages of 64 603 us, of 32 610; D = 64 with pages of 64 620, of 16 652 (D =
+// 256: alike).
 template <int D, bool CAP, bool BIG>
 __global__ __launch_bounds__(64 * PromptShape<D>::kWaves, D == 256 ? 1 : (D == 64 ? 3 : 2))
 void mx4_prompt_kernel(AttnParams p)

@@ -126,7 +126,11 @@ def append(cache, k, v, slots, scale_rule=_lib.GA_MX_SCALE_FLOOR_448, stream=Non
     """Quantises k, v [tokens, kv heads, D] (float32 or bfloat16, any row and head
     strides that are multiples of 4) into slots, int64 [tokens]. A slot outside the
     cache, such as -1, writes nothing; the others have to differ. The rules are
-    those of ops.quant_mxfp4."""
+    those of ops.quant_mxfp4; the default is that of the library's products, which
+    cuts a block's largest values by up to half. GA_MX_SCALE_OCP loses less: of
+    normally distributed values 0.115 of their root mean square instead of 0.20, of an
+    attention output over such a cache 0.19 instead of 0.34 (4096 tokens, D = 128, keys
+    with strong channels)."""
     if k.dim() != 3:
         raise ValueError("k must be [tokens, kv heads, D], is %s" % (tuple(k.shape),))
     kind = _IN_TYPES.get(k.dtype)
@@ -203,7 +207,13 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
     for each sequence. Row i of a sequence's n stands at position len - n + i and
     sees, if causal, the tokens up to it, of these the last `window` if window is
     not 0. softcap c > 0: scores c tanh(s / c). A row that sees nothing
-    gets zeros and lse -inf. heads is a multiple of the cache's kv heads.
+    gets zeros and lse -inf. heads is a multiple of the cache's kv heads. Positions are
+    places in the cache: after evict() a window counts the tokens that were kept.
+
+    With more than 64 rows of a kv head in a sequence the probabilities p enter the sum of
+    the values as bf16 (those over a 16th of a running sum with 16 bits): out is off by up
+    to 2^-8 of sum p |v - out| besides its own rounding, in all 1.1 to 1.3 times that
+    rounding for random values. With fewer rows all have 16 bits.
 
     max_q and max_len bound the rows and tokens of a sequence on the host; they
     choose the launch and may be larger than what the tensors hold (default: all
@@ -309,7 +319,8 @@ def evict(cache, table, lens, weights, keep, recent, dst_table, head_dim, new_we
 
     -> (kept int32 [sequences, kv heads, keep], -1 behind a shorter sequence;
     new_lens int32 [sequences]; new_weights float32 [sequences, kv heads, keep, or
-    the width of the new_weights given], zeros behind). kept (contiguous), new_lens and
+    the width of the new_weights given], zeros behind). weights hold every length. A window of
+    later attention counts kept tokens, not positions in the text. kept (contiguous), new_lens and
     new_weights can be given to write to. The pages of dst_table must
     be pages that no table holds for tokens in use; those of `table` are free
     for others once the call has run on its stream."""

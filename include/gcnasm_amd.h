@@ -609,7 +609,10 @@ size_t ga_mx4_page_bytes(int page_size, int head_dim);
 /* k, v [tokens, kv_heads, D] (fp32 or bf16; row and head strides in elements,
  * multiples of 4; 16-byte aligned fp32, 8-byte aligned bf16) quantised by
  * ga_quant_mxfp4's rules into slots[0 .. tokens - 1]. A slot outside the cache
- * (a negative one, say) writes nothing; the others have to differ. */
+ * (a negative one, say) writes nothing; the others have to differ. Rule 0, that of the
+ * library's products by default, cuts a block's largest values by up to half; of normally
+ * distributed values it leaves an error of 0.20 of their root mean square, the rules 1
+ * and 2 one of 0.115. */
 ga_status ga_mx4_append(const ga_mx4_cache* cache, const void* k, const void* v, int in_dtype,
                         int tokens, long long stride_k_row, long long stride_k_head,
                         long long stride_v_row, long long stride_v_head, const long long* slots,
@@ -639,7 +642,11 @@ ga_status ga_mx4_read(const ga_mx4_cache* cache, const long long* slots, int tok
  * tokens up to its position, and with window > 0 (causal only) the last
  * `window` of them. Scores are scale * q.k, with softcap > 0
  * softcap * tanh(scale * q.k / softcap). A row that sees no token gets zeros,
- * and lse -inf. */
+ * and lse -inf. Sums are fp32. With more than 64 rows of a kv head in a sequence the
+ * probabilities p of a row enter the sum of the values rounded to bf16 (those over a 16th of
+ * a running sum to 16 bits) and are divided by the sum of the rounded ones: an output element
+ * is off by up to 2^-8 of sum p |v - out| besides its own rounding. With fewer rows all have
+ * 16 bits. */
 typedef struct ga_mx4_attention_args {
     const void* q;
     void* out;
@@ -695,7 +702,9 @@ ga_status ga_mx4_attention_weights(const ga_mx4_cache* cache, const ga_mx4_atten
  * The pages of dst_table that a sequence needs (ceil(new_len / P)) must be pages
  * that no table holds for tokens in use, and new_weights and new_lens no part of
  * weights and lens. A kept token of a page outside the cache becomes zeros, as do the
- * places behind the last one up to a multiple of four. */
+ * values (not the keys) of the places behind the last one up to a multiple of four. Places
+ * are positions from then on: a window over the thinned cache counts kept tokens, not those of
+ * the text. */
 typedef struct ga_mx4_evict_args {
     const int* table;
     const int* lens;
