@@ -20,8 +20,8 @@ __device__ __forceinline__ v16f mfma_bf16_32x32x16(v4i a, v4i b, v16f c)
 // (512 equal scores below a larger one, values of 1.5: 1.492 divided by the sum of the unrounded
 // ones, which stays the one that lse is taken of). What is left of an output element is at most
 // 2^-8 of sum p |v - out|. Of random values it is, with the output's own rounding, 1.12, 1.21 and
-// 1.25 times that rounding's root mean square (2048 tokens, D = 64, 128, 256), and more tokens do
-// not lower it. Where a probability is more than kShare of its lane's sum so far a second bf16 term
+// 1.25 times that rounding's root mean square (2048 tokens, D = 64, 128, 256), 1.3 for the D = 64
+// pieces measured below and up to 1.4 where no row has a second term. Where a probability is more than kShare of its lane's sum so far a second bf16 term
 // follows, 16 bits together: few tokens carry such a row. A second term for all of them would take
 // the rest away and makes the second product twice as long: the two measured below 740 and
 // 747 us where this took 596 and 648, and without the rounded ones' sum 576 and 610.

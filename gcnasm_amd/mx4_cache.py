@@ -212,7 +212,7 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
 
     With more than 64 rows of a kv head in a sequence the probabilities p enter the sum of
     the values as bf16 (those over a 16th of a running sum with 16 bits): out is off by up
-    to 2^-8 of sum p |v - out| besides its own rounding, in all 1.1 to 1.3 times that
+    to 2^-8 of sum p |v - out| besides its own rounding, in all 1.1 to 1.4 times that
     rounding for random values. With fewer rows all have 16 bits.
 
     max_q and max_len bound the rows and tokens of a sequence on the host; they
