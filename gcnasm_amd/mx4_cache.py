@@ -143,6 +143,11 @@ def append(cache, k, v, slots, scale_rule=_lib.GA_MX_SCALE_FLOOR_448, stream=Non
     _check(slots, "slots", torch.int64, (tokens,), device)
     sk = _check(k, "k", k.dtype, shape, device)
     sv = _check(v, "v", k.dtype, shape, device)
+    # the stride of a dimension of one element can be anything
+    if tokens == 1:
+        sk, sv = (0, sk[1]), (0, sv[1])
+    if heads == 1:
+        sk, sv = (sk[0], 0), (sv[0], 0)
     check(lib().ga_mx4_append(c, k.data_ptr(), v.data_ptr(), kind, tokens, sk[0], sk[1], sv[0],
                               sv[1], slots.data_ptr(), scale_rule, _stream(stream, device)))
 
@@ -190,7 +195,8 @@ def _args(q, cache, table, lens, q_starts, max_q, max_len, scale, causal, window
     if window > _INT_MAX:
         window = _INT_MAX
     return c, device, _lib.Mx4AttentionArgs(
-        q.data_ptr(), None, None, table.data_ptr(), lens.data_ptr(), starts, sq[0], sq[1], 0, 0, 0,
+        q.data_ptr(), None, None, table.data_ptr(), lens.data_ptr(), starts,
+        sq[0] if rows > 1 else 0, sq[1] if heads > 1 else 0, 0, 0, 0,
         st[0], seqs, rows, heads, pages, max_q, max_len,
         1 if causal else 0, window, dim ** -0.5 if scale is None else scale, softcap)
 
@@ -227,6 +233,7 @@ def attention(q, cache, table, lens, q_starts=None, max_q=None, max_len=None, sc
     so, sl = (heads * dim, dim), (heads,)
     if out is not None:
         so = _check(out, "out", torch.bfloat16, q.shape, device)
+        so = so[0] if a.rows > 1 else 0, so[1] if heads > 1 else 0
     if lse is not None:
         sl = _check(lse, "lse", torch.float32, q.shape[:2], device)
     with _on(stream):
