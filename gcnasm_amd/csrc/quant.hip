@@ -50,24 +50,6 @@ __device__ __forceinline__ void mx_store_codes(const float (&v)[EPL], int e, uin
     }
 }
 
-// EPL elements divided by their scale as E4M3 bytes at dst. NAN_RULE false: no
-// quotient is a NaN, i.e. no element is one and the scale is neither infinite
-// (inf/inf) nor zero (0/0); ScaleDiv::fast holds for no such scale.
-template <bool NAN_RULE, int EPL, class D>
-__device__ __forceinline__ void fp8_store_codes(const D& d, const float (&v)[EPL], uint8_t* dst)
-{
-    float t[EPL];
-    d.div(v, t);
-    uint32_t w[EPL / 4];
-#pragma unroll
-    for (int j = 0; j < EPL / 4; j++)
-        w[j] = e4m3_encode4<NAN_RULE>(t[4 * j], t[4 * j + 1], t[4 * j + 2], t[4 * j + 3]);
-    if constexpr (EPL == 8)
-        *(uint2*)dst = make_uint2(w[0], w[1]);
-    else
-        *(uint32_t*)dst = w[0];
-}
-
 // ---- MX 1x32 (E4M3 or packed e2m1 codes) -------------------------------------
 // A 1x32 block is LPB = 32/EPL lanes of EPL elements (16-byte loads where the
 // layout allows); each lane handles U blocks, BPP = 256/LPB blocks apart, so U
@@ -181,48 +163,6 @@ __global__ __launch_bounds__(256) void prepare_mx_a_kernel(const void* __restric
 }
 
 // ---- DeepSeek 1x128 -----------------------------------------------------------
-__device__ __forceinline__ float ds_scale(float amax) { return amax > 0.0f ? amax / 448.0f : 1.0f; }
-
-// x / s for the elements that share one scale s, exact wherever the quotient
-// decides an E4M3 code. For finite s >= 2^-64: the reciprocal r = 1/s
-// (correctly rounded, once per scale), q0 = x*r, and two corrections
-// q <- q + (x - q*s)*r, each residual and product one FMA. With r within
-// half an ulp of 1/s and q within one ulp of x/s, the corrected quotient is
-// x/s correctly rounded (Markstein's theorem; the first correction brings
-// q0, within 1.5 ulp, inside one ulp). The residuals stay normal numbers for
-// every x whose quotient is at least 2^-12 (|x| >= 2^-76), the range in which
-// the fp32 quotient can change an E4M3 code; smaller quotients come out
-// below 2^-11 with x's sign, and such values encode to the signed zero either
-// way. The sign is taken from x, so -0 stays -0. tests/scale_div_check.c
-// restates this arithmetic on the CPU and compares it with IEEE division
-// (every bf16 x and random fp32 x under scales over the whole range; 1.4e9
-// quotients without a mismatch). Other scales (subnormal, infinite) divide. Five VALU instructions per element instead
-// of the IEEE division's ten; the choice is made once per scale.
-struct ScaleDiv {
-    float s, r;
-    bool fast;
-    __device__ __forceinline__ explicit ScaleDiv(float s_)
-        : s(s_), r(1.0f / s_), fast(s_ >= 0x1p-64f && s_ <= 3.40282347e38f)
-    {
-    }
-    template <int N>
-    __device__ __forceinline__ void div(const float (&v)[N], float (&t)[N]) const
-    {
-        if (fast) {
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const float q0 = v[j] * r;
-                const float q1 = fmaf(fmaf(-q0, s, v[j]), r, q0);
-                t[j] = copysignf(fmaf(fmaf(-q1, s, v[j]), r, q1), v[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j++)
-                t[j] = v[j] / s;
-        }
-    }
-};
-
 // A 1x128 group is LPB = 128/EPL lanes; U groups per lane as above.
 template <int IN, int EPL, int U>
 __global__ __launch_bounds__(256) void quant_1x128_kernel(const void* __restrict__ x, int rows,
