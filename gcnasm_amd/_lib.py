@@ -29,6 +29,11 @@ GA_MX_SCALE_FLOOR_448 = 0
 GA_MX_SCALE_CEIL_448 = 1
 GA_MX_SCALE_OCP = 2
 GA_NAME_MAX = 96
+GA_EXPERTS_MAX = 1024
+GA_EXPERTS_MAX_TOP = 64
+GA_EXPERTS_MAX_GROUPS = 64
+GA_EXPERTS_SOFTMAX = 0
+GA_EXPERTS_SIGMOID = 1
 # ga_mx_plan.kernel
 GA_MX_RUNS_ENTRY = 0
 GA_MX_RUNS_K_SPLIT = 1
@@ -206,6 +211,26 @@ class Mx4EvictArgs(ctypes.Structure):
                            "recent"]]
 
 
+class ExpertsRouteArgs(ctypes.Structure):
+    """ga_experts_route_args."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ["logits", "bias", "ids", "weights"]
+                ] + [("stride_logits", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in
+                     ["in_dtype", "tokens", "experts", "top", "scores", "groups", "top_groups",
+                      "group_rank", "renormalise"]] + [("scale", ctypes.c_float)]
+
+
+class ExpertsProductArgs(ctypes.Structure):
+    """ga_experts_product_args."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ["a", "sfa", "b", "sfb", "starts", "rows_of", "out"]
+                ] + [(n, ctypes.c_longlong) for n in
+                     ["a_rows", "stride_a", "stride_sfa", "stride_b_expert", "stride_b",
+                      "stride_sfb_expert", "stride_sfb", "stride_out"]
+                     ] + [(n, ctypes.c_int) for n in ["experts", "rows", "n", "k"]]
+
+
 assert ctypes.sizeof(OpusGemmKargs) == 96
 assert ctypes.sizeof(F4gemmKargs) == 0x174
 assert ctypes.sizeof(SplitkWsHandle) == 16
@@ -214,6 +239,8 @@ assert ctypes.sizeof(FlatmmSplitkKargs) == 96
 assert ctypes.sizeof(Mx4Cache) == 40
 assert ctypes.sizeof(Mx4AttentionArgs) == 136
 assert ctypes.sizeof(Mx4EvictArgs) == 136
+assert ctypes.sizeof(ExpertsRouteArgs) == 80
+assert ctypes.sizeof(ExpertsProductArgs) == 136
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -298,6 +325,11 @@ SIGNATURES = {
                                                       ctypes.POINTER(Mx4AttentionArgs), _i,
                                                       ctypes.POINTER(_sz)]),
     "ga_mx4_evict": (_i, [ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4EvictArgs), _vp]),
+    "ga_experts_route": (_i, [ctypes.POINTER(ExpertsRouteArgs), _vp]),
+    "ga_experts_arrange": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "ga_experts_product": (_i, [ctypes.POINTER(ExpertsProductArgs), _vp]),
+    "ga_experts_activate": (_i, [_vp, _i, _i, _i, _ll, _vp, _ll, _vp, _ll, _vp, _vp]),
+    "ga_experts_combine": (_i, [_vp, _i, _i, _ll, _vp, _vp, _i, _i, _vp, _i, _ll, _vp]),
     "ga_device_num_cu": (_i, [ctypes.POINTER(_i)]),
 }
 

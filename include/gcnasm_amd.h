@@ -721,6 +721,106 @@ typedef struct ga_mx4_evict_args {
 } ga_mx4_evict_args;
 ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Layers of experts: routing, the map of rows, the experts' products in FP8   */
+/* block scale (no counterpart in the reference).                              */
+/* ------------------------------------------------------------------------- */
+/* A token's logits choose `top` experts; the pairs (token, choice) are put in the
+ * order of their experts, so that expert e has the sorted rows starts[e] ..
+ * starts[e + 1] - 1; products run over those rows. Counts, ids and row numbers are
+ * data on the GPU: nothing waits for them, and the kernels keep them inside the
+ * operands. */
+#define GA_EXPERTS_MAX 1024     /* experts of a call                            */
+#define GA_EXPERTS_MAX_TOP 64   /* choices of a token                           */
+#define GA_EXPERTS_MAX_GROUPS 64
+#define GA_EXPERTS_SOFTMAX 0
+#define GA_EXPERTS_SIGMOID 1
+
+/* The experts of each token.
+ *   logits   [tokens, experts] fp32 or bf16 (in_dtype GA_IN_*), rows stride_logits
+ *            elements apart
+ *   bias     [experts] fp32, added to the scores for the choice alone; may be NULL
+ *   ids, weights  [tokens, top] contiguous
+ * scores: softmax over a token's logits, or the sigmoid of each. An expert's key is its
+ * score + bias in 64 bits, without a bias its logit. With top_groups < groups only
+ * the experts of top_groups groups (of experts / groups consecutive experts) can be chosen:
+ * those with the largest key (group_rank 1) or sum of their two largest keys (2; without a
+ * bias, of the two largest scores). Of these experts the `top` of largest key are chosen, in
+ * that order; of equal keys, as of equal groups, the lowest index comes first. weights are the
+ * scores of the chosen ones, divided by their sum if renormalise, times scale. A logit or bias
+ * of -inf or NaN takes an expert out (logits +inf count as the largest finite value); where
+ * fewer than `top` experts are left, ids are -1 and weights 0. */
+typedef struct ga_experts_route_args {
+    const void* logits;
+    const float* bias;
+    int* ids;
+    float* weights;
+    long long stride_logits;
+    int in_dtype, tokens, experts, top;
+    int scores, groups, top_groups, group_rank, renormalise;
+    float scale;
+} ga_experts_route_args;
+ga_status ga_experts_route(const ga_experts_route_args* args, void* stream);
+
+/* The map of rows: ids [tokens, top] contiguous; the experts first .. first + experts - 1
+ * are those of this call, other ids are left out.
+ *   starts     [experts + 1]
+ *   row_tokens [tokens * top]  the token of each sorted row, -1 from starts[experts] on
+ *   place      [tokens, top]   the row of each choice, -1 where it is left out
+ * Rows of an expert are in the order of their tokens and choices. starts, row_tokens and place may
+ * not overlap ids. */
+ga_status ga_experts_arrange(const int* ids, int tokens, int top, int experts, int first,
+                             int* starts, int* row_tokens, int* place, void* stream);
+
+/* out[r, n] = sum over 128-groups g of K of sfa[g, m] * sfb[e, n / 128, g] *
+ * sum over k in g of a[m, k] * b[e, n, k], for the rows r of expert e, m = rows_of[r], or r
+ * where rows_of is NULL: the block-scale product, each expert's rows with its weights.
+ *   a      [a_rows, k] E4M3, rows stride_a bytes apart
+ *   sfa    [k / 128, a_rows] fp32, rows stride_sfa elements apart
+ *   b      [experts, n, k] E4M3, experts stride_b_expert and rows stride_b bytes apart
+ *   sfb    [experts, ceil(n / 128), k / 128] fp32, strides in elements
+ *   starts [experts + 1]; rows from starts[experts] on are not written
+ *   out    [rows, n] bf16, rows stride_out elements apart
+ * k % 128 == 0; strides of a and b multiples of 16, both 16-byte aligned. A row of rows_of
+ * outside a counts as zeros; without rows_of a_rows must be at least rows. starts outside
+ * 0 .. rows are taken as the nearest of those, and an expert that ends before it starts has no
+ * rows; where starts decrease it is not said which of the rows' experts has written them.
+ * Limits: 256 rows of a or b, and with rows_of all of a, span at most 0xE0000000 bytes; sfa at most
+ * 4 GiB, with rows_of 0x0FFF0000 bytes. */
+typedef struct ga_experts_product_args {
+    const void* a;
+    const float* sfa;
+    const void* b;
+    const float* sfb;
+    const int* starts;
+    const int* rows_of;
+    void* out;
+    long long a_rows;
+    long long stride_a, stride_sfa;
+    long long stride_b_expert, stride_b;
+    long long stride_sfb_expert, stride_sfb;
+    long long stride_out;
+    int experts, rows, n, k;
+} ga_experts_product_args;
+ga_status ga_experts_product(const ga_experts_product_args* args, void* stream);
+
+/* Between an expert's products: x [rows, 2 * inner] (fp32 or bf16, rows stride_x elements
+ * apart), its first half the gate g, the second u: y = u * g / (1 + exp(-g)) in fp32, quantised
+ * as by ga_quant_fp8_1x128: q [rows, inner] E4M3 (rows stride_q bytes apart), scales
+ * [inner / 128, rows] (rows stride_scales elements apart). inner % 128 == 0; 16-byte loads
+ * where x and its stride allow. limit: device address of a row count (starts + experts), rows
+ * from it on are not looked at and nothing of theirs is written; NULL: all rows. */
+ga_status ga_experts_activate(const void* x, int in_dtype, int rows, int inner, long long stride_x,
+                              void* q, long long stride_q, float* scales, long long stride_scales,
+                              const int* limit, void* stream);
+
+/* out[t] = sum over j of weights[t, j] * y[place[t, j]] in fp32, in the order of j; a place
+ * outside [0, rows) is left out. y [rows, n] bf16, rows stride_y elements apart; place, weights
+ * [tokens, top] contiguous; out [tokens, n] bf16 or fp32, rows stride_out elements apart. */
+ga_status ga_experts_combine(const void* y, int rows, int n, long long stride_y, const int* place,
+                             const float* weights, int tokens, int top, void* out, int out_dtype,
+                             long long stride_out, void* stream);
+
 /* Device count of compute units of the current device (hipDeviceProp). */
 ga_status ga_device_num_cu(int* num_cu);
 
