@@ -32,6 +32,7 @@ GA_NAME_MAX = 96
 GA_EXPERTS_MAX = 1024
 GA_EXPERTS_MAX_TOP = 64
 GA_EXPERTS_MAX_GROUPS = 64
+GA_EXPERTS_CUTS = 8
 GA_EXPERTS_SOFTMAX = 0
 GA_EXPERTS_SIGMOID = 1
 # ga_mx_plan.kernel
@@ -228,7 +229,7 @@ class ExpertsProductArgs(ctypes.Structure):
                 ] + [(n, ctypes.c_longlong) for n in
                      ["a_rows", "stride_a", "stride_sfa", "stride_b_expert", "stride_b",
                       "stride_sfb_expert", "stride_sfb", "stride_out"]
-                     ] + [(n, ctypes.c_int) for n in ["experts", "rows", "n", "k"]]
+                     ] + [(n, ctypes.c_int) for n in ["experts", "rows", "n", "k", "cut"]]
 
 
 assert ctypes.sizeof(OpusGemmKargs) == 96
@@ -240,7 +241,7 @@ assert ctypes.sizeof(Mx4Cache) == 40
 assert ctypes.sizeof(Mx4AttentionArgs) == 136
 assert ctypes.sizeof(Mx4EvictArgs) == 136
 assert ctypes.sizeof(ExpertsRouteArgs) == 80
-assert ctypes.sizeof(ExpertsProductArgs) == 136
+assert ctypes.sizeof(ExpertsProductArgs) == 144
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int

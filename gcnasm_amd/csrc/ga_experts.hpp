@@ -21,53 +21,76 @@ struct ExpertTile {
     int before, tiles;
 };
 
-// The expert that tile t of those of all experts belongs to. First rows are taken as the nearest of
-// 0 .. rows, an expert whose end lies before its start has none. total: all tiles. Every lane of a
-// wave calls it, and everything it returns is uniform. t >= total: nothing.
-// A lane has a run of experts, one scan over the wave gives the tiles before them.
-__device__ __forceinline__ ExpertTile find_expert(const int* __restrict__ starts, int experts,
-                                                  int rows, int height, int lane, int t, int* total)
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int x)
 {
-    const int per = (experts + 63) / 64;
-    const int e0 = min(experts, lane * per), e1 = min(experts, e0 + per);
-    int mine = 0;
-    const int from = min(max(starts[e0], 0), rows);
-    int f = from;
-    for (int e = e0; e < e1; e++) {
-        const int to = min(max(starts[e + 1], 0), rows);
-        mine += (max(to - f, 0) + height - 1) / height;
-        f = to;
-    }
-    int upto = mine;
+    auto dpp = [](int v, auto ctrl, auto rows) {
+        return __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xF,
+                                           true);
+    };
+    using std::integral_constant;
+    x += dpp(x, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{}); // row_shr 1
+    x += dpp(x, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{}); // 2
+    x += dpp(x, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{}); // 4
+    x += dpp(x, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{}); // 8
+    x += dpp(x, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}); // row_bcast 15
+    x += dpp(x, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}); // row_bcast 31
+    return x;
+}
+
+// The tiles of all experts, and the expert of one of them. First rows are taken as the nearest of
+// 0 .. rows, an expert whose end lies before its start has none. Every lane of a wave calls it: a
+// lane has a run of P experts in registers, one scan over the wave gives the tiles before them.
+// pick(total) says which tile (uniform; outside 0 .. total - 1: none, and false is returned).
+template <int P, class Pick>
+__device__ __forceinline__ bool find_expert_run(const int* __restrict__ starts, int experts, int rows,
+                                                int height, int lane, const Pick& pick,
+                                                ExpertTile& x)
+{
+    int s[P + 1];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(upto, d, 64);
-        upto += lane >= d ? o : 0;
-    }
-    *total = __builtin_amdgcn_readlane(upto, 63);
-    ExpertTile x = {0, 0, 0, 0, 0};
-    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > t);
-    if (past == 0)
-        return x;
-    const int l = __builtin_ctzll(past);
-    // the run of lane l, again, by every lane
-    int e = __builtin_amdgcn_readlane(e0, l);
-    int before = __builtin_amdgcn_readlane(upto - mine, l);
-    f = __builtin_amdgcn_readlane(from, l);
-    for (;; e++) {
-        const int to = min(max(__builtin_amdgcn_readfirstlane(starts[e + 1]), 0), rows);
-        const int n = (max(to - f, 0) + height - 1) / height;
-        if (before + n > t) {
-            x.expert = e;
-            x.first = f;
-            x.last = to;
-            x.before = before;
-            x.tiles = n;
-            return x;
-        }
+    for (int i = 0; i <= P; i++)
+        s[i] = starts[min(lane * P + i, experts)];
+#pragma unroll
+    for (int i = 0; i <= P; i++)
+        s[i] = min(max(s[i], 0), rows);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < P; i++)
+        mine += (max(s[i + 1] - s[i], 0) + height - 1) / height;
+    const int upto = wave_scan(mine);
+    const int total = __builtin_amdgcn_readlane(upto, 63);
+    const int t = pick(total);
+    if (t < 0 || t >= total)
+        return false;
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > t));
+    int before = upto - mine;
+    ExpertTile o = {0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        const int n = (max(s[i + 1] - s[i], 0) + height - 1) / height;
+        if (before <= t && t < before + n)
+            o = {lane * P + i, s[i], s[i + 1], before, n};
         before += n;
-        f = to;
     }
+    x.expert = __builtin_amdgcn_readlane(o.expert, l);
+    x.first = __builtin_amdgcn_readlane(o.first, l);
+    x.last = __builtin_amdgcn_readlane(o.last, l);
+    x.before = __builtin_amdgcn_readlane(o.before, l);
+    x.tiles = __builtin_amdgcn_readlane(o.tiles, l);
+    return true;
+}
+
+template <class Pick>
+__device__ __forceinline__ bool find_expert(const int* __restrict__ starts, int experts, int rows,
+                                            int height, int lane, const Pick& pick, ExpertTile& x)
+{
+    static_assert(GA_EXPERTS_MAX <= 64 * 16, "a lane's run");
+    if (experts <= 64)
+        return find_expert_run<1>(starts, experts, rows, height, lane, pick, x);
+    if (experts <= 256)
+        return find_expert_run<4>(starts, experts, rows, height, lane, pick, x);
+    return find_expert_run<16>(starts, experts, rows, height, lane, pick, x);
 }
 
 } // namespace ga

@@ -7,12 +7,14 @@
 // its expert (ga_experts.hpp), those past the last tile end at once. Rows are gathered by the
 // copies into LDS, whose addresses are a lane's own.
 #include "ga_bs_decode.hpp"
+#include "ga_bs_pp.hpp"
 #include "ga_device.hpp"
 #include "ga_experts.hpp"
 #include "ga_internal.hpp"
 #include "ga_pp.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace ga {
 namespace {
@@ -36,21 +38,41 @@ __device__ __forceinline__ uint32_t row_offset(const ga_experts_product_args& a,
     return m >= 0 && m < a.a_rows ? (uint32_t)m * ld : kNowhere;
 }
 
+__device__ __forceinline__ uint2 bf16x4(const v4f& v)
+{
+    return make_uint2((uint32_t)f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
+                      (uint32_t)f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
+}
+
+// Four results of row m, columns n .. n + 3, those below N.
+__device__ __forceinline__ void expert_store4(uint16_t* out, long long ld, int m, int n, int N,
+                                              bool even, const v4f& v)
+{
+    uint16_t* o = out + (size_t)m * ld + n;
+    if (even && n + 4 <= N) {
+        *(uint2*)o = bf16x4(v);
+    } else {
+        for (int e = 0; e < 4 && n + e < N; e++)
+            o[e] = f32_to_bf16(v[e]);
+    }
+}
+
 // ---- few rows: weights streamed, K slices over the waves of a workgroup --------------
+constexpr int kFewWaves = 4;
+
 template <int TM, int NG>
-__global__ __attribute__((amdgpu_flat_work_group_size(64, 512), amdgpu_waves_per_eu(1, 2)))
+__global__ __attribute__((amdgpu_flat_work_group_size(64, 64 * kFewWaves), amdgpu_waves_per_eu(1, 2)))
 void experts_few_kernel(ga_experts_product_args a, int shares, int ks, int gps)
 {
     using Cfg = BdCfg<TM, NG>;
-    __shared__ __attribute__((aligned(1024))) char smem[8 * Cfg::kWave];
+    __shared__ __attribute__((aligned(1024))) char smem[kFewWaves * Cfg::kWave];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slice = wave % ks, tl = wave / ks;
-    int total;
     const int t = blockIdx.x / shares, share = blockIdx.x % shares;
-    const ExpertTile x = find_expert(a.starts, a.experts, a.rows, 16 * TM, lane, t, &total);
-    if (t >= total)
+    ExpertTile x;
+    if (!find_expert(a.starts, a.experts, a.rows, 16 * TM, lane, [&](int) { return t; }, x))
         return;
     const int row0 = x.first + (t - x.before) * 16 * TM;
     const int M = min(16 * TM, x.last - row0), N = a.n;
@@ -138,25 +160,19 @@ void experts_few_kernel(ga_experts_product_args a, int shares, int ks, int gps)
         const int m = i * 16 + r;
         if (c >= ng_here || n >= N || m >= M)
             return;
-        uint16_t* o = out + (size_t)m * a.stride_out + n;
-        if (even && n + 4 <= N) {
-            *(uint2*)o = make_uint2((uint32_t)f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
-                                    (uint32_t)f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
-        } else {
-            for (int e = 0; e < 4 && n + e < N; e++)
-                o[e] = f32_to_bf16(v[e]);
-        }
+        expert_store4(out, a.stride_out, m, n, N, even, v);
     };
     bd_join<TM, NG>(smem, wave, lane, slice, tl, ks, live, acc, store);
 }
 
 template <int TM, int NG>
-ga_status launch_few(const ga_experts_product_args& a, hipStream_t st)
+ga_status launch_few(const ga_experts_product_args& a, int ks, hipStream_t st)
 {
-    const int G = a.k / 128, groups = (a.n + 15) / 16;
-    const int ks = G >= 8 ? 4 : G >= 2 ? 2 : 1;
+    const int G = a.k / 128, groups = (a.n - 1) / 16 + 1;
+    while (ks > G)
+        ks /= 2;
     const int gps = (G + ks - 1) / ks;
-    const int tasks = std::min(8 / ks, (groups + NG - 1) / NG);
+    const int tasks = std::min(kFewWaves / ks, (groups + NG - 1) / NG);
     const int shares = (groups + tasks * NG - 1) / (tasks * NG);
     const long long grid = most_expert_tiles(a.rows, a.experts, 16 * TM) * shares;
     if (grid > most_workgroups(64 * tasks * ks))
@@ -165,6 +181,317 @@ ga_status launch_few(const ga_experts_product_args& a, hipStream_t st)
                        st, a, shares, ks, gps);
     GA_HIP_CHECK(hipGetLastError());
     return GA_OK;
+}
+
+// ---- many rows: eight-wave tiles -------------------------------------------------------
+// The chains of the dense kernels (ga_bs_pp.hpp), with rows gathered: a lane of the copies has a row
+// offset for each 64 rows of the tile.
+template <bool GATHER>
+struct ExpertLoad : bspp::BsLoad {
+    uint32_t vrow[4];
+};
+
+template <bool GATHER>
+__device__ __forceinline__ void issue_a(const ExpertLoad<GATHER>& L, char* smem, int h, int t,
+                                        int wave)
+{
+    if constexpr (!GATHER) {
+        bspp::issue_a((const bspp::BsLoad&)L, smem, h, t, wave);
+    } else {
+        char* dst = smem + pp::kARegion + (t & 1) * pp::kOpSlot + h * pp::kHalf + wave * 1024;
+        const uint32_t o = pp::uni((uint32_t)t * 128);
+        lds_load16(L.ra, (lds_void*)dst, L.vrow[2 * h], o);
+        lds_load16(L.ra, (lds_void*)(dst + 8192), L.vrow[2 * h + 1], o);
+    }
+}
+
+template <int NB, int MODE, bool GATHER>
+__device__ __forceinline__ void issue_half(const ExpertLoad<GATHER>& L, char* smem, int t, int slot,
+                                           int wave)
+{
+    using H = bspp::BsHalfCfg<NB>;
+    if constexpr (!GATHER) {
+        bspp::issue_half<NB, MODE>((const bspp::BsLoad&)L, smem, t, slot, wave);
+    } else {
+        char* dst = smem + slot * H::kSlot + wave * 1024;
+        const uint32_t o = (uint32_t)t * 128;
+        lds_load16(L.ra, (lds_void*)dst, L.vrow[0] + pp::uni(o), 0);
+        lds_load16(L.ra, (lds_void*)(dst + 8192), L.vrow[1] + pp::uni(o), 0);
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++)
+            lds_load16(L.rb, (lds_void*)(dst + pp::kHalf + c * 8192),
+                       L.vb + pp::uni(o + c * L.b_hstep), 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            L.rs,
+            (lds_void*)(smem + H::kScaleBase + (t & (H::kRing - 1)) * bspp::kSSlot + wave * 256), 4,
+            L.vs + pp::uni((uint32_t)t * L.s_kstep), 0, 0, 0);
+    }
+}
+
+// The copies of the tile of M rows from row0 on, columns from n0 on.
+template <int ROWS, bool GATHER>
+__device__ __forceinline__ void expert_load_setup(const ga_experts_product_args& a, int expert,
+                                                  int row0, int M, int n0, int wave, int lane,
+                                                  ExpertLoad<GATHER>& L)
+{
+    const uint32_t lda = (uint32_t)a.stride_a, ldb = (uint32_t)a.stride_b;
+    const int N = a.n, G = a.k / 128;
+    int crow, ckc;
+    pp::copy_lane(wave, lane, crow, ckc);
+    L.ra = make_rsrc((const char*)a.a + (GATHER ? 0 : (size_t)row0 * lda),
+                     rows_bytes(GATHER ? a.a_rows : M, lda, a.k));
+    L.va = (uint32_t)crow * lda + ckc * 16;
+    L.a_hstep = 64 * lda;
+    if constexpr (GATHER)
+#pragma unroll
+        for (int i = 0; i < ROWS / 64; i++)
+            L.vrow[i] = row_offset(a, row0, M, i * 64 + crow, lda) + ckc * 16;
+    L.rb = make_rsrc((const char*)a.b + (size_t)expert * a.stride_b_expert + (size_t)n0 * ldb,
+                     rows_bytes(N - n0, ldb, a.k));
+    L.vb = (uint32_t)crow * ldb + ckc * 16;
+    L.b_hstep = 64 * ldb;
+    if (wave < 4) {
+        // position w*64 + l holds row w*64 + (l%4)*16 + l/4, those past M the last one
+        L.rs = make_rsrc(a.sfa + (GATHER ? 0 : row0),
+                         rows_bytes_f32(G, a.stride_sfa, GATHER ? a.a_rows : M));
+        L.vs = row_offset(a, row0, M, min(wave * 64 + (lane & 3) * 16 + (lane >> 2), M - 1), 4);
+        L.s_kstep = (uint32_t)a.stride_sfa * 4;
+    } else {
+        const int nblk = (N + 127) / 128;
+        L.rs = make_rsrc(a.sfb + (size_t)expert * a.stride_sfb_expert,
+                         rows_bytes_f32(nblk, a.stride_sfb, G));
+        L.vs = (uint32_t)min(n0 / 128 + (lane & 1), nblk - 1) * (uint32_t)a.stride_sfb * 4;
+        L.s_kstep = 4;
+    }
+}
+
+__device__ __forceinline__ bspp::BsRead expert_read_setup(char* smem, int lane, int grp, int simd,
+                                                          int b_region, int scales)
+{
+    bspp::BsRead rb;
+    uint32_t o, o64;
+    pp::operand_lane(lane, o, o64);
+    rb.a0 = smem + grp * 64 * 128 + o;
+    rb.a1 = smem + grp * 64 * 128 + o64;
+    rb.b0 = smem + b_region + simd * 32 * 128 + o;
+    rb.b1 = smem + b_region + simd * 32 * 128 + o64;
+    rb.sa = smem + scales + grp * 256 + (lane & 15) * 16;
+    rb.sb = smem + scales + 1024;
+    return rb;
+}
+
+// A tile's results to out: quadrant q of ROWS / 128 * NB, rows first, `result(q, i, t)` of its 16x16
+// tile i, t: lane l holds row l % 16, columns 4 (l / 16) on. Through LDS, so that whole rows are
+// written (rows below M; columns below N, a multiple of 8), where out is aligned for it.
+template <int ROWS, int NB, class Result>
+__device__ __forceinline__ void expert_store(const ga_experts_product_args& a, char* smem, int row0,
+                                             int M, int n0, int wave, int lane, const Result& result)
+{
+    const int grp = wave >> 2, simd = wave & 3, N = a.n - n0;
+    const long long ld = a.stride_out;
+    uint16_t* out = (uint16_t*)a.out + (size_t)row0 * ld + n0;
+    const bool wide = ((uintptr_t)a.out & 15) == 0 && (ld & 7) == 0 && (N & 7) == 0;
+    const bool even = ((uintptr_t)a.out & 7) == 0 && (ld & 3) == 0;
+    if (wide)
+        barrier_lds(); // every wave's operand and scale reads are done
+#pragma unroll
+    for (int q = 0; q < ROWS / 128 * NB; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int m = q / NB * 128 + grp * 64 + i * 16 + (lane & 15);
+                const int n = q % NB * 128 + simd * 32 + t * 16 + (lane >> 4) * 4;
+                if (wide)
+                    *(uint2*)(smem + m * pp::kStagePitch + n * 2) = bf16x4(result(q, i, t));
+                else if (m < M && n < N)
+                    expert_store4(out, ld, m, n, N, even, result(q, i, t));
+            }
+    if (!wide)
+        return;
+    barrier_lds();
+    constexpr int kLanes = NB * 16; // lanes of a row
+#pragma unroll
+    for (int it = 0; it < ROWS / 8 * kLanes / 64; it++) {
+        const int row = wave * (ROWS / 8) + it * (64 / kLanes) + lane / kLanes;
+        const int col = lane % kLanes * 8;
+        if (row < M && col < N)
+            *(v4i*)(out + (size_t)row * ld + col) =
+                *(const v4i*)(smem + row * pp::kStagePitch + col * 2);
+    }
+}
+
+// Which tile a workgroup has: XCD by XCD a run of tiles, an expert's column by column within
+// bands of `band` row tiles, so that what runs at a time on an XCD shares weights and rows in its L2.
+// False: none.
+__device__ __forceinline__ bool expert_tile(const ga_experts_product_args& a, int height, int tn,
+                                            int lane, int band, ExpertTile& x, int& tile_m,
+                                            int& tile_n)
+{
+    int lin = blockIdx.x;
+    auto pick = [&](int tiles) { // the grid has most_expert_tiles() * tn workgroups, an int
+        const int total = tiles * tn;
+        if (lin >= total)
+            return -1;
+        if (lin < total / 8 * 8)
+            lin = lin % 8 * (total / 8) + lin / 8;
+        return lin / tn;
+    };
+    if (!find_expert(a.starts, a.experts, a.rows, height, lane, pick, x))
+        return false;
+    const int r = lin - x.before * tn;
+    const int first = r / (band * tn) * band;
+    const int q = r - first * tn, h = min(x.tiles - first, band);
+    tile_m = first + q % h;
+    tile_n = q / h;
+    return true;
+}
+
+constexpr int kExpertBand = 4;
+
+// A tile of 128 rows (M of them there) and NB * 128 columns.
+template <int NB, bool GATHER>
+__device__ __forceinline__ void expert_half_tile(const ga_experts_product_args& a, char* smem,
+                                                 int expert, int row0, int M, int n0, int wave,
+                                                 int lane)
+{
+    using namespace bspp;
+    using H = BsHalfCfg<NB>;
+    const int grp = wave >> 2, simd = wave & 3;
+    v4f acc[NB][4][2];
+#pragma unroll
+    for (int q = 0; q < NB; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                acc[q][i][t] = (v4f){0.f, 0.f, 0.f, 0.f};
+    ExpertLoad<GATHER> L;
+    expert_load_setup<128>(a, expert, row0, M, n0, wave, lane, L);
+    const BsRead rb = expert_read_setup(smem, lane, grp, simd, pp::kHalf, H::kScaleBase);
+    bs_half_chain<NB, PS_GROUP128>(L, rb, smem, a.k / 128, wave, grp, acc);
+    expert_store<128, NB>(a, smem, row0, M, n0, wave, lane, [&](int q, int i, int t) {
+        return acc[q][i][t];
+    });
+}
+
+// 256x256 tiles; of an expert's last, if at most 128 rows are left, the upper half alone.
+template <bool GATHER>
+__global__ __attribute__((amdgpu_flat_work_group_size(pp::kNT, pp::kNT), amdgpu_waves_per_eu(2, 2)))
+void experts_tile_kernel(ga_experts_product_args a, int tn)
+{
+    using namespace bspp;
+    constexpr int kLds = kLdsBs > BsHalfCfg<2>::kLds ? kLdsBs : BsHalfCfg<2>::kLds;
+    __shared__ __attribute__((aligned(1024))) char smem[kLds];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave >> 2, simd = wave & 3;
+    ExpertTile x;
+    int tile_m, tile_n;
+    if (!expert_tile(a, 256, tn, lane, kExpertBand, x, tile_m, tile_n))
+        return;
+    const int row0 = x.first + tile_m * 256, n0 = tile_n * 256;
+    const int M = min(256, x.last - row0);
+    if (M <= 128) {
+        expert_half_tile<2, GATHER>(a, smem, x.expert, row0, M, n0, wave, lane);
+        return;
+    }
+
+    v4f acc[4][4][2];
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                acc[q][i][t] = (v4f){0.f, 0.f, 0.f, 0.f};
+    ExpertLoad<GATHER> L;
+    expert_load_setup<256>(a, x.expert, row0, M, n0, wave, lane, L);
+    const BsRead rb = expert_read_setup(smem, lane, grp, simd, kBRegion, kSBase);
+    bs_pp_chain<PS_GROUP128>(L, rb, smem, a.k / 128, wave, grp, acc);
+    expert_store<256, 2>(a, smem, row0, M, n0, wave, lane, [&](int q, int i, int t) {
+        return acc[q][i][t];
+    });
+}
+
+template <int NB, bool GATHER>
+__global__ __attribute__((amdgpu_flat_work_group_size(pp::kNT, pp::kNT), amdgpu_waves_per_eu(2, 2)))
+void experts_half_kernel(ga_experts_product_args a, int tn)
+{
+    __shared__ __attribute__((aligned(1024))) char smem[bspp::BsHalfCfg<NB>::kLds];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    ExpertTile x;
+    int tile_m, tile_n;
+    if (!expert_tile(a, 128, tn, lane, kExpertBand, x, tile_m, tile_n))
+        return;
+    const int row0 = x.first + tile_m * 128;
+    expert_half_tile<NB, GATHER>(a, smem, x.expert, row0, min(128, x.last - row0),
+                                 tile_n * 128 * NB, wave, lane);
+}
+
+template <bool GATHER>
+ga_status launch_tiles(const ga_experts_product_args& a, int height, int width, hipStream_t st)
+{
+    const int tn = (a.n - 1) / width + 1;
+    const long long grid = most_expert_tiles(a.rows, a.experts, height) * tn;
+    if (grid > most_workgroups(pp::kNT))
+        return fail(GA_ERR_SHAPE, "experts_product: too many tiles for one call");
+    const dim3 g((unsigned)grid), b(pp::kNT);
+    if (height == 256)
+        hipLaunchKernelGGL((experts_tile_kernel<GATHER>), g, b, 0, st, a, tn);
+    else if (width == 256)
+        hipLaunchKernelGGL((experts_half_kernel<2, GATHER>), g, b, 0, st, a, tn);
+    else
+        hipLaunchKernelGGL((experts_half_kernel<1, GATHER>), g, b, 0, st, a, tn);
+    GA_HIP_CHECK(hipGetLastError());
+    return GA_OK;
+}
+
+// How a product is cut: a workgroup's rows and columns, its slices of K (0: an eight-wave tile),
+// how many a CU has at a time, its start and its time for a 128-K step in us.
+struct ExpertCut {
+    int height, width, ks, at_once;
+    float start, step;
+};
+
+// The cut with the smallest estimated time. The counts are on the GPU, so the tiles are those of
+// rows spread over the experts by chance. A call's time is that of its rounds of workgroups,
+// but at least what its bytes take from memory (active weights, rows, results) and what all its
+// copies take from the caches. The coefficients are a fit to 1491 problems measured on MI355X with
+// every cut (2-256 experts, 1-800 rows each, N 100-7168, K 256-7168): the cut it picks is on
+// average 2.5 % slower than the fastest, at the worst 1.6 times (few rows of 2 experts). One
+// cut for all would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take 132
+// us in 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in
+// 16x32, 62 in 128x256, 83 in 256x256; 64 of 4096x4096 with 1024 rows 3490 in 16x256, 1330 in
+// 128x256, 1150 in 256x256.
+const ExpertCut& expert_cut(const ga_experts_product_args& a, int num_cu)
+{
+    static const ExpertCut kCuts[GA_EXPERTS_CUTS] = {
+        {16, 64, 2, 2, 4.35f, 0.17f}, {16, 32, 4, 2, 2.53f, 0.25f}, {16, 256, 1, 2, 2.71f, 0.35f},
+        {64, 256, 1, 2, 6.25f, 0.76f}, {64, 64, 4, 2, 4.51f, 0.66f}, {128, 128, 0, 1, 2.83f, 0.46f},
+        {128, 256, 0, 1, 5.01f, 0.81f}, {256, 256, 0, 1, 6.14f, 0.94f}};
+    if (a.cut)
+        return kCuts[a.cut - 1];
+    const float n = (float)a.n, k = (float)a.k, rows = (float)a.rows;
+    const float active = a.experts * (1.0f - std::exp(-rows / a.experts));
+    const float memory = (active * n * k + 0.25f * rows * k + 2.0f * rows * n) / 6.0e6f;
+    const ExpertCut* best = nullptr;
+    float least = 0.0f;
+    for (const ExpertCut& c : kCuts) {
+        const float tiles = std::max(active, rows / c.height + 0.5f * active);
+        const float groups = tiles * ((a.n - 1) / c.width + 1);
+        const int slices = std::max(1, c.ks), steps = (a.k / 128 + slices - 1) / slices;
+        const float rounds = std::max(1.0f, groups / (num_cu * c.at_once));
+        const float copies = groups * k * (std::min((float)c.width, n) +
+                                           std::min((float)c.height, rows / active)) / 12.0e6f;
+        const float t = std::max(rounds * (c.start + steps * c.step), std::max(memory, copies));
+        if (!best || t < least) {
+            best = &c;
+            least = t;
+        }
+    }
+    return *best;
 }
 
 } // namespace
@@ -177,7 +504,8 @@ extern "C" ga_status ga_experts_product(const ga_experts_product_args* args, voi
     if (!args)
         return fail(GA_ERR_ARG, "experts_product: null argument");
     const ga_experts_product_args& a = *args;
-    if (a.experts <= 0 || a.rows < 0 || a.n <= 0 || a.k <= 0 || a.a_rows < 0)
+    if (a.experts <= 0 || a.rows < 0 || a.n <= 0 || a.k <= 0 || a.a_rows < 0 || a.cut < 0 ||
+        a.cut > GA_EXPERTS_CUTS)
         return fail(GA_ERR_ARG, "experts_product: bad count");
     if (a.experts > GA_EXPERTS_MAX)
         return fail(GA_ERR_SHAPE, "experts_product: more than %d experts", GA_EXPERTS_MAX);
@@ -209,10 +537,15 @@ extern "C" ga_status ga_experts_product(const ga_experts_product_args* args, voi
         return fail(GA_ERR_SHAPE, "experts_product: scales pass 4 GiB, or 0x0FFF0000 bytes with "
                                   "gathered rows");
     hipStream_t st = (hipStream_t)stream;
-    const long long each = ((long long)a.rows + a.experts - 1) / a.experts;
-    if (each <= 16)
-        return launch_few<1, 2>(a, st);
-    if (each <= 32)
-        return launch_few<2, 2>(a, st);
-    return launch_few<4, 4>(a, st);
+    int num_cu = 0;
+    const ga_status status = device_cu_count(&num_cu);
+    if (status != GA_OK)
+        return status;
+    const ExpertCut& c = expert_cut(a, num_cu);
+    if (c.ks == 0)
+        return a.rows_of ? launch_tiles<true>(a, c.height, c.width, st)
+                         : launch_tiles<false>(a, c.height, c.width, st);
+    if (c.height == 64)
+        return launch_few<4, 4>(a, c.ks, st);
+    return c.ks == 1 ? launch_few<1, 4>(a, c.ks, st) : launch_few<1, 2>(a, c.ks, st);
 }

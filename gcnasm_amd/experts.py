@@ -132,7 +132,7 @@ def arrange(ids, experts, first=0, stream=None):
     return starts, tokens, place
 
 
-def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None):
+def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None, cut=0):
     """Each expert's rows times its weights: out[r] = a[m] b[e]^T (bfloat16), m = rows[r] or,
     without rows, r; e the expert with starts[e] <= r < starts[e + 1].
 
@@ -140,8 +140,9 @@ def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None):
     [experts, N, K], sfb float32 [experts, ceil(N / 128), K / 128] (ops.quant_fp8_128x128);
     starts int32 [experts + 1] and rows int32 [R] as arrange() gives them. out [R, N]
     (without rows R = A); its rows from starts[-1] on are left as they are. A row outside a
-    counts as zeros. Sums are fp32, in the order of K (for few rows of an expert in up to 8
-    pieces)."""
+    counts as zeros. Sums are fp32, in the order of K (for few rows of an expert in up to 4
+    pieces). cut: 0, or 1 .. GA_EXPERTS_CUTS for one of the ways of cutting the product in place
+    of the one that its sizes choose (include/gcnasm_amd.h), for callers that tune."""
     count, k = _matrix(a, "a")
     device = _gpu(a, "a")
     sa = _check(a, "a", torch.uint8, a.shape, device)[0]
@@ -168,7 +169,7 @@ def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None):
         a.data_ptr(), sfa.data_ptr(), b.data_ptr(), sfb.data_ptr(), starts.data_ptr(), ptr,
         out.data_ptr(), count, sa if count > 1 else k, ssa if k > 128 else count,
         sb[0] if experts > 1 else 0, sb[1] if n > 1 else k, ssb[0] if experts > 1 else 0,
-        ssb[1] if n > 128 else k // 128, so if total > 1 else n, experts, total, n, k),
+        ssb[1] if n > 128 else k // 128, so if total > 1 else n, experts, total, n, k, cut),
         _stream(stream, device)))
     return out
 

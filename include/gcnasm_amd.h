@@ -733,6 +733,7 @@ ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args,
 #define GA_EXPERTS_MAX 1024     /* experts of a call                            */
 #define GA_EXPERTS_MAX_TOP 64   /* choices of a token                           */
 #define GA_EXPERTS_MAX_GROUPS 64
+#define GA_EXPERTS_CUTS 8       /* ways to cut a product                        */
 #define GA_EXPERTS_SOFTMAX 0
 #define GA_EXPERTS_SIGMOID 1
 
@@ -785,6 +786,11 @@ ga_status ga_experts_arrange(const int* ids, int tokens, int top, int experts, i
  * outside a counts as zeros; without rows_of a_rows must be at least rows. starts outside
  * 0 .. rows are taken as the nearest of those, and an expert that ends before it starts has no
  * rows; where starts decrease it is not said which of the rows' experts has written them.
+ * cut: 0, or one of 1 .. GA_EXPERTS_CUTS to run that way of cutting the product (rows x columns
+ * of a workgroup: 1 16x64, 2 16x32, 3 16x256, 4 64x256, 5 64x64, 6 128x128, 7 128x256, 8 256x256) in
+ * place of the one that the sizes choose. K is summed in 128-groups in order, by the cuts 1, 2 and
+ * 5 in 2, 4 and 4 pieces (fewer where K has fewer groups) that are added in order; otherwise the
+ * cuts give the same results.
  * Limits: 256 rows of a or b, and with rows_of all of a, span at most 0xE0000000 bytes; sfa at most
  * 4 GiB, with rows_of 0x0FFF0000 bytes. */
 typedef struct ga_experts_product_args {
@@ -801,6 +807,7 @@ typedef struct ga_experts_product_args {
     long long stride_sfb_expert, stride_sfb;
     long long stride_out;
     int experts, rows, n, k;
+    int cut;
 } ga_experts_product_args;
 ga_status ga_experts_product(const ga_experts_product_args* args, void* stream);
 

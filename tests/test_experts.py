@@ -50,14 +50,14 @@ def test_arrangements_that_are_refused():
 
 def product(**kw):
     a = _lib.ExpertsProductArgs(0x1000, 0x2000, 0x3000, 0x4000, 0x5000, 0x6000, 0x7000, 10, 256, 10,
-                                300 * 256, 256, 6, 2, 300, 4, 20, 300, 256)
+                                300 * 256, 256, 6, 2, 300, 4, 20, 300, 256, 0)
     return _lib.lib().ga_experts_product(ctypes.byref(set_all(a, kw)), None)
 
 
 @pytest.mark.parametrize("change,status", [
     (dict(a=None), ARG), (dict(sfa=None), ARG), (dict(b=None), ARG), (dict(sfb=None), ARG),
     (dict(starts=None), ARG), (dict(out=None), ARG), (dict(experts=0), ARG), (dict(rows=-1), ARG),
-    (dict(n=0), ARG), (dict(k=0), ARG), (dict(a_rows=-1), ARG), (dict(experts=1025), SHAPE),
+    (dict(n=0), ARG), (dict(k=0), ARG), (dict(cut=-1), ARG), (dict(cut=9), ARG), (dict(a_rows=-1), ARG), (dict(experts=1025), SHAPE),
     (dict(k=192), _lib.GA_ERR_GROUP), (dict(a_rows=0), SHAPE), (dict(rows_of=None), SHAPE),
     (dict(a=0x1008), SHAPE), (dict(b=0x3004), SHAPE), (dict(stride_a=264), SHAPE),
     (dict(stride_b=264), SHAPE), (dict(stride_b_expert=300 * 256 + 8), SHAPE),

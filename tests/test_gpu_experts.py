@@ -139,20 +139,22 @@ def operands(rows, experts, n, k, seed):
     return a, sfa, b, sfb
 
 
-def check_product(dev, a, sfa, b, sfb, starts, rows=None, label=""):
+def check_product(dev, a, sfa, b, sfb, starts, rows=None, label="", cuts=(0,)):
     total = a.shape[0] if rows is None else len(rows)
-    out = torch.full((total, b.shape[1]), 77.0, dtype=torch.bfloat16, device=dev)
-    got = ex.product(on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev),
-                     on(np.asarray(starts, np.int32), dev),
-                     None if rows is None else on(np.asarray(rows, np.int32), dev), out=out)
-    assert got is out
     want, mass, written = H.product(a, sfa, b, sfb, starts, rows)
-    bits = host(out.view(torch.int16)).view(np.uint16)
-    assert (bits[~written] == 0x429A).all(), "rows that are nobody's have been written"
-    _, st = bf16_compare(bits[written], want[written], mass[written])
-    assert_parity(st, "product %s" % label)
+    args = [on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev), on(np.asarray(starts, np.int32), dev),
+            None if rows is None else on(np.asarray(rows, np.int32), dev)]
+    for cut in cuts:
+        out = torch.full((total, b.shape[1]), 77.0, dtype=torch.bfloat16, device=dev)
+        got = ex.product(*args, out=out, cut=cut)
+        assert got is out
+        bits = host(out.view(torch.int16)).view(np.uint16)
+        assert (bits[~written] == 0x429A).all(), "rows that are nobody's have been written"
+        _, st = bf16_compare(bits[written], want[written], mass[written])
+        assert_parity(st, "product %s cut %d" % (label, cut))
 
 
+CUTS = range(_lib.GA_EXPERTS_CUTS + 1)  # 0: what the sizes choose
 COUNTS = {  # rows of each expert
     "one": [1], "single": [0, 1, 0, 0, 1, 1, 0], "few": [3, 0, 16, 17, 1, 15], "wave": [33, 64, 0, 65],
     "tile": [128, 1, 129, 127, 0], "large": [300, 0, 513, 256, 255], "skewed": [1, 700, 2, 0, 0, 3]}
@@ -175,7 +177,7 @@ def test_product(dev, counts, n, k, gathered):
         rows[rng.random(total) < 0.05] = m
         rows[rng.random(total) < 0.02] = 2 ** 31 - 1
         rows[rng.random(total) < 0.02] = -2 ** 31
-    check_product(dev, a, sfa, b, sfb, starts, rows, "%s %dx%d" % (counts, n, k))
+    check_product(dev, a, sfa, b, sfb, starts, rows, "%s %dx%d" % (counts, n, k), CUTS)
 
 
 @pytest.mark.parametrize("experts", [63, 64, 65, 130, 1024])
@@ -184,14 +186,14 @@ def test_product_of_many_experts(dev, experts):
     c = rng.integers(0, 4, experts)
     starts = np.concatenate([[0], np.cumsum(c)])
     a, sfa, b, sfb = operands(int(starts[-1]), experts, 32, 256, seed=experts)
-    check_product(dev, a, sfa, b, sfb, starts, None, "%d experts" % experts)
+    check_product(dev, a, sfa, b, sfb, starts, None, "%d experts" % experts, CUTS)
 
 
 @pytest.mark.parametrize("starts", [[-5, 3, 3, 9, 40], [0, 0, 0, 0, 0], [7, 7, 12, 12, 2 ** 31 - 1],
                                     [-2 ** 31, -1, 4, 4, 20], [20, 20, 21, 22, 23]])
 def test_product_keeps_first_rows_inside(dev, starts):
     a, sfa, b, sfb = operands(20, 4, 48, 256, seed=4)
-    check_product(dev, a, sfa, b, sfb, starts, None, str(starts))
+    check_product(dev, a, sfa, b, sfb, starts, None, str(starts), CUTS)
 
 
 @pytest.mark.parametrize("starts", [[-5, 3, 2, 9, 40], [7, 7, 30, 11, 20], [100, 200, 5, -1, 8],
@@ -199,9 +201,14 @@ def test_product_keeps_first_rows_inside(dev, starts):
 def test_product_of_first_rows_that_decrease(dev, starts):
     """Each row is one of its experts', or has been left: nothing is written elsewhere."""
     a, sfa, b, sfb = operands(20, 4, 48, 256, seed=4)
+    for cut in CUTS:
+        check_decreasing(dev, a, sfa, b, sfb, starts, cut)
+
+
+def check_decreasing(dev, a, sfa, b, sfb, starts, cut):
     guarded = torch.full((60, 48), 77.0, dtype=torch.bfloat16, device=dev)
     ex.product(on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev),
-               on(np.array(starts, np.int32), dev), out=guarded[20:40])
+               on(np.array(starts, np.int32), dev), out=guarded[20:40], cut=cut)
     got = host(guarded.float())
     assert (got[:20] == 77).all() and (got[40:] == 77).all()
     right = got[20:40] == 77
@@ -225,16 +232,15 @@ def test_product_of_strided_operands(dev):
     B[:, :136, :384] = on(b, dev)
     T = torch.zeros((3, 4, 7), device=dev)
     T[:, :2, :3] = on(sfb, dev)
-    for width, first in ((140, 0), (143, 1)):  # out's rows aligned, and not
+    for (width, first), cut in itertools.product(((144, 0), (140, 0), (143, 1)), CUTS):
         O = torch.full((49, width), 5.0, dtype=torch.bfloat16, device=dev)
         out = O[:, first:first + 136]
-        ex.product(A[:, :384], S[:, :49], B[:, :136, :384], T[:, :2, :3], starts, out=out)
+        ex.product(A[:, :384], S[:, :49], B[:, :136, :384], T[:, :2, :3], starts, out=out, cut=cut)
         bits = host(out.contiguous().view(torch.int16)).view(np.uint16)
         _, st = bf16_compare(bits, want, mass)
         assert_parity(st, "strided")
         O[:, first:first + 136] = 5.0
         assert (O == 5.0).all()  # nothing beside
-    del c
 
 
 def test_product_scales_with_infinity_stay_in_their_rows(dev):
@@ -243,11 +249,12 @@ def test_product_scales_with_infinity_stay_in_their_rows(dev):
     sfa = sfa.copy()
     sfa[0, 0], sfa[1, 1] = np.inf, np.nan
     rows = np.array([2, -1, 0, 3, 1, 99, 4, 5], np.int32)
-    out = host(ex.product(on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev),
-                          on(np.array([0, 5, 8], np.int32), dev), on(rows, dev)).float())
-    clean = np.array([0, 1, 3, 5, 6, 7])
-    assert np.isfinite(out[clean]).all() and not np.isfinite(out[[2, 4]]).any()
-    assert (out[[1, 5]] == 0).all()
+    for cut in CUTS:
+        out = host(ex.product(on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev),
+                              on(np.array([0, 5, 8], np.int32), dev), on(rows, dev), cut=cut).float())
+        clean = np.array([0, 1, 3, 5, 6, 7])
+        assert np.isfinite(out[clean]).all() and not np.isfinite(out[[2, 4]]).any()
+        assert (out[[1, 5]] == 0).all()
 
 
 # ---- activate --------------------------------------------------------------------------
@@ -458,8 +465,9 @@ def test_results_do_not_change_from_call_to_call(dev):
     ids = on(rng.integers(0, 9, (400, 3)).astype(np.int32), dev)
     starts, tokens, _ = ex.arrange(ids, 9)
     a, sfa, b, sfb = (on(v, dev) for v in operands(400, 9, 200, 512, seed=3))
-    outs = [ex.product(a, sfa, b, sfb, starts, tokens) for _ in range(5)]
-    assert all(torch.equal(outs[0], o) for o in outs[1:])
+    for cut in CUTS:
+        outs = [ex.product(a, sfa, b, sfb, starts, tokens, cut=cut) for _ in range(5)]
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
 
 
 # ---- refusals ----------------------------------------------------------------------------
