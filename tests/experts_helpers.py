@@ -51,12 +51,13 @@ def route(logits, top, bias=None, kind="softmax", groups=1, top_groups=None, gro
         ids[t, :len(chosen)] = chosen
         if not chosen:
             continue
-        if renormalise and kind == "softmax":  # where all the chosen scores vanish too
-            c = np.exp(x[t, chosen] - x[t, chosen].max())
-        else:
-            c = p[t, chosen]
-        if renormalise:
-            c = c / c.sum() if c.sum() > 0 else np.zeros_like(c)
+        c, z = p[t, chosen], x[t, chosen]
+        if renormalise:  # relative to the largest one, where all the chosen scores vanish too
+            if kind == "softmax":
+                c = np.exp(z - z.max())
+            else:
+                c = np.exp(np.minimum(z, 0) - min(z.max(), 0)) / (1 + np.exp(-np.abs(z)))
+            c = c / c.sum()
         w[t, :len(chosen)] = c * scale
     return ids, w
 
