@@ -268,12 +268,14 @@ def check_activate(x, q, s, live=None):
     live = len(x) if live is None else live
     y, want = H.activate(x[:live])
     q, s = host(q)[:live], host(s)[:, :live]
-    # exp within 2 ulp, sum, quotient and product rounded: 2^-21 in all; the scale's division 2^-24
-    assert (np.abs(s - want) <= 2.0 ** -20 * want).all()
+    # an element: the exponential's argument and its base's, |g| 2^-22.6, four roundings and two
+    # results of the hardware's, 2^-21; a scale: that of one of its elements, and its division
+    off = np.minimum(np.abs(x[:live, :x.shape[1] // 2]), 200) * 2.0 ** -22.5 + 2.0 ** -20.5
+    assert (np.abs(s - want) <= off.reshape(live, -1, 128).max(2).T * want).all()
     v = oracle.e4m3_decode_table()[q].astype(np.float64)
     r = y / np.repeat(s.T.astype(np.float64), 128, 1)
     # the nearest code: half a step of its binade (2^-4 of a value, 2^-10 below 2^-6), and r's error
-    assert (np.abs(v - r) <= np.maximum(np.abs(r) * 2.0 ** -4, 2.0 ** -10) + np.abs(r) * 2.0 ** -19).all()
+    assert (np.abs(v - r) <= np.maximum(np.abs(r) * 2.0 ** -4, 2.0 ** -10) + np.abs(r) * 2 * off).all()
 
 
 @pytest.mark.parametrize("rows,inner", [(1, 128), (5, 256), (31, 128), (32, 384), (33, 1408),
