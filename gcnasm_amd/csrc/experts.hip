@@ -45,6 +45,10 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t a)
 {
     return wave_all(a, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u);
 }
+__device__ __forceinline__ float wave_max(float a)
+{
+    return wave_all(a, [](float x, float y) { return fmaxf(x, y); }, -__builtin_inff());
+}
 __device__ __forceinline__ float wave_sum(float a)
 {
     return wave_all(a, [](float x, float y) { return x + y; }, 0.0f);
@@ -93,16 +97,24 @@ __device__ __forceinline__ float score_of(float x, bool softmax, float largest)
     return softmax ? __expf(x - largest) : __builtin_amdgcn_rcpf(1.0f + __expf(-x));
 }
 
-// The groups that are kept, a bit at each one's first lane (group << shift), by the values of the
-// lanes' experts in LDS; sure: no other group is within `margin` of a kept one.
-template <class T>
-__device__ __forceinline__ uint64_t kept_groups(const ga_experts_route_args& a, const T* by, int lane,
-                                                int shift, T margin, bool& sure)
+// A number and an index in one integer: of the larger number, of equal ones the lower index is the
+// larger. Numbers from `top` (the largest) down to top - 2^22 / steps become steps, those below
+// step 1; 0 is nothing.
+__device__ __forceinline__ uint32_t packed(float x, float top, float steps, int index)
 {
-    const T none = (T)kMinus;
+    const float d = 4194303.0f - (top - x) * steps;
+    return (uint32_t)fmaxf(d, 1.0f) << 10 | (uint32_t)(1023 - index);
+}
+__device__ __forceinline__ int index_of(uint32_t key) { return 1023 - (int)(key & 1023u); }
+
+// The two largest of a group's values, at its first lane.
+template <class T>
+__device__ __forceinline__ void two_largest(const ga_experts_route_args& a, const T* by, int lane,
+                                            int shift, T& b1, T& b2)
+{
     const int size = a.experts / a.groups;
     const int g = lane >> shift, sub = lane & ((1 << shift) - 1);
-    T b1 = none, b2 = none; // the two largest
+    b1 = b2 = (T)kMinus;
     if (g < a.groups)
         for (int i = sub; i < size; i += 1 << shift) {
             const T d = by[g * size + i];
@@ -114,20 +126,56 @@ __device__ __forceinline__ uint64_t kept_groups(const ga_experts_route_args& a, 
         b2 = max(min(b1, o1), max(b2, o2));
         b1 = max(b1, o1);
     }
+}
+
+// The groups that are kept, a bit at each one's first lane (group << shift), by their values.
+template <class T>
+__device__ __forceinline__ uint64_t kept_groups(const ga_experts_route_args& a, const T* by, int lane,
+                                                int shift)
+{
+    T b1, b2;
+    two_largest(a, by, lane, shift, b1, b2);
+    const T none = (T)kMinus;
     const T value = a.group_rank == 2 && b2 > none ? b1 + b2 : b1;
-    int before = 0, close = 0;
+    const int g = lane >> shift;
+    int before = 0;
     for (int j = 0; j < a.groups; j++) {
         const T o = __shfl(value, j << shift, 64);
         before += o > value || (o == value && j < g);
-        close += j != g && !(o - value > margin) && !(value - o > margin);
     }
-    const bool there = g < a.groups && sub == 0 && value > none;
-    const bool keep = there && before < a.top_groups;
-    // one that is close to another counts only at the border: the order of those kept is all the same
-    sure = margin == (T)0 ||
-           __builtin_amdgcn_ballot_w64(there && close && before < a.top_groups + close &&
-                                       before + close >= a.top_groups) == 0;
-    return __builtin_amdgcn_ballot_w64(keep);
+    return __builtin_amdgcn_ballot_w64(g < a.groups && (lane & ((1 << shift) - 1)) == 0 &&
+                                       value > none && before < a.top_groups);
+}
+
+// The same one after the other by packed values; sure: no group left out is within `gap` steps of
+// a kept one.
+__device__ __forceinline__ uint64_t kept_groups_packed(const ga_experts_route_args& a,
+                                                       const float* by, int lane, int shift,
+                                                       float steps, uint32_t gap, bool& sure)
+{
+    float b1, b2;
+    two_largest(a, by, lane, shift, b1, b2);
+    const float value = a.group_rank == 2 && b2 > kMinus ? b1 + b2 : b1;
+    const int g = lane >> shift;
+    const bool there =
+        g < a.groups && (lane & ((1 << shift) - 1)) == 0 && value > kMinus;
+    const float top = unordered(wave_max(there ? ordered(value) : 0u));
+    uint32_t key = there ? packed(value, top, steps, g) : 0u, last = 0;
+    uint64_t kept = 0;
+    for (int j = 0; j <= a.top_groups; j++) {
+        const uint32_t best = wave_max(key);
+        if (best == 0)
+            break;
+        if (j == a.top_groups) {
+            sure &= (last >> 10) - (best >> 10) > gap;
+            break;
+        }
+        kept |= 1ull << (index_of(best) << shift);
+        key = key == best ? 0u : key;
+        last = best;
+    }
+    sure &= top < __builtin_inff();
+    return kept;
 }
 
 // Whether expert v * 64 + lane is in a kept group: e / size by a multiplication, exact for e and
@@ -138,16 +186,13 @@ __device__ __forceinline__ bool in_kept(uint64_t kept, int shift, int size, int 
     return kept >> ((((uint32_t)e * inv) >> 20) << shift) & 1;
 }
 
-// The experts of largest keys one after the other: choice j's expert in lane j, its logit beside.
-// gap: consecutive keys (and the first that is left) further apart than this, or sure is false.
+// The experts of largest keys one after the other, choice j's expert in lane j. Keys of 64 bits, or
+// (WIDE false) the first 32 alone.
 template <int VPT, bool WIDE>
-__device__ __forceinline__ int choose(const RouteToken<VPT>& t, uint32_t (&key)[VPT],
-                                      uint32_t (&low)[VPT], int top, float gap, float& logit,
-                                      bool& sure)
+__device__ __forceinline__ int choose(int lane, uint32_t (&key)[VPT], uint32_t (&low)[VPT], int top)
 {
     int id = -1;
-    float last = __builtin_inff();
-    for (int j = 0; j < top + (gap > 0.0f); j++) {
+    for (int j = 0; j < top; j++) {
         uint32_t best = key[0], second = 0;
 #pragma unroll
         for (int v = 1; v < VPT; v++)
@@ -155,13 +200,6 @@ __device__ __forceinline__ int choose(const RouteToken<VPT>& t, uint32_t (&key)[
         best = wave_max(best);
         if (best == 0)
             break;
-        if (!WIDE && gap > 0.0f) {
-            const float k = unordered(best);
-            sure &= j == 0 ? k < __builtin_inff() : last - k > gap;
-            last = k;
-            if (j == top)
-                break;
-        }
         if constexpr (WIDE) {
 #pragma unroll
             for (int v = 0; v < VPT; v++)
@@ -175,17 +213,41 @@ __device__ __forceinline__ int choose(const RouteToken<VPT>& t, uint32_t (&key)[
                 __builtin_amdgcn_ballot_w64(key[v] == best && (!WIDE || low[v] == second));
             if (!found && has != 0) {
                 const int l = __builtin_ctzll(has);
-                const float x = __uint_as_float(
-                    __builtin_amdgcn_readlane(__float_as_uint(t.x[v]), l));
                 found = true;
-                if (t.lane == l)
+                if (lane == l)
                     key[v] = low[v] = 0u;
-                if (t.lane == j) {
+                if (lane == j)
                     id = v * 64 + l;
-                    logit = x;
-                }
             }
         }
+    }
+    return id;
+}
+
+// The same by packed keys. sure: consecutive ones, and the first that is left, are further apart
+// than `gap` steps, so that they are in the order of what they stand for.
+template <int VPT>
+__device__ __forceinline__ int choose_packed(int lane, uint32_t (&key)[VPT], int top, uint32_t gap,
+                                             bool& sure)
+{
+    int id = -1;
+    uint32_t last = ~0u;
+    for (int j = 0; j <= top; j++) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int v = 1; v < VPT; v++)
+            best = max(best, key[v]);
+        best = wave_max(best);
+        if (best == 0)
+            break;
+        sure &= j == 0 || (last >> 10) - (best >> 10) > gap;
+        if (j == top)
+            break;
+#pragma unroll
+        for (int v = 0; v < VPT; v++)
+            key[v] = key[v] == best ? 0u : key[v];
+        id = lane == j ? index_of(best) : id;
+        last = best;
     }
     return id;
 }
@@ -193,7 +255,7 @@ __device__ __forceinline__ int choose(const RouteToken<VPT>& t, uint32_t (&key)[
 // The choice by keys of 64 bits.
 template <int VPT>
 __device__ __forceinline__ int choose64(const ga_experts_route_args& a, const RouteToken<VPT>& t,
-                                        double* by, int shift, float& logit)
+                                        double* by, int shift)
 {
     const bool softmax = a.scores == GA_EXPERTS_SOFTMAX;
     const int lane = t.lane, E = a.experts, size = E / a.groups;
@@ -237,19 +299,17 @@ __device__ __forceinline__ int choose64(const ga_experts_route_args& a, const Ro
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        bool sure;
-        const uint64_t kept = kept_groups(a, by, lane, shift, 0.0, sure);
+        const uint64_t kept = kept_groups(a, by, lane, shift);
 #pragma unroll
         for (int v = 0; v < VPT; v++)
             if (!in_kept(kept, shift, size, v * 64 + lane))
                 key[v] = low[v] = 0u;
     }
-    bool sure;
-    return choose<VPT, true>(t, key, low, a.top, 0.0f, logit, sure);
+    return a.bias ? choose<VPT, true>(lane, key, low, a.top)
+                  : choose<VPT, false>(lane, key, low, a.top);
 }
 
-// SCORES: scores decide (a bias, or sums of two in groups), else the logits alone.
-template <int VPT, int IN, bool SCORES>
+template <int VPT, int IN>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_route_args a)
 {
     extern __shared__ double by_all[]; // [wave][expert], with groups
@@ -260,25 +320,33 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         return;
     const int E = a.experts, size = E / a.groups;
     const bool softmax = a.scores == GA_EXPERTS_SOFTMAX, grouped = a.top_groups < a.groups;
+    // scores decide, not the logits alone
+    const bool by_group = grouped && a.group_rank == 2, by_score = a.bias || by_group;
     const int shift = 31 - __builtin_clz(64 / a.groups); // log2 of the lanes of a group
 
+    const long long row = token * a.stride_logits;
+    auto logit = [&](int e) {
+        const float x = IN == GA_IN_F32 ? ((const float*)a.logits)[row + e]
+                                        : bf16_to_f32(((const uint16_t*)a.logits)[row + e]);
+        return x > kMinus ? fminf(x, 3.40282347e38f) : kMinus;
+    };
     RouteToken<VPT> t;
     t.lane = lane;
-    uint32_t top = 0;
+    float top = kMinus;
 #pragma unroll
     for (int v = 0; v < VPT; v++) {
         const int e = v * 64 + lane;
-        const long long i = token * a.stride_logits + min(e, E - 1);
-        const float x = IN == GA_IN_F32 ? ((const float*)a.logits)[i]
-                                        : bf16_to_f32(((const uint16_t*)a.logits)[i]);
-        t.x[v] = e < E && x > kMinus ? fminf(x, 3.40282347e38f) : kMinus;
-        top = max(top, ordered(t.x[v]));
+        t.x[v] = e < E ? logit(min(e, E - 1)) : kMinus;
+        top = fmaxf(top, t.x[v]);
     }
-    t.largest = unordered(wave_max(top));
+    t.largest = wave_max(top);
 
-    uint32_t key[VPT], low[VPT];
-    float by[VPT], sum = 0.0f, margin = 0.0f;
-    if (SCORES || (softmax && !a.renormalise)) {
+    // in 32 bits: the keys, and what the groups go by
+    float key[VPT], by[VPT], sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; v++)
+        key[v] = by[v] = t.x[v];
+    if (by_score || (softmax && !a.renormalise)) {
 #pragma unroll
         for (int v = 0; v < VPT; v++) {
             by[v] = t.x[v] > kMinus ? score_of(t.x[v], softmax, t.largest) : 0.0f;
@@ -286,35 +354,35 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         }
         sum = wave_sum(sum);
     }
-    if constexpr (SCORES) {
+    // A step of a packed key, and how many of them two keys that are off can be apart: logits are
+    // exact, a step of 2^-18 reaches 16 down; scores lie within 1, a step of 2^-21 reaches 2
+    float steps = 0x1p18f, off = 0.0f;
+    if (by_score) {
         const float scale = softmax ? 1.0f / sum : 1.0f;
-        float most = 0.0f; // the largest |key|
+        float most = 0.0f; // the largest |score + bias|
 #pragma unroll
         for (int v = 0; v < VPT; v++) {
-            const int e = v * 64 + lane;
-            by[v] *= scale;
-            bool there = t.x[v] > kMinus;
+            float s = by[v] * scale;
             if (a.bias) {
-                by[v] += a.bias[min(e, E - 1)];
-                there = there && by[v] > kMinus;
+                s += a.bias[min(v * 64 + lane, E - 1)];
+                key[v] = t.x[v] > kMinus && s > kMinus ? s : kMinus;
+                s = key[v];
+                most = s > kMinus ? fmaxf(most, fabsf(s)) : most;
             }
-            key[v] = there ? ordered(a.bias ? by[v] : t.x[v]) : 0u;
-            by[v] = there ? by[v] : kMinus;
-            most = there ? fmaxf(most, fabsf(by[v])) : most;
+            by[v] = t.x[v] > kMinus ? s : kMinus;
         }
-        margin = 2.0f * (kScoreError + 0x1p-23f * unordered(wave_max(ordered(most))));
+        most = a.bias ? wave_max(most) : 1.0f;
+        off = 2.0f * (kScoreError + 0x1p-23f * most);
+        if (a.bias)
+            steps = 0x1p21f;
     } else {
 #pragma unroll
-        for (int v = 0; v < VPT; v++) {
-            key[v] = t.x[v] > kMinus ? ordered(t.x[v]) : 0u;
+        for (int v = 0; v < VPT; v++)
             by[v] = t.x[v];
-        }
     }
-#pragma unroll
-    for (int v = 0; v < VPT; v++)
-        low[v] = 0u;
 
     bool sure = true;
+    uint64_t kept = ~0ull;
     double* lds = by_all + wave * E;
     if (grouped) {
         float* f = (float*)lds;
@@ -325,26 +393,45 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const uint64_t kept = kept_groups(a, f, lane, shift, 2.0f * margin, sure);
+        // sums of two scores lie within 2: a step of 2^-20 reaches 4; sums are off by twice as much
+        const float gsteps = by_score ? 0x1p20f : steps;
+        kept = kept_groups_packed(a, f, lane, shift, gsteps, 2 + (uint32_t)(2.0f * off * gsteps),
+                                  sure);
         __builtin_amdgcn_wave_barrier(); // read before 64 bits are written there
 #pragma unroll
         for (int v = 0; v < VPT; v++)
             if (!in_kept(kept, shift, size, v * 64 + lane))
-                key[v] = 0u;
+                key[v] = kMinus;
     }
-    float xi = kMinus;
     int id = -1;
-    if (sure)
-        id = choose<VPT, false>(t, key, low, a.top, a.bias ? margin : 0.0f, xi, sure);
-    if (SCORES && !sure) {
-        xi = kMinus;
-        id = choose64(a, t, lds, shift, xi);
+    if (sure) {
+        float best = kMinus;
+#pragma unroll
+        for (int v = 0; v < VPT; v++)
+            best = fmaxf(best, key[v]);
+        best = wave_max(best);
+        uint32_t pack[VPT];
+        const bool bf16 = IN == GA_IN_BF16 && !a.bias; // 16 bits and the index hold all of it
+#pragma unroll
+        for (int v = 0; v < VPT; v++) {
+            const int e = v * 64 + lane;
+            pack[v] = !(key[v] > kMinus) ? 0u
+                      : bf16             ? (ordered(key[v]) >> 16) << 10 | (uint32_t)(1023 - e)
+                                         : packed(key[v], best, steps, e);
+        }
+        sure = best < __builtin_inff();
+        bool apart = true;
+        id = choose_packed<VPT>(lane, pack, a.top, 2 + (uint32_t)(off * steps), apart);
+        sure &= bf16 || apart;
     }
+    if (!sure)
+        id = choose64(a, t, lds, shift);
 
     // weights: each relative to the largest of the chosen logits, which so cancels
+    const float xi = id >= 0 ? logit(id) : kMinus;
     float w = 0.0f;
     if (a.renormalise) {
-        const float from = unordered(wave_max(ordered(xi)));
+        const float from = wave_max(xi);
         if (id >= 0)
             w = softmax ? expf(xi - from)
                         : expf(fminf(xi, 0.0f) - fminf(from, 0.0f)) / (1.0f + expf(-fabsf(xi)));
@@ -359,13 +446,13 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
     }
 }
 
-template <int IN, bool SCORES>
+template <int IN>
 void launch_route(const ga_experts_route_args& a, hipStream_t st)
 {
     const dim3 grid((unsigned)((a.tokens + (long long)kRouteWaves - 1) / kRouteWaves));
     const size_t lds = a.top_groups < a.groups ? sizeof(double) * kRouteWaves * a.experts : 0;
     auto go = [&](auto V) {
-        hipLaunchKernelGGL((route_kernel<decltype(V)::value, IN, SCORES>), grid,
+        hipLaunchKernelGGL((route_kernel<decltype(V)::value, IN>), grid,
                            dim3(64 * kRouteWaves), lds, st, a);
     };
     const int v = (a.experts + 63) / 64;
@@ -713,11 +800,7 @@ ga_status ga_experts_route(const ga_experts_route_args* args, void* stream)
     if (a.stride_logits < (a.tokens > 1 ? a.experts : 0))
         return fail(GA_ERR_SHAPE, "experts_route: stride_logits must be >= experts");
     hipStream_t st = (hipStream_t)stream;
-    const bool by_scores = a.bias || (a.top_groups < a.groups && a.group_rank == 2);
-    if (a.in_dtype == GA_IN_F32)
-        by_scores ? launch_route<GA_IN_F32, true>(a, st) : launch_route<GA_IN_F32, false>(a, st);
-    else
-        by_scores ? launch_route<GA_IN_BF16, true>(a, st) : launch_route<GA_IN_BF16, false>(a, st);
+    a.in_dtype == GA_IN_F32 ? launch_route<GA_IN_F32>(a, st) : launch_route<GA_IN_BF16>(a, st);
     GA_HIP_CHECK(hipGetLastError());
     return GA_OK;
 }
