@@ -20,7 +20,7 @@ namespace {
 // bits first, with a bound of what they are off by, and again in 64 where two keys that
 // decide it lie within that bound (of random logits one token in a hundred): instructions bound
 // this kernel, and exponentials and comparisons of 64 bits cost two to four times as many.
-// 16384 tokens, 192 experts in 8 groups, sigmoid and bias: 64 bits throughout 25.4 us, so ROUTE_US.
+// 16384 tokens, 192 experts in 8 groups, sigmoid and bias: 64 bits throughout 25.4 us, so 17.8.
 
 // Exchange between the lanes of a row of 16, then between rows: lane 63 has all.
 template <class T, class Op>
@@ -77,6 +77,14 @@ __device__ __forceinline__ float unordered(uint32_t k)
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// LDS of one wave alone: what its lanes wrote is there, what they read has been.
+__device__ __forceinline__ void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 constexpr int kRouteWaves = 4;
 constexpr float kMinus = -__builtin_inff();
 
@@ -91,6 +99,21 @@ struct RouteToken {
     float largest;
     int lane;
 };
+
+// Steps of packed keys to 1: logits, exact, reach 16 down from the largest; scores with a bias 2,
+// sums of two of them 4.
+constexpr float kLogitSteps = 0x1p18f, kScoreSteps = 0x1p21f, kSumSteps = 0x1p20f;
+
+// The weight of a chosen logit x before it is divided by the sum over the chosen ones, relative to the
+// largest of them, `from`; without renormalising its score (sum: a softmax's).
+__device__ __forceinline__ float weight_of(const ga_experts_route_args& a, float x, float from,
+                                           float largest, float sum)
+{
+    if (a.scores == GA_EXPERTS_SOFTMAX)
+        return a.renormalise ? expf(x - from) : expf(x - largest) / sum;
+    const float e = fminf(x, 0.0f) - (a.renormalise ? fminf(from, 0.0f) : 0.0f);
+    return expf(e) / (1.0f + expf(-fabsf(x)));
+}
 
 __device__ __forceinline__ float score_of(float x, bool softmax, float largest)
 {
@@ -296,9 +319,7 @@ __device__ __forceinline__ int choose64(const ga_experts_route_args& a, const Ro
         for (int v = 0; v < VPT; v++)
             if (v * 64 + lane < E)
                 by[v * 64 + lane] = score[v];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_lds_fence();
         const uint64_t kept = kept_groups(a, by, lane, shift);
 #pragma unroll
         for (int v = 0; v < VPT; v++)
@@ -354,9 +375,8 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         }
         sum = wave_sum(sum);
     }
-    // A step of a packed key, and how many of them two keys that are off can be apart: logits are
-    // exact, a step of 2^-18 reaches 16 down; scores lie within 1, a step of 2^-21 reaches 2
-    float steps = 0x1p18f, off = 0.0f;
+    // the steps of packed keys, and what two keys can be off by
+    float steps = kLogitSteps, off = 0.0f;
     if (by_score) {
         const float scale = softmax ? 1.0f / sum : 1.0f;
         float most = 0.0f; // the largest |score + bias|
@@ -374,7 +394,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         most = a.bias ? wave_max(most) : 1.0f;
         off = 2.0f * (kScoreError + 0x1p-23f * most);
         if (a.bias)
-            steps = 0x1p21f;
+            steps = kScoreSteps;
     } else {
 #pragma unroll
         for (int v = 0; v < VPT; v++)
@@ -390,14 +410,11 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         for (int v = 0; v < VPT; v++)
             if (v * 64 + lane < E)
                 f[v * 64 + lane] = by[v];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        // sums of two scores lie within 2: a step of 2^-20 reaches 4; sums are off by twice as much
-        const float gsteps = by_score ? 0x1p20f : steps;
+        wave_lds_fence();
+        const float gsteps = by_score ? kSumSteps : steps; // sums are off by twice as much
         kept = kept_groups_packed(a, f, lane, shift, gsteps, 2 + (uint32_t)(2.0f * off * gsteps),
                                   sure);
-        __builtin_amdgcn_wave_barrier(); // read before 64 bits are written there
+        wave_lds_fence(); // read before 64 bits are written there
 #pragma unroll
         for (int v = 0; v < VPT; v++)
             if (!in_kept(kept, shift, size, v * 64 + lane))
@@ -429,45 +446,277 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
 
     // weights: each relative to the largest of the chosen logits, which so cancels
     const float xi = id >= 0 ? logit(id) : kMinus;
-    float w = 0.0f;
+    const float from = wave_max(xi);
+    float w = id >= 0 ? weight_of(a, xi, from, t.largest, sum) : 0.0f;
     if (a.renormalise) {
-        const float from = wave_max(xi);
-        if (id >= 0)
-            w = softmax ? expf(xi - from)
-                        : expf(fminf(xi, 0.0f) - fminf(from, 0.0f)) / (1.0f + expf(-fabsf(xi)));
         const float all = wave_sum(w);
         w = id >= 0 ? w / all : 0.0f;
-    } else if (id >= 0) {
-        w = softmax ? expf(xi - t.largest) / sum : expf(fminf(xi, 0.0f)) / (1.0f + expf(-fabsf(xi)));
     }
     if (lane < a.top) {
         a.ids[token * a.top + lane] = id;
-        a.weights[token * a.top + lane] = id >= 0 ? w * a.scale : 0.0f;
+        a.weights[token * a.top + lane] = w * a.scale;
+    }
+}
+
+// ---- route, four tokens a wave -----------------------------------------------------------
+// Up to 256 experts, 16 groups and 16 choices: a token has a row of 16 lanes, runs of four experts
+// each (lane r the experts 64 c + 4 r + i), so that the reductions, which take as many instructions
+// for one token as for four, are shared. Tokens that 32 bits do not decide are gone over again, one
+// at a time, by the whole wave.
+template <class T, class Op>
+__device__ __forceinline__ T row_all(T a, const Op& op)
+{
+    auto dpp = [](T v, auto ctrl) {
+        return __builtin_bit_cast(
+            T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF,
+                                           0xF, false));
+    };
+    a = op(a, dpp(a, std::integral_constant<int, 0xB1>{}));  // xor 1
+    a = op(a, dpp(a, std::integral_constant<int, 0x4E>{}));  // xor 2
+    a = op(a, dpp(a, std::integral_constant<int, 0x141>{})); // half mirror
+    return op(a, dpp(a, std::integral_constant<int, 0x140>{})); // mirror
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t a)
+{
+    return row_all(a, [](uint32_t x, uint32_t y) { return max(x, y); });
+}
+__device__ __forceinline__ float row_max(float a)
+{
+    return row_all(a, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ float row_sum(float a)
+{
+    return row_all(a, [](float x, float y) { return x + y; });
+}
+
+template <int C, int IN>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts_route_args a,
+                                                                      int vector)
+{
+    constexpr int VPT = 4 * C;
+    extern __shared__ double by_all[]; // [wave][2 E], with groups
+    const int lane = threadIdx.x & 63, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long first = ((long long)blockIdx.x * kRouteWaves + wave) * 4;
+    if (first >= a.tokens)
+        return;
+    const long long token = min(first + (lane >> 4), (long long)a.tokens - 1);
+    const int E = a.experts, size = E / a.groups;
+    const bool softmax = a.scores == GA_EXPERTS_SOFTMAX, grouped = a.top_groups < a.groups;
+    const bool by_score = a.bias || (grouped && a.group_rank == 2);
+
+    auto there = [](float x) { return x > kMinus ? fminf(x, 3.40282347e38f) : kMinus; };
+    const long long row = token * a.stride_logits;
+    auto logit = [&](long long at, int e) {
+        return there(IN == GA_IN_F32 ? ((const float*)a.logits)[at + e]
+                                     : bf16_to_f32(((const uint16_t*)a.logits)[at + e]));
+    };
+    float x[VPT], largest = kMinus;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int e = c * 64 + r * 4;
+        if (vector) { // E a multiple of 4, rows aligned
+            const int f = min(e, E - 4);
+            if constexpr (IN == GA_IN_F32) {
+                const v4f d = *(const v4f*)((const float*)a.logits + row + f);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    x[4 * c + i] = e < E ? there(d[i]) : kMinus;
+            } else {
+                const uint2 d = *(const uint2*)((const uint16_t*)a.logits + row + f);
+                const uint32_t u[4] = {d.x << 16, d.x & 0xFFFF0000u, d.y << 16, d.y & 0xFFFF0000u};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    x[4 * c + i] = e < E ? there(__uint_as_float(u[i])) : kMinus;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                x[4 * c + i] = e + i < E ? logit(row, min(e + i, E - 1)) : kMinus;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; v++)
+        largest = fmaxf(largest, x[v]);
+    largest = row_max(largest);
+
+    float key[VPT], by[VPT], sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; v++)
+        key[v] = by[v] = x[v];
+    if (by_score || (softmax && !a.renormalise)) {
+#pragma unroll
+        for (int v = 0; v < VPT; v++) {
+            by[v] = x[v] > kMinus ? score_of(x[v], softmax, largest) : 0.0f;
+            sum += by[v];
+        }
+        sum = row_sum(sum);
+    }
+    float steps = kLogitSteps, off = 0.0f;
+    if (by_score) {
+        const float scale = softmax ? 1.0f / sum : 1.0f;
+        float most = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VPT; v++) {
+            float s = by[v] * scale;
+            if (a.bias) {
+                s += a.bias[min(v / 4 * 64 + r * 4 + v % 4, E - 1)];
+                key[v] = x[v] > kMinus && s > kMinus ? s : kMinus;
+                s = key[v];
+                most = s > kMinus ? fmaxf(most, fabsf(s)) : most;
+            }
+            by[v] = x[v] > kMinus ? s : kMinus;
+        }
+        most = a.bias ? row_max(most) : 1.0f;
+        off = 2.0f * (kScoreError + 0x1p-23f * most);
+        if (a.bias)
+            steps = kScoreSteps;
+    } else {
+#pragma unroll
+        for (int v = 0; v < VPT; v++)
+            by[v] = x[v];
+    }
+
+    bool sure = true;
+    double* lds = by_all + (size_t)wave * 2 * E;
+    if (grouped) {
+        float* f = (float*)lds + (lane >> 4) * E;
+#pragma unroll
+        for (int v = 0; v < VPT; v++) {
+            const int e = v / 4 * 64 + r * 4 + v % 4;
+            if (e < E)
+                f[e] = by[v];
+        }
+        wave_lds_fence();
+        const int shift = 31 - __builtin_clz(16 / a.groups); // log2 of the lanes of a group
+        float b1, b2;
+        two_largest(a, f, r, shift, b1, b2);
+        const float value = a.group_rank == 2 && b2 > kMinus ? b1 + b2 : b1;
+        const int g = r >> shift;
+        const bool leads = g < a.groups && (r & ((1 << shift) - 1)) == 0 && value > kMinus;
+        const float top = row_max(leads ? value : kMinus);
+        const float gsteps = by_score ? kSumSteps : steps;
+        const uint32_t gap = 2 + (uint32_t)(2.0f * off * gsteps);
+        uint32_t gkey = leads ? packed(value, top, gsteps, g) : 0u, last = 0, kept = 0;
+        for (int j = 0; j <= a.top_groups; j++) {
+            const uint32_t best = row_max(gkey);
+            if (j == a.top_groups)
+                sure &= best == 0 || (last >> 10) - (best >> 10) > gap;
+            else if (best != 0)
+                kept |= 1u << index_of(best);
+            gkey = gkey == best ? 0u : gkey;
+            last = best;
+        }
+        sure &= top < __builtin_inff();
+        // e / size by a multiplication, exact for e and size up to 1024; a run's at once where it can be
+        const uint32_t inv = ((1u << 20) + size - 1) / size;
+#pragma unroll
+        for (int v = 0; v < VPT; v++) {
+            const uint32_t e = v / 4 * 64 + r * 4 + v % 4;
+            if (!(kept >> ((e * inv) >> 20) & 1))
+                key[v] = kMinus;
+        }
+    }
+
+    float best_key = kMinus;
+#pragma unroll
+    for (int v = 0; v < VPT; v++)
+        best_key = fmaxf(best_key, key[v]);
+    best_key = row_max(best_key);
+    const bool bf16 = IN == GA_IN_BF16 && !a.bias; // 16 bits and the index hold all of it
+    uint32_t pack[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; v++) {
+        const int e = v / 4 * 64 + r * 4 + v % 4;
+        pack[v] = !(key[v] > kMinus) ? 0u
+                  : bf16             ? (ordered(key[v]) >> 16) << 10 | (uint32_t)(1023 - e)
+                                     : packed(key[v], best_key, steps, e);
+    }
+    const uint32_t gap = 2 + (uint32_t)(off * steps);
+    bool apart = true;
+    uint32_t last = 0;
+    int id = -1;
+    for (int j = 0; j <= a.top; j++) {
+        uint32_t best = pack[0];
+#pragma unroll
+        for (int v = 1; v < VPT; v++)
+            best = max(best, pack[v]);
+        best = row_max(best);
+        apart &= j == 0 || best == 0 || (last >> 10) - (best >> 10) > gap;
+        if (j == a.top)
+            break;
+#pragma unroll
+        for (int v = 0; v < VPT; v++)
+            pack[v] = pack[v] == best ? 0u : pack[v];
+        id = r == j && best != 0 ? index_of(best) : id;
+        last = best;
+    }
+    sure &= (bf16 || apart) && best_key < __builtin_inff();
+
+    for (uint64_t again = __builtin_amdgcn_ballot_w64(!sure); again;) {
+        const int lead = __builtin_ctzll(again) & ~15; // of the token's lanes
+        again &= ~(0xFFFFull << lead);
+        RouteToken<C> t;
+        t.lane = lane;
+        t.largest = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(largest), lead));
+        const long long at = min(first + lead / 16, (long long)a.tokens - 1) * a.stride_logits;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int e = c * 64 + lane;
+            t.x[c] = e < E ? logit(at, min(e, E - 1)) : kMinus;
+        }
+        if (grouped)
+            wave_lds_fence(); // what was there has been read
+        const int id64 = choose64(a, t, lds, 31 - __builtin_clz(64 / a.groups));
+        const int mine = __shfl(id64, r, 64);
+        if ((lane & ~15) == lead)
+            id = mine;
+    }
+
+    // weights: each relative to the largest of the chosen logits, which so cancels
+    const float xi = id >= 0 ? logit(row, id) : kMinus;
+    const float from = row_max(xi);
+    float w = id >= 0 ? weight_of(a, xi, from, largest, sum) : 0.0f;
+    if (a.renormalise) {
+        const float all = row_sum(w);
+        w = id >= 0 ? w / all : 0.0f;
+    }
+    if (r < a.top && first + (lane >> 4) < a.tokens) {
+        a.ids[token * a.top + r] = id;
+        a.weights[token * a.top + r] = w * a.scale;
     }
 }
 
 template <int IN>
 void launch_route(const ga_experts_route_args& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)((a.tokens + (long long)kRouteWaves - 1) / kRouteWaves));
-    const size_t lds = a.top_groups < a.groups ? sizeof(double) * kRouteWaves * a.experts : 0;
-    auto go = [&](auto V) {
-        hipLaunchKernelGGL((route_kernel<decltype(V)::value, IN>), grid,
-                           dim3(64 * kRouteWaves), lds, st, a);
-    };
     const int v = (a.experts + 63) / 64;
-    if (v <= 1)
-        go(std::integral_constant<int, 1>{});
-    else if (v <= 2)
-        go(std::integral_constant<int, 2>{});
-    else if (v <= 3)
-        go(std::integral_constant<int, 3>{});
-    else if (v <= 4)
-        go(std::integral_constant<int, 4>{});
-    else if (v <= 8)
-        go(std::integral_constant<int, 8>{});
-    else
-        go(std::integral_constant<int, 16>{});
+    const bool grouped = a.top_groups < a.groups;
+    if (v <= 4 && a.groups <= 16 && a.top <= 16) {
+        const int el = IN == GA_IN_F32 ? 4 : 2;
+        const int vector = a.experts % 4 == 0 && (uintptr_t)a.logits % (4 * el) == 0 &&
+                           (a.tokens == 1 || a.stride_logits % 4 == 0);
+        const dim3 grid((unsigned)((a.tokens + 4ll * kRouteWaves - 1) / (4 * kRouteWaves)));
+        const size_t lds = grouped ? 2 * sizeof(double) * kRouteWaves * a.experts : 0;
+        auto go = [&](auto C) {
+            hipLaunchKernelGGL((route_rows_kernel<decltype(C)::value, IN>), grid,
+                               dim3(64 * kRouteWaves), lds, st, a, vector);
+        };
+        v == 1   ? go(std::integral_constant<int, 1>{})
+        : v == 2 ? go(std::integral_constant<int, 2>{})
+        : v == 3 ? go(std::integral_constant<int, 3>{})
+                 : go(std::integral_constant<int, 4>{});
+        return;
+    }
+    const dim3 grid((unsigned)((a.tokens + (long long)kRouteWaves - 1) / kRouteWaves));
+    const size_t lds = grouped ? sizeof(double) * kRouteWaves * a.experts : 0;
+    auto go = [&](auto V) {
+        hipLaunchKernelGGL((route_kernel<decltype(V)::value, IN>), grid, dim3(64 * kRouteWaves), lds,
+                           st, a);
+    };
+    v <= 4   ? go(std::integral_constant<int, 4>{})
+    : v <= 8 ? go(std::integral_constant<int, 8>{})
+             : go(std::integral_constant<int, 16>{});
 }
 
 // ---- arrange ----------------------------------------------------------------------
