@@ -28,11 +28,18 @@ from .mx4_cache import _IN_TYPES, _OUT_TYPES, _current_device, _on, _stream
 _SCORES = {"softmax": _lib.GA_EXPERTS_SOFTMAX, "sigmoid": _lib.GA_EXPERTS_SIGMOID}
 
 
-def _gpu(x, what):
-    device = x.get_device()
+# The checks below run on every call, of which a decode step makes several for each layer: they
+# ask a tensor for as little as they can.
+def _matrix(x, what):
+    """Rows, columns, row stride and GPU of a matrix whose rows are contiguous."""
+    shape, strides, device = x.shape, x.stride(), x.get_device()
+    if len(shape) != 2:
+        raise ValueError("%s must be a matrix, is %s" % (what, tuple(shape)))
+    if strides[1] != 1 and shape[1] > 1 and x.numel():
+        raise ValueError("%s must be contiguous along its rows (strides %s)" % (what, strides))
     if device < 0 or device != _current_device():
         raise ValueError("%s is on %s, not on the current GPU" % (what, x.device))
-    return device
+    return shape[0], shape[1], strides[0], device
 
 
 def _check(x, what, dtype, shape, device):
@@ -57,12 +64,6 @@ def _dense(x, what, dtype, shape, device):
         raise ValueError("%s must be contiguous (strides %s)" % (what, x.stride()))
 
 
-def _matrix(x, what):
-    if x.dim() != 2:
-        raise ValueError("%s must be a matrix, is %s" % (what, tuple(x.shape)))
-    return x.shape
-
-
 def route(logits, top, bias=None, scores="softmax", groups=1, top_groups=None, group_rank=1,
           renormalise=True, scale=1.0, ids=None, weights=None, stream=None):
     """The experts of each token: logits [tokens, experts] (float32 or bfloat16) ->
@@ -79,14 +80,12 @@ def route(logits, top, bias=None, scores="softmax", groups=1, top_groups=None, g
     A logit or bias of -inf or NaN takes an expert out; where fewer than `top` are left, ids
     are -1 and weights 0. At most 1024 experts, 64 choices, 64 groups. ids and weights
     (contiguous) can be given to write to."""
-    tokens, experts = _matrix(logits, "logits")
-    kind = _IN_TYPES.get(logits.dtype)
+    kind, by = _IN_TYPES.get(logits.dtype), _SCORES.get(scores)
     if kind is None:
         raise TypeError("logits must be float32 or bfloat16")
-    device = _gpu(logits, "logits")
-    stride = _check(logits, "logits", logits.dtype, logits.shape, device)[0]
-    if scores not in _SCORES:
+    if by is None:
         raise ValueError('scores must be "softmax" or "sigmoid"')
+    tokens, experts, stride, device = _matrix(logits, "logits")
     ptr = None
     if bias is not None:
         _check(bias, "bias", torch.float32, (experts,), device)
@@ -105,7 +104,7 @@ def route(logits, top, bias=None, scores="softmax", groups=1, top_groups=None, g
                 weights = logits.new_empty((tokens, top), dtype=torch.float32)
     check(lib().ga_experts_route(_lib.ExpertsRouteArgs(
         logits.data_ptr(), ptr, ids.data_ptr(), weights.data_ptr(), stride, kind, tokens, experts,
-        top, _SCORES[scores], groups, groups if top_groups is None else top_groups, group_rank,
+        top, by, groups, groups if top_groups is None else top_groups, group_rank,
         1 if renormalise else 0, scale), _stream(stream, device)))
     return ids, weights
 
@@ -118,15 +117,17 @@ def arrange(ids, experts, first=0, stream=None):
     them) are left out. Expert e has the sorted rows starts[e] .. starts[e + 1] - 1, in the
     order of their tokens and choices; tokens gives the token of each sorted row (-1 from
     starts[experts] on), place the row of each choice (-1 where it is left out)."""
-    count, top = _matrix(ids, "ids")
-    device = _gpu(ids, "ids")
-    _dense(ids, "ids", torch.int32, ids.shape, device)
+    count, top, _, device = _matrix(ids, "ids")
+    if ids.dtype is not torch.int32:
+        raise TypeError("ids must be torch.int32, is %s" % ids.dtype)
+    if not ids.is_contiguous():
+        raise ValueError("ids must be contiguous (strides %s)" % (ids.stride(),))
     if not 0 < experts <= _lib.GA_EXPERTS_MAX:
         raise ValueError("experts must be 1 .. %d" % _lib.GA_EXPERTS_MAX)
     with _on(stream):
-        starts = ids.new_empty((experts + 1,))
-        tokens = ids.new_empty((count * top,))
-        place = ids.new_empty((count, top))
+        starts = ids.new_empty(experts + 1)
+        tokens = ids.new_empty(count * top)
+        place = torch.empty_like(ids)
     check(lib().ga_experts_arrange(ids.data_ptr(), count, top, experts, first, starts.data_ptr(),
                                    tokens.data_ptr(), place.data_ptr(), _stream(stream, device)))
     return starts, tokens, place
@@ -143,9 +144,9 @@ def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None, cut=0):
     counts as zeros. Sums are fp32, in the order of K (for few rows of an expert in up to 4
     pieces). cut: 0, or 1 .. GA_EXPERTS_CUTS for one of the ways of cutting the product in place
     of the one that its sizes choose (include/gcnasm_amd.h), for callers that tune."""
-    count, k = _matrix(a, "a")
-    device = _gpu(a, "a")
-    sa = _check(a, "a", torch.uint8, a.shape, device)[0]
+    count, k, sa, device = _matrix(a, "a")
+    if a.dtype is not torch.uint8:
+        raise TypeError("a must be torch.uint8, is %s" % a.dtype)
     if b.dim() != 3 or k == 0:
         raise ValueError("a must be [rows, K], b [experts, N, K]")
     experts, n = b.shape[0], b.shape[1]
@@ -180,12 +181,10 @@ def activate(x, starts=None, stream=None):
     ops.quant_fp8_1x128 -> (q uint8 [rows, I], scales float32 [I / 128, rows]). With starts (as
     arrange() gives them) rows from starts[-1] on are left out: theirs of q and scales
     are not written."""
-    rows, both = _matrix(x, "x")
     kind = _IN_TYPES.get(x.dtype)
     if kind is None:
         raise TypeError("x must be float32 or bfloat16")
-    device = _gpu(x, "x")
-    stride = _check(x, "x", x.dtype, x.shape, device)[0]
+    rows, both, stride, device = _matrix(x, "x")
     inner = both // 2
     if both % 256 or not both:
         raise ValueError("x must be [rows, 2 I], I a multiple of 128, is %s" % (tuple(x.shape),))
@@ -208,12 +207,14 @@ def combine(y, place, weights, dtype=torch.bfloat16, out=None, stream=None):
     weights float32 [tokens, top] -> out [tokens, N] (bfloat16 or float32), out[t] the sum over j of
     weights[t, j] * y[place[t, j]] in fp32, in the order of j. A place outside y, such as -1,
     is left out."""
-    rows, n = _matrix(y, "y")
-    tokens, top = _matrix(place, "place")
-    device = _gpu(y, "y")
-    sy = _check(y, "y", torch.bfloat16, y.shape, device)[0]
-    _dense(place, "place", torch.int32, place.shape, device)
-    _dense(weights, "weights", torch.float32, place.shape, device)
+    rows, n, sy, device = _matrix(y, "y")
+    if y.dtype is not torch.bfloat16:
+        raise TypeError("y must be torch.bfloat16, is %s" % y.dtype)
+    if place.dim() != 2:
+        raise ValueError("place must be [tokens, top], is %s" % (tuple(place.shape),))
+    tokens, top = shape = place.shape
+    _dense(place, "place", torch.int32, shape, device)
+    _dense(weights, "weights", torch.float32, shape, device)
     if out is not None:
         dtype = out.dtype
     kind = _OUT_TYPES.get(dtype)
