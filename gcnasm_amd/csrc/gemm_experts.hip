@@ -316,8 +316,10 @@ __device__ __forceinline__ void expert_store(const ga_experts_product_args& a, c
         const int row = wave * (ROWS / 8) + it * (64 / kLanes) + lane / kLanes;
         const int col = lane % kLanes * 8;
         if (row < M && col < N)
-            *(v4i*)(out + (size_t)row * ld + col) =
-                *(const v4i*)(smem + row * pp::kStagePitch + col * 2);
+            // non-temporal: 6000 rows of 60 experts of 2048x1408 65.3 -> 61.7 us, 65536 of 64 of
+            // 4096x4096 1 % less; a layer, whose activation reads them next, no slower
+            __builtin_nontemporal_store(*(const v4i*)(smem + row * pp::kStagePitch + col * 2),
+                                        (v4i*)(out + (size_t)row * ld + col));
     }
 }
 
