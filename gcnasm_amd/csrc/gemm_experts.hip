@@ -509,8 +509,9 @@ extern "C" ga_status ga_experts_product(const ga_experts_product_args* args, voi
     if (a.experts <= 0 || a.rows < 0 || a.n <= 0 || a.k <= 0 || a.a_rows < 0 || a.cut < 0 ||
         a.cut > GA_EXPERTS_CUTS)
         return fail(GA_ERR_ARG, "experts_product: bad count");
-    if (a.experts > GA_EXPERTS_MAX)
-        return fail(GA_ERR_SHAPE, "experts_product: more than %d experts", GA_EXPERTS_MAX);
+    if (a.experts > GA_EXPERTS_MAX || a.rows > 0x7FFF0000)
+        return fail(GA_ERR_SHAPE, "experts_product: more than %d experts or 0x7FFF0000 rows",
+                    GA_EXPERTS_MAX);
     if (a.k % 128)
         return fail(GA_ERR_GROUP, "K must be a multiple of GROUP_K (128), got %d", a.k);
     if (a.rows == 0)

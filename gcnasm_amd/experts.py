@@ -28,6 +28,16 @@ from .mx4_cache import _IN_TYPES, _OUT_TYPES, _current_device, _on, _stream
 _SCORES = {"softmax": _lib.GA_EXPERTS_SOFTMAX, "sigmoid": _lib.GA_EXPERTS_SIGMOID}
 
 
+_INT_MAX = 0x7FFFFFFF
+
+
+# ctypes takes the low 32 bits of what passes an int: counts are checked here.
+def _count(n, what, least, most):
+    if not least <= n <= most:
+        raise ValueError("%s must be %d .. %d, is %d" % (what, least, most, n))
+    return n
+
+
 # The checks below run on every call, of which a decode step makes several for each layer: they
 # ask a tensor for as little as they can.
 def _matrix(x, what):
@@ -35,6 +45,8 @@ def _matrix(x, what):
     shape, strides, device = x.shape, x.stride(), x.get_device()
     if len(shape) != 2:
         raise ValueError("%s must be a matrix, is %s" % (what, tuple(shape)))
+    if shape[0] > _INT_MAX or shape[1] > _INT_MAX:
+        raise ValueError("%s is more than a call takes: %s" % (what, tuple(shape)))
     if strides[1] != 1 and shape[1] > 1 and x.numel():
         raise ValueError("%s must be contiguous along its rows (strides %s)" % (what, strides))
     if device < 0 or device != _current_device():
@@ -86,6 +98,15 @@ def route(logits, top, bias=None, scores="softmax", groups=1, top_groups=None, g
     if by is None:
         raise ValueError('scores must be "softmax" or "sigmoid"')
     tokens, experts, stride, device = _matrix(logits, "logits")
+    _count(top, "top", 1, _lib.GA_EXPERTS_MAX_TOP)
+    if groups != 1:
+        _count(groups, "groups", 1, _lib.GA_EXPERTS_MAX_GROUPS)
+    if top_groups is None:
+        top_groups = groups
+    elif top_groups != groups:
+        _count(top_groups, "top_groups", 1, groups)
+    if group_rank != 1:
+        _count(group_rank, "group_rank", 1, 2)
     ptr = None
     if bias is not None:
         _check(bias, "bias", torch.float32, (experts,), device)
@@ -95,8 +116,6 @@ def route(logits, top, bias=None, scores="softmax", groups=1, top_groups=None, g
     if weights is not None:
         _dense(weights, "weights", torch.float32, (tokens, top), device)
     if ids is None or weights is None:
-        if not 0 < top <= _lib.GA_EXPERTS_MAX_TOP:
-            raise ValueError("top must be 1 .. %d" % _lib.GA_EXPERTS_MAX_TOP)
         with _on(stream):
             if ids is None:
                 ids = logits.new_empty((tokens, top), dtype=torch.int32)
@@ -104,7 +123,7 @@ def route(logits, top, bias=None, scores="softmax", groups=1, top_groups=None, g
                 weights = logits.new_empty((tokens, top), dtype=torch.float32)
     check(lib().ga_experts_route(_lib.ExpertsRouteArgs(
         logits.data_ptr(), ptr, ids.data_ptr(), weights.data_ptr(), stride, kind, tokens, experts,
-        top, by, groups, groups if top_groups is None else top_groups, group_rank,
+        top, by, groups, top_groups, group_rank,
         1 if renormalise else 0, scale), _stream(stream, device)))
     return ids, weights
 
@@ -122,8 +141,11 @@ def arrange(ids, experts, first=0, stream=None):
         raise TypeError("ids must be torch.int32, is %s" % ids.dtype)
     if not ids.is_contiguous():
         raise ValueError("ids must be contiguous (strides %s)" % (ids.stride(),))
-    if not 0 < experts <= _lib.GA_EXPERTS_MAX:
-        raise ValueError("experts must be 1 .. %d" % _lib.GA_EXPERTS_MAX)
+    _count(experts, "experts", 1, _lib.GA_EXPERTS_MAX)
+    if first:
+        _count(first, "first", 0, _INT_MAX - experts)
+    if count * top > _INT_MAX:
+        raise ValueError("%d x %d choices are more than a call takes" % (count, top))
     with _on(stream):
         starts = ids.new_empty(experts + 1)
         tokens = ids.new_empty(count * top)
@@ -156,7 +178,9 @@ def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None, cut=0):
     _check(starts, "starts", torch.int32, (experts + 1,), device)
     total, ptr = count, None
     if rows is not None:
-        total = rows.shape[0]
+        if rows.dim() != 1:
+            raise ValueError("rows must be [R], is %s" % (tuple(rows.shape),))
+        total = _count(rows.shape[0], "the number of rows", 0, _INT_MAX)
         _check(rows, "rows", torch.int32, (total,), device)
         ptr = rows.data_ptr()
     if out is None:
@@ -165,6 +189,8 @@ def product(a, sfa, b, sfb, starts, rows=None, out=None, stream=None, cut=0):
         so = n
     else:
         so = _check(out, "out", torch.bfloat16, (total, n), device)[0]
+    if cut:
+        _count(cut, "cut", 0, _lib.GA_EXPERTS_CUTS)
     # the stride of a dimension of one element can be anything
     check(lib().ga_experts_product(_lib.ExpertsProductArgs(
         a.data_ptr(), sfa.data_ptr(), b.data_ptr(), sfb.data_ptr(), starts.data_ptr(), ptr,
@@ -213,6 +239,8 @@ def combine(y, place, weights, dtype=torch.bfloat16, out=None, stream=None):
     if place.dim() != 2:
         raise ValueError("place must be [tokens, top], is %s" % (tuple(place.shape),))
     tokens, top = shape = place.shape
+    if tokens > _INT_MAX:
+        raise ValueError("%d tokens are more than a call takes" % tokens)
     _dense(place, "place", torch.int32, shape, device)
     _dense(weights, "weights", torch.float32, shape, device)
     if out is not None:

@@ -784,15 +784,14 @@ ga_status ga_experts_arrange(const int* ids, int tokens, int top, int experts, i
  *   out    [rows, n] bf16, rows stride_out elements apart
  * k % 128 == 0; strides of a and b multiples of 16, both 16-byte aligned. A row of rows_of
  * outside a counts as zeros; without rows_of a_rows must be at least rows. starts outside
- * 0 .. rows are taken as the nearest of those, and an expert that ends before it starts has no
- * rows; where starts decrease it is not said which of the rows' experts has written them.
+ * 0 .. rows are taken as the nearest of those, and where they decrease as the largest before.
  * cut: 0, or one of 1 .. GA_EXPERTS_CUTS to run that way of cutting the product (rows x columns
  * of a workgroup: 1 16x64, 2 16x32, 3 16x256, 4 64x256, 5 64x64, 6 128x128, 7 128x256, 8 256x256) in
  * place of the one that the sizes choose. K is summed in 128-groups in order, by the cuts 1, 2 and
  * 5 in 2, 4 and 4 pieces (fewer where K has fewer groups) that are added in order; otherwise the
  * cuts give the same results.
  * Limits: 256 rows of a or b, and with rows_of all of a, span at most 0xE0000000 bytes; sfa at most
- * 4 GiB, with rows_of 0x0FFF0000 bytes. */
+ * 4 GiB, with rows_of 0x0FFF0000 bytes; rows at most 0x7FFF0000. */
 typedef struct ga_experts_product_args {
     const void* a;
     const float* sfa;

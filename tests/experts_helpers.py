@@ -76,9 +76,10 @@ def arrange(ids, experts, first=0):
 
 
 def ranges(starts, rows):
-    """[first, last) of each expert, as the kernels take first rows: the nearest of 0 .. rows."""
-    s = [min(max(int(x), 0), rows) for x in starts]
-    return [(lo, max(lo, hi)) for lo, hi in zip(s, s[1:])]
+    """[first, last) of each expert, as the kernels take first rows: the nearest of 0 .. rows, and the
+    largest before where they decrease."""
+    s = np.maximum.accumulate([min(max(int(x), 0), rows) for x in starts]).tolist()
+    return list(zip(s, s[1:]))
 
 
 def product(a, sfa, b, sfb, starts, rows=None, total=None):

@@ -57,7 +57,7 @@ def product(**kw):
 @pytest.mark.parametrize("change,status", [
     (dict(a=None), ARG), (dict(sfa=None), ARG), (dict(b=None), ARG), (dict(sfb=None), ARG),
     (dict(starts=None), ARG), (dict(out=None), ARG), (dict(experts=0), ARG), (dict(rows=-1), ARG),
-    (dict(n=0), ARG), (dict(k=0), ARG), (dict(cut=-1), ARG), (dict(cut=9), ARG), (dict(a_rows=-1), ARG), (dict(experts=1025), SHAPE),
+    (dict(n=0), ARG), (dict(k=0), ARG), (dict(cut=-1), ARG), (dict(cut=9), ARG), (dict(a_rows=-1), ARG), (dict(experts=1025), SHAPE), (dict(rows=0x7FFF0001), SHAPE),
     (dict(k=192), _lib.GA_ERR_GROUP), (dict(a_rows=0), SHAPE), (dict(rows_of=None), SHAPE),
     (dict(a=0x1008), SHAPE), (dict(b=0x3004), SHAPE), (dict(stride_a=264), SHAPE),
     (dict(stride_b=264), SHAPE), (dict(stride_b_expert=300 * 256 + 8), SHAPE),
@@ -128,4 +128,4 @@ def test_the_definition_by_hand():
     assert H.route([[-np.inf, np.nan]], 2)[0].tolist() == [[-1, -1]]
     s, t, p = H.arrange([[1, 0], [1, 7]], 2)
     assert s.tolist() == [0, 1, 3] and t.tolist() == [0, 0, 1, -1] and p.tolist() == [[1, 0], [2, -1]]
-    assert H.ranges([-3, 5, 2, 99], 20) == [(0, 5), (5, 5), (2, 20)]
+    assert H.ranges([-3, 5, 2, 99], 20) == [(0, 5), (5, 5), (5, 20)]

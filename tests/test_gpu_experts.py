@@ -195,33 +195,26 @@ def test_product_of_many_experts(dev, experts):
 
 
 @pytest.mark.parametrize("starts", [[-5, 3, 3, 9, 40], [0, 0, 0, 0, 0], [7, 7, 12, 12, 2 ** 31 - 1],
-                                    [-2 ** 31, -1, 4, 4, 20], [20, 20, 21, 22, 23]])
+                                    [-2 ** 31, -1, 4, 4, 20], [20, 20, 21, 22, 23],
+                                    [-5, 3, 2, 9, 40], [7, 7, 30, 11, 20], [100, 200, 5, -1, 8],
+                                    [2 ** 31 - 1, 0, -2 ** 31, 1, 2 ** 31 - 1], [9, 3, 12, 1, 17]])
 def test_product_keeps_first_rows_inside(dev, starts):
+    """First rows that pass the rows or decrease: taken as documented, nothing written elsewhere."""
     a, sfa, b, sfb = operands(20, 4, 48, 256, seed=4)
     check_product(dev, a, sfa, b, sfb, starts, None, str(starts), CUTS)
-
-
-@pytest.mark.parametrize("starts", [[-5, 3, 2, 9, 40], [7, 7, 30, 11, 20], [100, 200, 5, -1, 8],
-                                    [2 ** 31 - 1, 0, -2 ** 31, 1, 2 ** 31 - 1]])
-def test_product_of_first_rows_that_decrease(dev, starts):
-    """Each row is one of its experts', or has been left: nothing is written elsewhere."""
-    a, sfa, b, sfb = operands(20, 4, 48, 256, seed=4)
-    for cut in CUTS:
-        check_decreasing(dev, a, sfa, b, sfb, starts, cut)
-
-
-def check_decreasing(dev, a, sfa, b, sfb, starts, cut):
     guarded = torch.full((60, 48), 77.0, dtype=torch.bfloat16, device=dev)
-    ex.product(on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev),
-               on(np.array(starts, np.int32), dev), out=guarded[20:40], cut=cut)
-    got = host(guarded.float())
-    assert (got[:20] == 77).all() and (got[40:] == 77).all()
-    right = got[20:40] == 77
-    for e, (lo, hi) in enumerate(H.ranges(starts, 20)):
-        want, mass, _ = H.product(a, sfa, b[e:e + 1], sfb[e:e + 1], [lo, hi])
-        bits = oracle.to_bf16_bits(got[20 + lo:20 + hi])
-        right[lo:hi] |= bf16_compare(bits, want[lo:hi], mass[lo:hi])[0]
-    assert right.all()
+    args = [on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev), on(np.array(starts, np.int32), dev)]
+    for cut in CUTS:
+        ex.product(*args, out=guarded[20:40], cut=cut)
+        assert (guarded[:20] == 77).all() and (guarded[40:] == 77).all()
+
+
+@pytest.mark.parametrize("experts", [70, 300, 1024])
+def test_product_of_many_first_rows_that_decrease(dev, experts):
+    rng = np.random.default_rng(experts)
+    starts = rng.integers(-3, 60, experts + 1)
+    a, sfa, b, sfb = operands(50, experts, 16, 128, seed=6)
+    check_product(dev, a, sfa, b, sfb, starts, None, "%d" % experts, CUTS)
 
 
 def test_product_of_strided_operands(dev):
@@ -486,16 +479,23 @@ def test_refusals(dev):
             (lambda: ex.route(x.half(), 2), TypeError), (lambda: ex.route(x[0], 2), ValueError),
             (lambda: ex.route(x.t(), 2), ValueError), (lambda: ex.route(x.cpu(), 2), ValueError),
             (lambda: ex.route(x, 0), ValueError), (lambda: ex.route(x, 17), GaError),
-            (lambda: ex.route(x, 65), ValueError), (lambda: ex.route(x, 2, scores="tanh"), ValueError),
+            (lambda: ex.route(x, 65), ValueError), (lambda: ex.route(x, 2 ** 32 + 2), ValueError),
+            (lambda: ex.route(x, 2, groups=2 ** 32 + 2), ValueError),
+            (lambda: ex.route(x, 2, groups=2, top_groups=2 ** 32 + 1), ValueError),
+            (lambda: ex.route(x, 2, groups=2, group_rank=2 ** 32 + 2), ValueError),
+            (lambda: ex.route(x, 2, groups=0), ValueError),
+            (lambda: ex.route(x, 2, scale=1e39), GaError),
+            (lambda: ex.arrange(i, 4, 2 ** 32), ValueError),
+            (lambda: ex.arrange(i, 4, 2 ** 31 - 4), ValueError), (lambda: ex.route(x, 2, scores="tanh"), ValueError),
             (lambda: ex.route(x, 2, bias=x[0, :8]), ValueError),
             (lambda: ex.route(x, 2, bias=x[0].double()), TypeError),
             (lambda: ex.route(x, 2, groups=3), GaError),
-            (lambda: ex.route(x, 2, groups=4, top_groups=5), GaError),
+            (lambda: ex.route(x, 2, groups=4, top_groups=5), ValueError),
             (lambda: ex.route(x, 2, ids=i.long()), TypeError),
             (lambda: ex.route(x, 2, weights=x[:, ::8]), ValueError),
             (lambda: ex.arrange(i.long(), 4), TypeError), (lambda: ex.arrange(i[:, ::2], 4), ValueError),
             (lambda: ex.arrange(i[0], 4), ValueError), (lambda: ex.arrange(i, 0), ValueError),
-            (lambda: ex.arrange(i, 1025), ValueError), (lambda: ex.arrange(i, 4, -1), GaError),
+            (lambda: ex.arrange(i, 1025), ValueError), (lambda: ex.arrange(i, 4, -1), ValueError),
             (lambda: ex.arrange(i.cpu(), 4), ValueError),
             (lambda: ex.activate(x), ValueError), (lambda: ex.activate(x[0]), ValueError),
             (lambda: ex.activate(torch.zeros((2, 256), dtype=torch.float16, device=dev)), TypeError),
@@ -523,6 +523,8 @@ def test_products_that_are_refused(dev):
                           (dict(b=b[0]), ValueError), (dict(b=b.transpose(0, 2)), ValueError),
                           (dict(sfb=t[:, :, :1]), ValueError), (dict(starts=starts[:3]), ValueError),
                           (dict(starts=starts.long()), TypeError), (dict(rows=rows.long()), TypeError),
+                          (dict(rows=rows[None]), ValueError), (dict(cut=9), ValueError),
+                          (dict(cut=2 ** 32 + 1), ValueError),
                           (dict(out=torch.zeros((5, 21), dtype=torch.bfloat16, device=dev)), ValueError),
                           (dict(out=torch.zeros((5, 20), device=dev)), TypeError)):
         with pytest.raises(error):
