@@ -846,49 +846,51 @@ __global__ __launch_bounds__(NT) void arrange_kernel(const int* __restrict__ ids
 // ---- activate ---------------------------------------------------------------------
 // A workgroup has kActRows rows of kActBlocks blocks of 128, a wave the blocks of a row at a time:
 // sixteen lanes a block, eight elements of gate and up each, all loads before the first use. The
-// scales, which lie row by row within a block, go through LDS. The exponential and the reciprocal
-// are the hardware's (an element is off by at most |g| 2^-22.6 + 2^-21 of itself, next to a rounding
-// to 2^-4): with the library's, and a division, instructions bound the kernel, 65536 rows of 2048
-// from bf16 167 us; so HBM does, 124 us, 5.4 TB/s. Eight rows a workgroup took as long,
-// 32 rows of one block 167 too.
+// scales, which lie row by row within a block, go through LDS. With the library's exponential and a
+// division instructions bound the kernel, 65536 rows of 2048 from bf16 167 us; with the hardware's,
+// made as exact, HBM does, 125 to 130 us. Eight rows a workgroup took as long.
 constexpr int kActBlocks = 4;
 constexpr int kActRows = 16;
 
 template <int IN>
-__device__ __forceinline__ void load8(const void* x, size_t i, bool wide, float (&v)[8])
+__device__ __forceinline__ void load8(const void* x, size_t i, float (&v)[8])
 {
     if constexpr (IN == GA_IN_F32) {
-        const float* p = (const float*)x + i;
-        if (wide) {
-            const v4f a = *(const v4f*)p, b = *(const v4f*)(p + 4);
+        const v4f_any* p = (const v4f_any*)((const float*)x + i);
+        const v4f a = p[0], b = p[1];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[j] = a[j];
-                v[4 + j] = b[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                v[j] = p[j];
+        for (int j = 0; j < 4; j++) {
+            v[j] = a[j];
+            v[4 + j] = b[j];
         }
     } else {
-        const uint16_t* p = (const uint16_t*)x + i;
-        if (wide) {
-            const v4i a = *(const v4i*)p;
+        const v4i a = *(const v4i_any*)((const uint16_t*)x + i);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[2 * j] = __uint_as_float((uint32_t)a[j] << 16);
-                v[2 * j + 1] = __uint_as_float((uint32_t)a[j] & 0xFFFF0000u);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                v[j] = bf16_to_f32(p[j]);
+        for (int j = 0; j < 4; j++) {
+            v[2 * j] = __uint_as_float((uint32_t)a[j] << 16);
+            v[2 * j + 1] = __uint_as_float((uint32_t)a[j] & 0xFFFF0000u);
         }
     }
 }
 
-template <int IN, bool WIDE>
+// g / (1 + exp(-g)), off by at most 2^-21.4 of itself (the hardware's exponential 2^-23, five
+// roundings): the exponential's argument in two parts, a Newton step for the reciprocal. Zero where
+// 1 / (1 + exp(-g)) is below the least normal number; -inf gives NaN, +inf itself.
+__device__ __forceinline__ float gated(float g)
+{
+    constexpr float kLog2e = 0x1.715476p+0f, kLess = 0x1.4ae0c0p-26f; // to fp32, and what it leaves
+    const float x = -__builtin_amdgcn_fmed3f(g, -88.6f, 200.0f); // beyond, 1 / (1 + exp) is 0 or 1
+    const float t = x * kLog2e;
+    const float rest = fmaf(x, kLess, fmaf(x, kLog2e, -t));
+    float e = __builtin_amdgcn_exp2f(t);
+    e = fmaf(e, rest * 0x1.62e430p-1f, e); // 2^rest = 1 + rest ln 2
+    const float d = 1.0f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    return g * r;
+}
+
+template <int IN>
 __global__ __launch_bounds__(256) void activate_kernel(const void* __restrict__ x, int rows,
                                                        int inner, long long stride_x,
                                                        uint8_t* __restrict__ q, long long stride_q,
@@ -911,8 +913,8 @@ __global__ __launch_bounds__(256) void activate_kernel(const void* __restrict__ 
     for (int u = 0; u < U; u++) {
         const long long r = min(r0 + u * 4 + wave, (long long)live - 1);
         const size_t at = (size_t)r * stride_x + gc * 128 + sub * 8;
-        load8<IN>(x, at, WIDE, gate[u]);
-        load8<IN>(x, at + inner, WIDE, up[u]);
+        load8<IN>(x, at, gate[u]);
+        load8<IN>(x, at + inner, up[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -920,7 +922,7 @@ __global__ __launch_bounds__(256) void activate_kernel(const void* __restrict__ 
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            y[j] = gate[u][j] * __builtin_amdgcn_rcpf(1.0f + __expf(-gate[u][j])) * up[u][j];
+            y[j] = gated(gate[u][j]) * up[u][j];
         bool nan;
         const float s = ds_scale(__uint_as_float(block_amax<16, 8>(y, nan)));
         const ScaleDiv d(s);
@@ -942,8 +944,10 @@ __global__ __launch_bounds__(256) void activate_kernel(const void* __restrict__ 
 }
 
 // ---- combine ----------------------------------------------------------------------
-// A thread has EL elements of a token and adds up its rows', eight rows' loads at a time.
-template <int EL, int OUT>
+// A thread has eight elements of a token and adds up its rows', eight rows' loads at a time; the
+// last elements of a row that are fewer go one by one. HBM bounds it: 8191 tokens x 8 rows of 4096
+// 119 us, 5.1 TB/s.
+template <int OUT>
 __global__ __launch_bounds__(256) void combine_kernel(const uint16_t* __restrict__ y, int rows,
                                                       int n, long long stride_y,
                                                       const int* __restrict__ place,
@@ -952,16 +956,17 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint16_t* __restrict
                                                       int parts)
 {
     const int t = blockIdx.x / parts;
-    const int c = ((blockIdx.x % parts) * 256 + threadIdx.x) * EL;
+    const int c = ((blockIdx.x % parts) * 256 + threadIdx.x) * 8;
     if (c >= n)
         return;
-    float acc[EL];
+    const int here = min(8, n - c);
+    float acc[8];
 #pragma unroll
-    for (int i = 0; i < EL; i++)
+    for (int i = 0; i < 8; i++)
         acc[i] = 0.0f;
     constexpr int B = 8;
     for (int j0 = 0; j0 < top; j0 += B) {
-        uint32_t raw[B][(EL + 1) / 2];
+        v4i raw[B];
         float w[B];
         bool ok[B];
 #pragma unroll
@@ -971,44 +976,51 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint16_t* __restrict
             ok[b] = j0 + b < top && r >= 0 && r < rows;
             w[b] = weights[(size_t)t * top + j];
             const uint16_t* p = y + (size_t)(ok[b] ? r : 0) * stride_y + c;
-            if constexpr (EL == 8) {
-                const v4i d = *(const v4i*)p;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    raw[b][i] = (uint32_t)d[i];
+            if (here == 8) {
+                raw[b] = *(const v4i_any*)p;
             } else {
-                raw[b][0] = *p;
+                raw[b] = (v4i){0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 7; i++)
+                    if (i < here)
+                        raw[b][i / 2] |= (int)((uint32_t)p[i] << (i % 2 * 16));
             }
         }
 #pragma unroll
         for (int b = 0; b < B; b++)
             if (ok[b])
 #pragma unroll
-                for (int i = 0; i < EL; i++) {
-                    const uint32_t u = raw[b][i / 2];
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t u = (uint32_t)raw[b][i / 2];
                     acc[i] = fmaf(w[b], __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16), acc[i]);
                 }
     }
     const size_t o = (size_t)t * stride_out + c;
     if constexpr (OUT == GA_DTYPE_F32) {
         float* p = (float*)out + o;
+        if (here == 8) {
+            *(v4f_any*)p = (v4f){acc[0], acc[1], acc[2], acc[3]};
+            *(v4f_any*)(p + 4) = (v4f){acc[4], acc[5], acc[6], acc[7]};
+        } else {
 #pragma unroll
-        for (int i = 0; i < EL; i += 4)
-            if constexpr (EL == 8)
-                *(v4f*)(p + i) = (v4f){acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
-            else
-                p[i] = acc[i];
+            for (int i = 0; i < 7; i++)
+                if (i < here)
+                    p[i] = acc[i];
+        }
     } else {
         uint16_t* p = (uint16_t*)out + o;
-        if constexpr (EL == 8) {
+        if (here == 8) {
             v4i d;
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 d[i] = (int)((uint32_t)f32_to_bf16(acc[2 * i]) |
                              ((uint32_t)f32_to_bf16(acc[2 * i + 1]) << 16));
-            *(v4i*)p = d;
+            *(v4i_any*)p = d;
         } else {
-            *p = f32_to_bf16(acc[0]);
+#pragma unroll
+            for (int i = 0; i < 7; i++)
+                if (i < here)
+                    p[i] = f32_to_bf16(acc[i]);
         }
     }
 }
@@ -1095,28 +1107,22 @@ ga_status ga_experts_activate(const void* x, int in_dtype, int rows, int inner, 
     const bool one = rows == 1;
     if ((!one && (stride_x < 2ll * inner || stride_q < inner)) || stride_scales < rows)
         return fail(GA_ERR_SHAPE, "experts_activate: rows overlap");
+    if ((uintptr_t)x % (in_dtype == GA_IN_F32 ? 4 : 2))
+        return fail(GA_ERR_SHAPE, "experts_activate: x must have its elements' alignment");
     if ((uintptr_t)q % 8 || (!one && stride_q % 8))
         return fail(GA_ERR_SHAPE, "experts_activate: q must be 8-byte aligned, its stride too");
     const int parts = (inner / 128 + kActBlocks - 1) / kActBlocks;
     const long long groups = parts * ((rows + (long long)kActRows - 1) / kActRows);
     if (groups > most_workgroups(256))
         return fail(GA_ERR_SHAPE, "experts_activate: too many elements for one call");
-    const int el = in_dtype == GA_IN_F32 ? 4 : 8; // elements of 16 bytes
-    const bool wide = (uintptr_t)x % 16 == 0 && (one || stride_x % el == 0);
     const dim3 grid((unsigned)groups);
     hipStream_t st = (hipStream_t)stream;
-    auto go = [&](auto IN, auto WIDE) {
-        hipLaunchKernelGGL((activate_kernel<decltype(IN)::value, decltype(WIDE)::value>), grid,
-                           dim3(256), 0, st, x, rows, inner, stride_x, (uint8_t*)q, stride_q,
-                           scales, stride_scales, limit, parts);
-    };
-    auto kind = [&](auto IN) {
-        wide ? go(IN, std::true_type{}) : go(IN, std::false_type{});
-    };
     if (in_dtype == GA_IN_F32)
-        kind(std::integral_constant<int, GA_IN_F32>{});
+        hipLaunchKernelGGL((activate_kernel<GA_IN_F32>), grid, dim3(256), 0, st, x, rows, inner,
+                           stride_x, (uint8_t*)q, stride_q, scales, stride_scales, limit, parts);
     else
-        kind(std::integral_constant<int, GA_IN_BF16>{});
+        hipLaunchKernelGGL((activate_kernel<GA_IN_BF16>), grid, dim3(256), 0, st, x, rows, inner,
+                           stride_x, (uint8_t*)q, stride_q, scales, stride_scales, limit, parts);
     GA_HIP_CHECK(hipGetLastError());
     return GA_OK;
 }
@@ -1139,26 +1145,21 @@ ga_status ga_experts_combine(const void* y, int rows, int n, long long stride_y,
         return fail(GA_ERR_SHAPE, "experts_combine: rows of %d elements", n);
     if (rows == 0) // every place is left out; what is loaded for it has to be readable
         y = out;
-    const bool wide = n % 8 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)out % 16 == 0 &&
-                      (rows == 1 || stride_y % 8 == 0) && (tokens == 1 || stride_out % 8 == 0);
-    const int el = wide ? 8 : 1;
-    const int parts = (int)(((long long)n + 256 * el - 1) / (256 * el));
+    if ((uintptr_t)y % 2 || (uintptr_t)out % (out_dtype == GA_DTYPE_F32 ? 4 : 2))
+        return fail(GA_ERR_SHAPE, "experts_combine: y and out must have their elements' alignment");
+    const int parts = (n - 1) / 2048 + 1;
     if ((long long)tokens * parts > most_workgroups(256))
         return fail(GA_ERR_SHAPE, "experts_combine: too many elements for one call");
     const dim3 grid((unsigned)(tokens * (long long)parts));
     hipStream_t st = (hipStream_t)stream;
-    auto go = [&](auto EL, auto OUT) {
-        hipLaunchKernelGGL((combine_kernel<decltype(EL)::value, decltype(OUT)::value>), grid,
-                           dim3(256), 0, st, (const uint16_t*)y, rows, n, stride_y, place, weights,
-                           top, out, stride_out, parts);
-    };
-    auto kind = [&](auto EL) {
-        if (out_dtype == GA_DTYPE_F32)
-            go(EL, std::integral_constant<int, GA_DTYPE_F32>{});
-        else
-            go(EL, std::integral_constant<int, GA_DTYPE_BF16>{});
-    };
-    wide ? kind(std::integral_constant<int, 8>{}) : kind(std::integral_constant<int, 1>{});
+    if (out_dtype == GA_DTYPE_F32)
+        hipLaunchKernelGGL((combine_kernel<GA_DTYPE_F32>), grid, dim3(256), 0, st,
+                           (const uint16_t*)y, rows, n, stride_y, place, weights, top, out,
+                           stride_out, parts);
+    else
+        hipLaunchKernelGGL((combine_kernel<GA_DTYPE_BF16>), grid, dim3(256), 0, st,
+                           (const uint16_t*)y, rows, n, stride_y, place, weights, top, out,
+                           stride_out, parts);
     GA_HIP_CHECK(hipGetLastError());
     return GA_OK;
 }

@@ -94,6 +94,12 @@ __device__ __forceinline__ uint32_t buf_load4(__amdgpu_buffer_rsrc_t r, uint32_t
     return __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0);
 }
 
+// Vectors at addresses of their elements' alignment: one instruction all the same, global memory
+// takes any alignment (a few more cycles where a line ends inside).
+typedef v4i v4i_any __attribute__((aligned(2)));
+typedef v4f v4f_any __attribute__((aligned(4)));
+typedef v2i v2i_any __attribute__((aligned(2)));
+
 // s_waitcnt encodings for gfx9: vmcnt[3:0] + vmcnt_hi[15:14], expcnt[6:4],
 // lgkmcnt[11:8]. Only vmcnt is waited on here.
 template <int N>

@@ -46,11 +46,12 @@ __device__ __forceinline__ uint2 bf16x4(const v4f& v)
 
 // Four results of row m, columns n .. n + 3, those below N.
 __device__ __forceinline__ void expert_store4(uint16_t* out, long long ld, int m, int n, int N,
-                                              bool even, const v4f& v)
+                                              const v4f& v)
 {
     uint16_t* o = out + (size_t)m * ld + n;
-    if (even && n + 4 <= N) {
-        *(uint2*)o = bf16x4(v);
+    if (n + 4 <= N) {
+        const uint2 d = bf16x4(v);
+        *(v2i_any*)o = (v2i){(int)d.x, (int)d.y};
     } else {
         for (int e = 0; e < 4 && n + e < N; e++)
             o[e] = f32_to_bf16(v[e]);
@@ -154,13 +155,12 @@ void experts_few_kernel(ga_experts_product_args a, int shares, int ks, int gps)
 
     // lane holds out[m][n .. n+3], m = 16i + lane%16, n = 16cg + 4(lane/16)
     uint16_t* out = (uint16_t*)a.out + (size_t)row0 * a.stride_out;
-    const bool even = ((uintptr_t)a.out & 7) == 0 && (a.stride_out & 3) == 0;
     auto store = [&](int c, int i, const v4f& v) {
         const int n = (cg0 + c) * 16 + g * 4;
         const int m = i * 16 + r;
         if (c >= ng_here || n >= N || m >= M)
             return;
-        expert_store4(out, a.stride_out, m, n, N, even, v);
+        expert_store4(out, a.stride_out, m, n, N, v);
     };
     bd_join<TM, NG>(smem, wave, lane, slice, tl, ks, live, acc, store);
 }
@@ -282,7 +282,7 @@ __device__ __forceinline__ bspp::BsRead expert_read_setup(char* smem, int lane, 
 
 // A tile's results to out: quadrant q of ROWS / 128 * NB, rows first, `result(q, i, t)` of its 16x16
 // tile i, t: lane l holds row l % 16, columns 4 (l / 16) on. Through LDS, so that whole rows are
-// written (rows below M; columns below N, a multiple of 8), where out is aligned for it.
+// written (those below M, columns below N).
 template <int ROWS, int NB, class Result>
 __device__ __forceinline__ void expert_store(const ga_experts_product_args& a, char* smem, int row0,
                                              int M, int n0, int wave, int lane, const Result& result)
@@ -290,10 +290,7 @@ __device__ __forceinline__ void expert_store(const ga_experts_product_args& a, c
     const int grp = wave >> 2, simd = wave & 3, N = a.n - n0;
     const long long ld = a.stride_out;
     uint16_t* out = (uint16_t*)a.out + (size_t)row0 * ld + n0;
-    const bool wide = ((uintptr_t)a.out & 15) == 0 && (ld & 7) == 0 && (N & 7) == 0;
-    const bool even = ((uintptr_t)a.out & 7) == 0 && (ld & 3) == 0;
-    if (wide)
-        barrier_lds(); // every wave's operand and scale reads are done
+    barrier_lds(); // every wave's operand and scale reads are done
 #pragma unroll
     for (int q = 0; q < ROWS / 128 * NB; q++)
 #pragma unroll
@@ -302,24 +299,25 @@ __device__ __forceinline__ void expert_store(const ga_experts_product_args& a, c
             for (int t = 0; t < 2; t++) {
                 const int m = q / NB * 128 + grp * 64 + i * 16 + (lane & 15);
                 const int n = q % NB * 128 + simd * 32 + t * 16 + (lane >> 4) * 4;
-                if (wide)
-                    *(uint2*)(smem + m * pp::kStagePitch + n * 2) = bf16x4(result(q, i, t));
-                else if (m < M && n < N)
-                    expert_store4(out, ld, m, n, N, even, result(q, i, t));
+                *(uint2*)(smem + m * pp::kStagePitch + n * 2) = bf16x4(result(q, i, t));
             }
-    if (!wide)
-        return;
     barrier_lds();
     constexpr int kLanes = NB * 16; // lanes of a row
 #pragma unroll
     for (int it = 0; it < ROWS / 8 * kLanes / 64; it++) {
         const int row = wave * (ROWS / 8) + it * (64 / kLanes) + lane / kLanes;
         const int col = lane % kLanes * 8;
-        if (row < M && col < N)
+        if (row >= M || col >= N)
+            continue;
+        uint16_t* o = out + (size_t)row * ld + col;
+        const char* from = smem + row * pp::kStagePitch + col * 2;
+        if (col + 8 <= N)
             // non-temporal: 6000 rows of 60 experts of 2048x1408 65.3 -> 61.7 us, 65536 of 64 of
             // 4096x4096 1 % less; a layer, whose activation reads them next, no slower
-            __builtin_nontemporal_store(*(const v4i*)(smem + row * pp::kStagePitch + col * 2),
-                                        (v4i*)(out + (size_t)row * ld + col));
+            __builtin_nontemporal_store(*(const v4i*)from, (v4i_any*)o);
+        else
+            for (int e = 0; e < N - col; e++)
+                o[e] = ((const uint16_t*)from)[e];
     }
 }
 
@@ -518,6 +516,8 @@ extern "C" ga_status ga_experts_product(const ga_experts_product_args* args, voi
         return GA_OK;
     if (!a.a || !a.sfa || !a.b || !a.sfb || !a.starts || !a.out)
         return fail(GA_ERR_ARG, "experts_product: null pointer");
+    if ((uintptr_t)a.out % 2)
+        return fail(GA_ERR_SHAPE, "experts_product: out must have its elements' alignment");
     if (a.a_rows < (a.rows_of ? 1 : a.rows))
         return fail(GA_ERR_SHAPE, "experts_product: a has %lld rows", a.a_rows);
     if (((uintptr_t)a.a | (uintptr_t)a.b | (unsigned long long)a.stride_a |
