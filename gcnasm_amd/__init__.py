@@ -13,6 +13,8 @@ Python modules:
              handle and split-K reduce
   mx4_cache  a key/value cache in MXFP4: append, attention over it, the weights of
              its tokens, eviction
+  experts    layers of experts: the choice of each token's experts, the map of rows, each
+             expert's rows times its weights in block scale, activation and weighted sum
   ops        tensor-level conveniences (torch tensors as device buffers)
 """
 from ._lib import GaError, lib  # noqa: F401
