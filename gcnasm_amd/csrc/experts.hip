@@ -18,7 +18,7 @@ namespace {
 //
 // Keys with a bias are sums that 32 bits round; the choice is that of 64 bits. It is made in 32
 // bits first, with a bound of what they are off by, and again in 64 where two keys that
-// decide it lie within that bound (of random logits one token in a hundred): instructions bound
+// decide it lie within that bound (31 of 16384 random tokens): instructions bound
 // this kernel, and exponentials and comparisons of 64 bits cost two to four times as many.
 // 16384 tokens, 192 experts in 8 groups, sigmoid and bias: 64 bits throughout 25.4 us, so 17.3.
 
@@ -92,7 +92,15 @@ constexpr float kMinus = -__builtin_inff();
 // argument, the exponential and the sum of up to 1024 of them, at most 2^-19 of a score in all.
 constexpr float kScoreError = 0x1p-18f;
 
-// A token's logits: -inf for those that are not there (-inf, NaN), +inf as the largest finite value.
+// A logit: -inf where it is not there (-inf, NaN), +inf as its type's largest finite value.
+template <int IN>
+__device__ __forceinline__ float logit_at(const void* p, long long i)
+{
+    const float x =
+        IN == GA_IN_F32 ? ((const float*)p)[i] : bf16_to_f32(((const uint16_t*)p)[i]);
+    return x > kMinus ? fminf(x, IN == GA_IN_F32 ? 0x1.FFFFFEp127f : 0x1.FEp127f) : kMinus;
+}
+
 template <int VPT>
 struct RouteToken {
     float x[VPT];
@@ -128,6 +136,9 @@ __device__ __forceinline__ uint32_t packed(float x, float top, float steps, int 
     const float d = 4194303.0f - (top - x) * steps;
     return (uint32_t)fmaxf(d, 1.0f) << 10 | (uint32_t)(1023 - index);
 }
+// Steps that numbers off by so many steps together have to be apart: those of the packing's own roundings
+// more, at most all there are.
+__device__ __forceinline__ uint32_t steps_apart(float off) { return 2 + (uint32_t)fminf(off, 4194303.0f); }
 __device__ __forceinline__ int index_of(uint32_t key) { return 1023 - (int)(key & 1023u); }
 
 // The two largest of a group's values, at its first lane.
@@ -346,11 +357,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
     const int shift = 31 - __builtin_clz(64 / a.groups); // log2 of the lanes of a group
 
     const long long row = token * a.stride_logits;
-    auto logit = [&](int e) {
-        const float x = IN == GA_IN_F32 ? ((const float*)a.logits)[row + e]
-                                        : bf16_to_f32(((const uint16_t*)a.logits)[row + e]);
-        return x > kMinus ? fminf(x, 3.40282347e38f) : kMinus;
-    };
+    auto logit = [&](int e) { return logit_at<IN>(a.logits, row + e); };
     RouteToken<VPT> t;
     t.lane = lane;
     float top = kMinus;
@@ -412,7 +419,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
                 f[v * 64 + lane] = by[v];
         wave_lds_fence();
         const float gsteps = by_score ? kSumSteps : steps; // sums are off by twice as much
-        kept = kept_groups_packed(a, f, lane, shift, gsteps, 2 + (uint32_t)(2.0f * off * gsteps),
+        kept = kept_groups_packed(a, f, lane, shift, gsteps, steps_apart(2.0f * off * gsteps),
                                   sure);
         wave_lds_fence(); // read before 64 bits are written there
 #pragma unroll
@@ -438,7 +445,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(ga_experts_rout
         }
         sure = best < __builtin_inff();
         bool apart = true;
-        id = choose_packed<VPT>(lane, pack, a.top, 2 + (uint32_t)(off * steps), apart);
+        id = choose_packed<VPT>(lane, pack, a.top, steps_apart(off * steps), apart);
         sure &= bf16 || apart;
     }
     if (!sure)
@@ -505,34 +512,33 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts
     const bool softmax = a.scores == GA_EXPERTS_SOFTMAX, grouped = a.top_groups < a.groups;
     const bool by_score = a.bias || (grouped && a.group_rank == 2);
 
-    auto there = [](float x) { return x > kMinus ? fminf(x, 3.40282347e38f) : kMinus; };
     const long long row = token * a.stride_logits;
-    auto logit = [&](long long at, int e) {
-        return there(IN == GA_IN_F32 ? ((const float*)a.logits)[at + e]
-                                     : bf16_to_f32(((const uint16_t*)a.logits)[at + e]));
-    };
     float x[VPT], largest = kMinus;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         const int e = c * 64 + r * 4;
         if (vector) { // E a multiple of 4, rows aligned
-            const int f = min(e, E - 4);
+            const long long f = row + min(e, E - 4);
+            const float none = kMinus;
             if constexpr (IN == GA_IN_F32) {
-                const v4f d = *(const v4f*)((const float*)a.logits + row + f);
+                const v4f d = *(const v4f*)((const float*)a.logits + f);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    x[4 * c + i] = e < E ? there(d[i]) : kMinus;
+                    x[4 * c + i] = e < E && d[i] > none ? fminf(d[i], 0x1.FFFFFEp127f) : none;
             } else {
-                const uint2 d = *(const uint2*)((const uint16_t*)a.logits + row + f);
+                const uint2 d = *(const uint2*)((const uint16_t*)a.logits + f);
                 const uint32_t u[4] = {d.x << 16, d.x & 0xFFFF0000u, d.y << 16, d.y & 0xFFFF0000u};
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    x[4 * c + i] = e < E ? there(__uint_as_float(u[i])) : kMinus;
+                for (int i = 0; i < 4; i++) {
+                    const float y = __uint_as_float(u[i]);
+                    x[4 * c + i] = e < E && y > none ? fminf(y, 0x1.FEp127f) : none;
+                }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                x[4 * c + i] = e + i < E ? logit(row, min(e + i, E - 1)) : kMinus;
+                x[4 * c + i] =
+                    e + i < E ? logit_at<IN>(a.logits, row + min(e + i, E - 1)) : kMinus;
         }
     }
 #pragma unroll
@@ -596,7 +602,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts
         const bool leads = g < a.groups && (r & ((1 << shift) - 1)) == 0 && value > kMinus;
         const float top = row_max(leads ? value : kMinus);
         const float gsteps = by_score ? kSumSteps : steps;
-        const uint32_t gap = 2 + (uint32_t)(2.0f * off * gsteps);
+        const uint32_t gap = steps_apart(2.0f * off * gsteps);
         uint32_t gkey = leads ? packed(value, top, gsteps, g) : 0u, last = 0, kept = 0;
         for (int j = 0; j <= a.top_groups; j++) {
             const uint32_t best = row_max(gkey);
@@ -645,7 +651,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts
     // The next key after `last` is last + the largest of (key - last) mod 2^32: of keys below last,
     // which wrap, the largest is the nearest, and any of them is above those that do not wrap. So
     // nothing has to be taken out.
-    const uint32_t gap = 2 + (uint32_t)(off * steps);
+    const uint32_t gap = steps_apart(off * steps);
     bool apart = true;
     uint32_t last = 0;
     int id = -1;
@@ -674,7 +680,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const int e = c * 64 + lane;
-            t.x[c] = e < E ? logit(at, min(e, E - 1)) : kMinus;
+            t.x[c] = e < E ? logit_at<IN>(a.logits, at + min(e, E - 1)) : kMinus;
         }
         if (grouped)
             wave_lds_fence(); // what was there has been read
@@ -685,7 +691,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts
     }
 
     // weights: each relative to the largest of the chosen logits, which so cancels
-    const float xi = id >= 0 ? logit(row, id) : kMinus;
+    const float xi = id >= 0 ? logit_at<IN>(a.logits, row + id) : kMinus;
     const float from = row_max(xi);
     float w = id >= 0 ? weight_of(a, xi, from, largest, sum) : 0.0f;
     if (a.renormalise) {

@@ -749,8 +749,8 @@ ga_status ga_mx4_evict(const ga_mx4_cache* cache, const ga_mx4_evict_args* args,
  * bias, of the two largest scores). Of these experts the `top` of largest key are chosen, in
  * that order; of equal keys, as of equal groups, the lowest index comes first. weights are the
  * scores of the chosen ones, divided by their sum if renormalise, times scale. A logit or bias
- * of -inf or NaN takes an expert out (logits +inf count as the largest finite value); where
- * fewer than `top` experts are left, ids are -1 and weights 0. */
+ * of -inf or NaN takes an expert out (a logit +inf counts as its type's largest finite value);
+ * where fewer than `top` experts are left, ids are -1 and weights 0. */
 typedef struct ga_experts_route_args {
     const void* logits;
     const float* bias;

@@ -4,12 +4,12 @@ import numpy as np
 import oracle
 
 
-def scores(x, kind):
+def scores(x, kind, most):
     """Scores of logits [T, E]: those that are not there (-inf, NaN) have none, +inf counts as the
-    largest finite value."""
+    type's largest finite value."""
     x = np.asarray(x, np.float64)
     there = x > -np.inf
-    x = np.where(there, np.minimum(x, np.float64(np.finfo(np.float32).max)), -np.inf)
+    x = np.where(there, np.minimum(x, most), -np.inf)
     with np.errstate(all="ignore"):
         if kind == "softmax":
             m = x.max(1, keepdims=True)
@@ -21,9 +21,9 @@ def scores(x, kind):
 
 
 def route(logits, top, bias=None, kind="softmax", groups=1, top_groups=None, group_rank=1,
-          renormalise=True, scale=1.0):
+          renormalise=True, scale=1.0, most=float(np.finfo(np.float32).max)):
     """ids [T, top] and weights [T, top] (float64)."""
-    x, there, p = scores(logits, kind)
+    x, there, p = scores(logits, kind, most)
     T, E = x.shape
     key = x.copy()
     if bias is not None:

@@ -33,7 +33,8 @@ def check_route(dev, logits, top, dtype, bias=None, **kw):
     x = torch.from_numpy(np.asarray(logits, np.float32)).to(dtype)
     b = None if bias is None else np.asarray(bias, np.float32)
     names = dict(kw)
-    want, w = H.route(host(x.float()), top, b, names.pop("scores", "softmax"), **names)
+    want, w = H.route(host(x.float()), top, b, names.pop("scores", "softmax"),
+                      most=torch.finfo(dtype).max, **names)
     ids, weights = ex.route(x.to(dev), top, None if b is None else on(b, dev), **kw)
     assert ids.dtype == torch.int32 and weights.dtype == torch.float32
     assert np.array_equal(host(ids), want)
@@ -89,6 +90,33 @@ def test_route_of_equal_and_missing_experts(dev, scores, bias):
         for renorm in (True, False):
             check_route(dev, x, top, torch.float32, b if bias else None, scores=scores,
                         groups=groups, top_groups=kept, group_rank=rank, renormalise=renorm)
+
+
+@pytest.mark.parametrize("experts,groups", [(48, 1), (250, 5), (256, 16), (600, 20), (1024, 1)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_by_keys_that_32_bits_do_not_tell_apart(dev, experts, groups, scores):
+    """Biases that leave of the scores what their rounding to fp32 does: keys of 2^-25 of them, in an
+    order that only 64 bits have. (Two keys of 64 bits are that near each other with a chance of
+    2^-20 here.)"""
+    rng = np.random.default_rng(experts)
+    x = np.tile(rng.standard_normal(experts).astype(np.float32), (7, 1))
+    bias = -H.scores(x[:1], scores, np.inf)[2][0].astype(np.float32)
+    for rank in (1, 2):
+        check_route(dev, x, 5, torch.float32, bias, scores=scores, groups=groups,
+                    top_groups=max(1, groups // 2), group_rank=rank)
+    # far from zero, where fp32 has steps of 2^-10, 1024 and more
+    for far in (2.0 ** 13, -2.0 ** 33, 1e30):
+        check_route(dev, rng.standard_normal((9, experts)), 4, torch.float32,
+                    far + rng.integers(0, 3, experts) * abs(far) * 2.0 ** -23, scores=scores)
+
+
+def test_route_of_the_largest_logits(dev):
+    """Of bf16 its own largest value is what an infinity counts as."""
+    x = np.zeros((3, 70), np.float32)
+    x[:, 40], x[:, 20], x[1, 3] = np.inf, 3.3895313892515355e38, np.inf
+    for dtype in (torch.float32, torch.bfloat16):
+        for E in (33, 70):
+            check_route(dev, np.roll(x, -9, 1)[:, :E], 3, dtype)
 
 
 def test_route_takes_rows_of_a_wider_matrix_and_given_results(dev):
