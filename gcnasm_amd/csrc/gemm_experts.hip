@@ -449,28 +449,30 @@ ga_status launch_tiles(const ga_experts_product_args& a, int height, int width, 
 }
 
 // How a product is cut: a workgroup's rows and columns, its slices of K (0: an eight-wave tile),
-// how many a CU has at a time, its start and its time for a 128-K step in us.
+// how many a CU has at a time, its start and its time for a 128-K step in us, and a CU's time for
+// a whole tile's 128 of K when all CUs are busy for long.
 struct ExpertCut {
     int height, width, ks, at_once;
-    float start, step;
+    float start, step, full;
 };
 
 // The cut with the smallest estimated time. The counts are on the GPU, so the tiles are those of
-// rows spread over the experts by chance. A call's time is that of its rounds of workgroups,
-// but at least what its bytes take from memory (active weights, rows, results) and what all its
-// copies take from the caches. The coefficients are a fit to 1491 problems measured on MI355X with
-// every cut (2-256 experts, 1-800 rows each, N 100-7168, K 256-7168): the cut it picks is on
-// average 2.5 % slower than the fastest, at the worst 1.6 times (few rows of 2 experts). One
-// cut for all would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take 132
-// us in 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in
+// rows spread over the experts by chance. A call's time is that of its rounds of workgroups (a last
+// one that is not full between its part and a whole one), but at least what its bytes take from
+// memory (active weights, rows, results) and its tiles at full rate. The coefficients are a fit to
+// 1995 problems measured on MI355X with every cut (2-256 experts, 1-4000 rows each, N 64-7168, K
+// 256-7168): the cut it picks is on average 2 % slower than the fastest, at the worst 1.4 times.
+// One cut for all would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take
+// 132 us in 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in
 // 16x32, 62 in 128x256, 83 in 256x256; 64 of 4096x4096 with 1024 rows 3490 in 16x256, 1330 in
-// 128x256, 1150 in 256x256.
+// 128x256, 1150 in 256x256; 60 of 99x6272 with 1354 rows 215, 143, 151, and 104 in 128x128.
 const ExpertCut& expert_cut(const ga_experts_product_args& a, int num_cu)
 {
     static const ExpertCut kCuts[GA_EXPERTS_CUTS] = {
-        {16, 64, 2, 2, 4.35f, 0.17f}, {16, 32, 4, 2, 2.53f, 0.25f}, {16, 256, 1, 2, 2.71f, 0.35f},
-        {64, 256, 1, 2, 6.25f, 0.76f}, {64, 64, 4, 2, 4.51f, 0.66f}, {128, 128, 0, 1, 2.83f, 0.46f},
-        {128, 256, 0, 1, 5.01f, 0.81f}, {256, 256, 0, 1, 6.14f, 0.94f}};
+        {16, 64, 2, 2, 3.97f, 0.16f, 0.16f},  {16, 32, 4, 2, 4.10f, 0.27f, 0.14f},
+        {16, 256, 1, 2, 2.34f, 0.45f, 0.55f}, {64, 256, 1, 2, 3.43f, 1.39f, 0.60f},
+        {64, 64, 4, 2, 3.20f, 0.70f, 0.35f},  {128, 128, 0, 1, 2.44f, 0.49f, 0.61f},
+        {128, 256, 0, 1, 3.60f, 0.77f, 0.90f}, {256, 256, 0, 1, 5.09f, 1.08f, 1.35f}};
     if (a.cut)
         return kCuts[a.cut - 1];
     const float n = (float)a.n, k = (float)a.k, rows = (float)a.rows;
@@ -482,10 +484,10 @@ const ExpertCut& expert_cut(const ga_experts_product_args& a, int num_cu)
         const float tiles = std::max(active, rows / c.height + 0.5f * active);
         const float groups = tiles * ((a.n - 1) / c.width + 1);
         const int slices = std::max(1, c.ks), steps = (a.k / 128 + slices - 1) / slices;
-        const float rounds = std::max(1.0f, groups / (num_cu * c.at_once));
-        const float copies = groups * k * (std::min((float)c.width, n) +
-                                           std::min((float)c.height, rows / active)) / 12.0e6f;
-        const float t = std::max(rounds * (c.start + steps * c.step), std::max(memory, copies));
+        const float part = groups / (num_cu * c.at_once);
+        const float rounds = part > 1.0f ? 0.5f * (part + std::ceil(part)) : 1.0f;
+        const float full = groups * (a.k / 128) * c.full / num_cu;
+        const float t = std::max(std::max(rounds * (c.start + steps * c.step), full), memory);
         if (!best || t < least) {
             best = &c;
             least = t;
