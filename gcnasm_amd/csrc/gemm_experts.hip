@@ -457,37 +457,39 @@ struct ExpertCut {
 };
 
 // The cut with the smallest estimated time. The counts are on the GPU, so the tiles are those of
-// rows spread over the experts by chance. A call's time is that of its rounds of workgroups (a last
-// one that is not full between its part and a whole one), but at least what its bytes take from
-// memory (active weights, rows, results) and its tiles at full rate. The coefficients are a fit to
-// 1995 problems measured on MI355X with every cut (2-256 experts, 1-4000 rows each, N 64-7168, K
-// 256-7168): the cut it picks is on average 2 % slower than the fastest, at the worst 1.4 times.
-// One cut for all would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take
-// 132 us in 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in
-// 16x32, 62 in 128x256, 83 in 256x256; 64 of 4096x4096 with 1024 rows 3490 in 16x256, 1330 in
-// 128x256, 1150 in 256x256; 60 of 99x6272 with 1354 rows 215, 143, 151, and 104 in 128x128.
+// rows spread over the experts by chance. A call takes its rounds of workgroups (a last one that is
+// not full counts as between its part and a whole one) or, where that is longer, its tiles at full
+// rate; about where they are equal it takes longer than both, as the fourth root of the sum of
+// fourth powers does. The coefficients are a fit to 2359 problems measured on MI355X with every
+// cut (2-256 experts, 1-4000 rows each, N 64-7168, K 256-7168): the cut it picks is on average 2 %
+// slower than the fastest, at the worst 1.4 times, of 99 in 100 at most 1.26. One cut for all
+// would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take 132 us in
+// 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in 16x32, 62 in
+// 128x256, 83 in 256x256; 64 of 4096x4096 with 64 rows 498, 198, 198, and 285 in 64x256; with 1024
+// rows 6450, 1330, 1120; 60 of 99x6272 with 1354 rows 400, 143, 151, and 104 in 128x128.
 const ExpertCut& expert_cut(const ga_experts_product_args& a, int num_cu)
 {
     static const ExpertCut kCuts[GA_EXPERTS_CUTS] = {
-        {16, 64, 2, 2, 3.97f, 0.16f, 0.16f},  {16, 32, 4, 2, 4.10f, 0.27f, 0.14f},
-        {16, 256, 1, 2, 2.34f, 0.45f, 0.55f}, {64, 256, 1, 2, 3.43f, 1.39f, 0.60f},
-        {64, 64, 4, 2, 3.20f, 0.70f, 0.35f},  {128, 128, 0, 1, 2.44f, 0.49f, 0.61f},
-        {128, 256, 0, 1, 3.60f, 0.77f, 0.90f}, {256, 256, 0, 1, 5.09f, 1.08f, 1.35f}};
+        {16, 64, 2, 2, 3.80f, 0.15f, 0.14f},   {16, 32, 4, 2, 3.65f, 0.28f, 0.10f},
+        {16, 256, 1, 2, 1.94f, 0.48f, 0.96f},  {64, 256, 1, 2, 3.46f, 1.37f, 0.69f},
+        {64, 64, 4, 2, 3.20f, 0.62f, 0.35f},   {128, 128, 0, 1, 2.58f, 0.49f, 0.57f},
+        {128, 256, 0, 1, 3.98f, 0.77f, 0.87f}, {256, 256, 0, 1, 4.95f, 1.19f, 0.97f}};
     if (a.cut)
         return kCuts[a.cut - 1];
-    const float n = (float)a.n, k = (float)a.k, rows = (float)a.rows;
-    const float active = a.experts * (1.0f - std::exp(-rows / a.experts));
-    const float memory = (active * n * k + 0.25f * rows * k + 2.0f * rows * n) / 6.0e6f;
+    const double rows = a.rows;
+    const double active = a.experts * (1.0 - std::exp(-rows / a.experts));
     const ExpertCut* best = nullptr;
-    float least = 0.0f;
+    double least = 0.0;
     for (const ExpertCut& c : kCuts) {
-        const float tiles = std::max(active, rows / c.height + 0.5f * active);
-        const float groups = tiles * ((a.n - 1) / c.width + 1);
+        const double tiles = std::max(active, rows / c.height + 0.5 * active);
+        const double groups = tiles * ((a.n - 1) / c.width + 1);
         const int slices = std::max(1, c.ks), steps = (a.k / 128 + slices - 1) / slices;
-        const float part = groups / (num_cu * c.at_once);
-        const float rounds = part > 1.0f ? 0.5f * (part + std::ceil(part)) : 1.0f;
-        const float full = groups * (a.k / 128) * c.full / num_cu;
-        const float t = std::max(std::max(rounds * (c.start + steps * c.step), full), memory);
+        const double part = groups / (num_cu * c.at_once);
+        const double rounds = part > 1.0 ? 0.5 * (part + std::ceil(part)) : 1.0;
+        const double in_rounds = rounds * (c.start + steps * c.step);
+        const double at_full = groups / num_cu * (a.k / 128) * c.full;
+        const double t = in_rounds * in_rounds * in_rounds * in_rounds +
+                         at_full * at_full * at_full * at_full;
         if (!best || t < least) {
             best = &c;
             least = t;
