@@ -38,10 +38,13 @@ __device__ __forceinline__ uint32_t row_offset(const ga_experts_product_args& a,
     return m >= 0 && m < a.a_rows ? (uint32_t)m * ld : kNowhere;
 }
 
+// The hardware's conversion (v_cvt_pk_bf16_f32, to the nearest, ties to even): in integer operations it
+// was 4 to 20 % of a call, 65536 rows of 64 experts of 4096x4096 1153 -> 1100 us, of 4096x1024 438 -> 373.
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ uint2 bf16x4(const v4f& v)
 {
-    return make_uint2((uint32_t)f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
-                      (uint32_t)f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
+    return __builtin_bit_cast(uint2, __builtin_convertvector(v, v4bf));
 }
 
 // Four results of row m, columns n .. n + 3, those below N.

@@ -269,6 +269,34 @@ def test_product_of_strided_operands(dev):
         assert (O == 5.0).all()  # nothing beside
 
 
+@pytest.mark.parametrize("n", [64, 255])
+def test_product_rounds_to_the_nearest_bfloat16(dev, n):
+    """Rows with one element, so that a result is a product in fp32: its rounding, ties, denormal
+    numbers, what passes the largest, NaN."""
+    rng = np.random.default_rng(n)
+    rows, k, starts = 300, 256, np.array([0, 7, 7, 140, 300], np.int32)
+    codes = np.setdiff1d(np.arange(256), [0x00, 0x80, 0x7F, 0xFF])
+    a = np.zeros((rows, k), np.uint8)
+    a[:, 3] = rng.choice(codes, rows)
+    a[5, 3] = 0x7F
+    b = rng.choice(codes, (4, n, k)).astype(np.uint8)
+    power = rng.integers(-140, 118, rows)
+    power[100:200] = rng.integers(-3, 3, 100)
+    s = rng.choice([1.0, 1.5, 1.25, 1.75, 1 + 2.0 ** -9, 1 + 2.0 ** -23, 1.3], rows)
+    sfa = np.ones((2, rows), np.float32)
+    sfa[0] = np.ldexp(s, power)
+    sfb = np.ones((4, (n + 127) // 128, 2), np.float32)
+    table = oracle.e4m3_decode_table().astype(np.float32)
+    expert = np.searchsorted(starts, np.arange(rows), side="right") - 1
+    with np.errstate(all="ignore"):
+        want = bf16(table[a[:, 3]][:, None] * table[b[expert, :, 3]] * sfa[0][:, None]).float()
+    assert (want.abs() == np.inf).any() and (want[5] != want[5]).all()
+    assert ((want != 0) & (want.abs() < 2.0 ** -126)).any()
+    for cut in CUTS:
+        out = ex.product(on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev), on(starts, dev), cut=cut)
+        assert torch.equal(out.float().cpu().nan_to_num(nan=7e37), want.nan_to_num(nan=7e37))
+
+
 def test_product_scales_with_infinity_stay_in_their_rows(dev):
     """An infinite or NaN scale of one row leaves the others, also those that are nowhere."""
     a, sfa, b, sfb = operands(6, 2, 32, 256, seed=11)
