@@ -77,14 +77,6 @@ __device__ __forceinline__ float unordered(uint32_t k)
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// LDS of one wave alone: what its lanes wrote is there, what they read has been.
-__device__ __forceinline__ void wave_lds_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 constexpr int kRouteWaves = 4;
 constexpr float kMinus = -__builtin_inff();
 

@@ -173,6 +173,14 @@ __device__ __forceinline__ v8i hi16(v8i x)
     return (v8i){x[4], x[5], x[6], x[7], 0, 0, 0, 0};
 }
 
+// LDS of one wave alone: what its lanes wrote is there, what they read has been.
+__device__ __forceinline__ void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // fp32 -> bf16 round to nearest even (quiet NaN kept quiet).
 __device__ __forceinline__ uint16_t f32_to_bf16(float x)
 {

@@ -208,31 +208,49 @@ __device__ __forceinline__ void issue_a(const ExpertLoad<GATHER>& L, char* smem,
     }
 }
 
+// Steps of 32 columns to copy c (0 .. 3) of 64 positions (expert_column).
+__device__ __forceinline__ constexpr uint32_t column_step(int c) { return (c >> 1) + 4 * (c & 1); }
+
+template <bool GATHER>
+__device__ __forceinline__ void issue_b(const ExpertLoad<GATHER>& L, char* smem, int h, int t,
+                                        int wave)
+{
+    char* dst = smem + pp::kBRegion + (t & 1) * pp::kOpSlot + h * pp::kHalf + wave * 1024;
+    const uint32_t o = (uint32_t)t * 128;
+    lds_load16(L.rb, (lds_void*)dst, L.vb, pp::uni(o + column_step(2 * h) * L.b_hstep));
+    lds_load16(L.rb, (lds_void*)(dst + 8192), L.vb,
+               pp::uni(o + column_step(2 * h + 1) * L.b_hstep));
+}
+
 template <int NB, int MODE, bool GATHER>
 __device__ __forceinline__ void issue_half(const ExpertLoad<GATHER>& L, char* smem, int t, int slot,
                                            int wave)
 {
     using H = bspp::BsHalfCfg<NB>;
-    if constexpr (!GATHER) {
-        bspp::issue_half<NB, MODE>((const bspp::BsLoad&)L, smem, t, slot, wave);
-    } else {
-        char* dst = smem + slot * H::kSlot + wave * 1024;
-        const uint32_t o = (uint32_t)t * 128;
-        lds_load16(L.ra, (lds_void*)dst, L.vrow[0] + pp::uni(o), 0);
-        lds_load16(L.ra, (lds_void*)(dst + 8192), L.vrow[1] + pp::uni(o), 0);
+    char* dst = smem + slot * H::kSlot + wave * 1024;
+    const uint32_t o = (uint32_t)t * 128;
+    lds_load16(L.ra, (lds_void*)dst, (GATHER ? L.vrow[0] : L.va) + pp::uni(o), 0);
+    lds_load16(L.ra, (lds_void*)(dst + 8192),
+               GATHER ? L.vrow[1] + pp::uni(o) : L.va + pp::uni(o + L.a_hstep), 0);
 #pragma unroll
-        for (int c = 0; c < 2 * NB; c++)
-            lds_load16(L.rb, (lds_void*)(dst + pp::kHalf + c * 8192),
-                       L.vb + pp::uni(o + c * L.b_hstep), 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            L.rs,
-            (lds_void*)(smem + H::kScaleBase + (t & (H::kRing - 1)) * bspp::kSSlot + wave * 256), 4,
-            L.vs + pp::uni((uint32_t)t * L.s_kstep), 0, 0, 0);
-    }
+    for (int c = 0; c < 2 * NB; c++)
+        lds_load16(L.rb, (lds_void*)(dst + pp::kHalf + c * 8192),
+                   L.vb + pp::uni(o + (NB == 2 ? column_step(c) : c) * L.b_hstep), 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        L.rs, (lds_void*)(smem + H::kScaleBase + (t & (H::kRing - 1)) * bspp::kSSlot + wave * 256),
+        4, L.vs + pp::uni((uint32_t)t * L.s_kstep), 0, 0, 0);
+}
+
+// Column of position p of the first 64 of a tile of 256 columns. Position 128 h + 32 w + 16 t + j, which
+// is wave w's element j of MFMA tile t of column half h, has column 64 w + 32 h + 8 (j / 4) + 4 t +
+// j % 4: so a wave has whole 128-byte lines of out and a lane eight consecutive columns of two tiles.
+__device__ __forceinline__ uint32_t expert_column(uint32_t p)
+{
+    return (p & 32) << 1 | (p & 12) << 1 | (p & 16) >> 2 | (p & 3);
 }
 
 // The copies of the tile of M rows from row0 on, columns from n0 on.
-template <int ROWS, bool GATHER>
+template <int ROWS, int NB, bool GATHER>
 __device__ __forceinline__ void expert_load_setup(const ga_experts_product_args& a, int expert,
                                                   int row0, int M, int n0, int wave, int lane,
                                                   ExpertLoad<GATHER>& L)
@@ -251,8 +269,8 @@ __device__ __forceinline__ void expert_load_setup(const ga_experts_product_args&
             L.vrow[i] = row_offset(a, row0, M, i * 64 + crow, lda) + ckc * 16;
     L.rb = make_rsrc((const char*)a.b + (size_t)expert * a.stride_b_expert + (size_t)n0 * ldb,
                      rows_bytes(N - n0, ldb, a.k));
-    L.vb = (uint32_t)crow * ldb + ckc * 16;
-    L.b_hstep = 64 * ldb;
+    L.vb = (NB == 2 ? expert_column(crow) : (uint32_t)crow) * ldb + ckc * 16;
+    L.b_hstep = (NB == 2 ? 32 : 64) * ldb;
     if (wave < 4) {
         // position w*64 + l holds row w*64 + (l%4)*16 + l/4, those past M the last one
         L.rs = make_rsrc(a.sfa + (GATHER ? 0 : row0),
@@ -263,7 +281,8 @@ __device__ __forceinline__ void expert_load_setup(const ga_experts_product_args&
         const int nblk = (N + 127) / 128;
         L.rs = make_rsrc(a.sfb + (size_t)expert * a.stride_sfb_expert,
                          rows_bytes_f32(nblk, a.stride_sfb, G));
-        L.vs = (uint32_t)min(n0 / 128 + (lane & 1), nblk - 1) * (uint32_t)a.stride_sfb * 4;
+        // of each column half (which has the same columns' scales): waves 0 and 1 of four, 2 and 3
+        L.vs = (uint32_t)min(n0 / 128 + (NB == 2 ? lane >> 1 & 1 : 0), nblk - 1) * (uint32_t)a.stride_sfb * 4;
         L.s_kstep = 4;
     }
 }
@@ -279,15 +298,29 @@ __device__ __forceinline__ bspp::BsRead expert_read_setup(char* smem, int lane, 
     rb.b0 = smem + b_region + simd * 32 * 128 + o;
     rb.b1 = smem + b_region + simd * 32 * 128 + o64;
     rb.sa = smem + scales + grp * 256 + (lane & 15) * 16;
-    rb.sb = smem + scales + 1024;
+    rb.sb = smem + scales + 1024 + simd / 2 * 8;
     return rb;
 }
 
-// A tile's results to out: quadrant q of ROWS / 128 * NB, rows first, `result(q, i, t)` of its 16x16
-// tile i, t: lane l holds row l % 16, columns 4 (l / 16) on. Through LDS, so that whole rows are
-// written (those below M, columns below N).
-template <int ROWS, int NB, class Result>
-__device__ __forceinline__ void expert_store(const ga_experts_product_args& a, char* smem, int row0,
+// Eight results of a row, those below n.
+__device__ __forceinline__ void expert_store8(uint16_t* o, const v4i& d, int n)
+{
+    if (n >= 8)
+        // non-temporal: 6000 rows of 60 experts of 2048x1408 65.3 -> 61.7 us, 65536 of 64 of
+        // 4096x4096 1 % less; a layer, whose activation reads them next, no slower
+        __builtin_nontemporal_store(d, (v4i_any*)o);
+    else
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < n)
+                o[e] = (uint16_t)((uint32_t)d[e / 2] >> e % 2 * 16);
+}
+
+// The results of 128 rows and columns to out, `result(i, t)` of 16x16 tile i, t: lane l holds row
+// l % 16, columns 4 (l / 16) on. Through LDS, so that whole rows are written (those below M, columns
+// below N).
+template <class Result>
+__device__ __forceinline__ void expert_store128(const ga_experts_product_args& a, char* smem, int row0,
                                              int M, int n0, int wave, int lane, const Result& result)
 {
     const int grp = wave >> 2, simd = wave & 3, N = a.n - n0;
@@ -295,33 +328,63 @@ __device__ __forceinline__ void expert_store(const ga_experts_product_args& a, c
     uint16_t* out = (uint16_t*)a.out + (size_t)row0 * ld + n0;
     barrier_lds(); // every wave's operand and scale reads are done
 #pragma unroll
-    for (int q = 0; q < ROWS / 128 * NB; q++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int m = q / NB * 128 + grp * 64 + i * 16 + (lane & 15);
-                const int n = q % NB * 128 + simd * 32 + t * 16 + (lane >> 4) * 4;
-                *(uint2*)(smem + m * pp::kStagePitch + n * 2) = bf16x4(result(q, i, t));
-            }
+        for (int t = 0; t < 2; t++) {
+            const int m = grp * 64 + i * 16 + (lane & 15);
+            const int n = simd * 32 + t * 16 + (lane >> 4) * 4;
+            *(uint2*)(smem + m * pp::kStagePitch + n * 2) = bf16x4(result(i, t));
+        }
     barrier_lds();
-    constexpr int kLanes = NB * 16; // lanes of a row
+    constexpr int kLanes = 16; // of a row
 #pragma unroll
-    for (int it = 0; it < ROWS / 8 * kLanes / 64; it++) {
-        const int row = wave * (ROWS / 8) + it * (64 / kLanes) + lane / kLanes;
+    for (int it = 0; it < 4; it++) {
+        const int row = wave * 16 + it * (64 / kLanes) + lane / kLanes;
         const int col = lane % kLanes * 8;
         if (row >= M || col >= N)
             continue;
         uint16_t* o = out + (size_t)row * ld + col;
         const char* from = smem + row * pp::kStagePitch + col * 2;
-        if (col + 8 <= N)
-            // non-temporal: 6000 rows of 60 experts of 2048x1408 65.3 -> 61.7 us, 65536 of 64 of
-            // 4096x4096 1 % less; a layer, whose activation reads them next, no slower
-            __builtin_nontemporal_store(*(const v4i*)from, (v4i_any*)o);
-        else
-            for (int e = 0; e < N - col; e++)
-                o[e] = ((const uint16_t*)from)[e];
+        expert_store8(o, *(const v4i*)from, N - col);
     }
+}
+
+constexpr int kOwnPitch = 128 + 16;
+constexpr int kOwnBytes = 16 * kOwnPitch; // of LDS, a wave's own
+
+// The results of ROWS rows and 256 columns: quadrant q of ROWS / 128 * 2, rows first, `result(q, i, t)`
+// of its 16x16 tile i, t: lane l holds row l % 16, four columns (expert_column). A wave turns
+// its own 16 rows of 64 columns at a time in LDS of its own (`own`), so that whole lines are
+// written and no wave waits for another: 65536 rows of 64 experts of 4096x512 251 us, 269 in one piece
+// with barriers (of 4096x4096 1100, 1110), 292 from the registers in half lines.
+template <int ROWS, class Result>
+__device__ __forceinline__ void expert_store(const ga_experts_product_args& a, char* own, int row0,
+                                             int M, int n0, int wave, int lane, const Result& result)
+{
+    const int grp = wave >> 2, simd = wave & 3, N = a.n - n0;
+    const long long ld = a.stride_out;
+    uint16_t* out = (uint16_t*)a.out + (size_t)row0 * ld + n0;
+    char* to = own + (lane & 15) * kOwnPitch + (lane >> 4) * 16;
+    const int col = simd * 64 + lane % 8 * 8;
+#pragma unroll
+    for (int r = 0; r < ROWS / 128; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint2 d0 = bf16x4(result(2 * r + h, i, 0)), d1 = bf16x4(result(2 * r + h, i, 1));
+                *(v4i*)(to + h * 64) = (v4i){(int)d0.x, (int)d0.y, (int)d1.x, (int)d1.y};
+            }
+            wave_lds_fence();
+#pragma unroll
+            for (int it = 0; it < 2; it++) {
+                const int row = it * 8 + lane / 8, m = r * 128 + grp * 64 + i * 16 + row;
+                const v4i d = *(const v4i*)(own + row * kOwnPitch + lane % 8 * 16);
+                if (m < M && col < N)
+                    expert_store8(out + (size_t)m * ld + col, d, N - col);
+            }
+            wave_lds_fence();
+        }
 }
 
 // Which tile a workgroup has: XCD by XCD a run of tiles, an expert's column by column within
@@ -370,12 +433,17 @@ __device__ __forceinline__ void expert_half_tile(const ga_experts_product_args& 
             for (int t = 0; t < 2; t++)
                 acc[q][i][t] = (v4f){0.f, 0.f, 0.f, 0.f};
     ExpertLoad<GATHER> L;
-    expert_load_setup<128>(a, expert, row0, M, n0, wave, lane, L);
+    expert_load_setup<128, NB>(a, expert, row0, M, n0, wave, lane, L);
     const BsRead rb = expert_read_setup(smem, lane, grp, simd, pp::kHalf, H::kScaleBase);
     bs_half_chain<NB, PS_GROUP128>(L, rb, smem, a.k / 128, wave, grp, acc);
-    expert_store<128, NB>(a, smem, row0, M, n0, wave, lane, [&](int q, int i, int t) {
-        return acc[q][i][t];
-    });
+    if constexpr (NB == 2) {
+        barrier_lds(); // every wave's operand and scale reads are done
+        expert_store<128>(a, smem + wave * kOwnBytes, row0, M, n0, wave, lane,
+                          [&](int q, int i, int t) { return acc[q][i][t]; });
+    } else {
+        expert_store128(a, smem, row0, M, n0, wave, lane,
+                        [&](int i, int t) { return acc[0][i][t]; });
+    }
 }
 
 // 256x256 tiles; of an expert's last, if at most 128 rows are left, the upper half alone.
@@ -384,7 +452,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(pp::kNT, pp::kNT), amdgpu_
 void experts_tile_kernel(ga_experts_product_args a, int tn)
 {
     using namespace bspp;
-    constexpr int kLds = kLdsBs > BsHalfCfg<2>::kLds ? kLdsBs : BsHalfCfg<2>::kLds;
+    constexpr int kLds = std::max(kLdsBs + 8 * kOwnBytes, BsHalfCfg<2>::kLds);
+    static_assert(kLds <= 160 * 1024, "LDS budget");
     __shared__ __attribute__((aligned(1024))) char smem[kLds];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -409,12 +478,11 @@ void experts_tile_kernel(ga_experts_product_args a, int tn)
             for (int t = 0; t < 2; t++)
                 acc[q][i][t] = (v4f){0.f, 0.f, 0.f, 0.f};
     ExpertLoad<GATHER> L;
-    expert_load_setup<256>(a, x.expert, row0, M, n0, wave, lane, L);
+    expert_load_setup<256, 2>(a, x.expert, row0, M, n0, wave, lane, L);
     const BsRead rb = expert_read_setup(smem, lane, grp, simd, kBRegion, kSBase);
     bs_pp_chain<PS_GROUP128>(L, rb, smem, a.k / 128, wave, grp, acc);
-    expert_store<256, 2>(a, smem, row0, M, n0, wave, lane, [&](int q, int i, int t) {
-        return acc[q][i][t];
-    });
+    expert_store<256>(a, smem + kLdsBs + wave * kOwnBytes, row0, M, n0, wave, lane,
+                      [&](int q, int i, int t) { return acc[q][i][t]; });
 }
 
 template <int NB, bool GATHER>
