@@ -537,14 +537,14 @@ struct ExpertCut {
 // would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take 132 us in
 // 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in 16x32, 62 in
 // 128x256, 83 in 256x256; 64 of 4096x4096 with 64 rows 498, 198, 198, and 285 in 64x256; with 1024
-// rows 6450, 1330, 1120; 60 of 99x6272 with 1354 rows 400, 143, 151, and 104 in 128x128.
+// rows 6450, 1315, 1100; 60 of 99x6272 with 1354 rows 400, 143, 151, and 104 in 128x128.
 const ExpertCut& expert_cut(const ga_experts_product_args& a, int num_cu)
 {
     static const ExpertCut kCuts[GA_EXPERTS_CUTS] = {
-        {16, 64, 2, 2, 3.80f, 0.15f, 0.14f},   {16, 32, 4, 2, 3.65f, 0.28f, 0.10f},
-        {16, 256, 1, 2, 1.94f, 0.48f, 0.96f},  {64, 256, 1, 2, 3.46f, 1.37f, 0.69f},
-        {64, 64, 4, 2, 3.20f, 0.62f, 0.35f},   {128, 128, 0, 1, 2.58f, 0.49f, 0.57f},
-        {128, 256, 0, 1, 3.98f, 0.77f, 0.87f}, {256, 256, 0, 1, 4.95f, 1.19f, 0.97f}};
+        {16, 64, 2, 2, 3.83f, 0.14f, 0.15f},   {16, 32, 4, 2, 3.60f, 0.26f, 0.12f},
+        {16, 256, 1, 2, 2.14f, 0.43f, 0.96f},  {64, 256, 1, 2, 3.41f, 1.31f, 0.84f},
+        {64, 64, 4, 2, 4.14f, 0.61f, 0.37f},   {128, 128, 0, 1, 2.39f, 0.39f, 0.59f},
+        {128, 256, 0, 1, 3.49f, 0.63f, 0.75f}, {256, 256, 0, 1, 3.62f, 1.03f, 0.88f}};
     if (a.cut)
         return kCuts[a.cut - 1];
     const double rows = a.rows;
