@@ -245,6 +245,15 @@ def test_product_of_many_first_rows_that_decrease(dev, experts):
     check_product(dev, a, sfa, b, sfb, starts, None, "%d" % experts, CUTS)
 
 
+@pytest.mark.parametrize("k", [128, 384])
+def test_product_of_one_row_gathered_many_times(dev, k):
+    """Copies ahead of the last step, and of rows that are nowhere, from a matrix of one row."""
+    a, sfa, b, sfb = operands(1, 2, 257, k, seed=k)
+    rows = np.zeros(430, np.int32)
+    rows[::7], rows[3::50] = -1, 1
+    check_product(dev, a, sfa, b, sfb, np.array([0, 250, 430]), rows, "one row, K %d" % k, CUTS)
+
+
 def test_product_of_strided_operands(dev):
     c = [40, 0, 9]
     starts = on(np.array([0, 40, 40, 49], np.int32), dev)
