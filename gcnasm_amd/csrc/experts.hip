@@ -314,6 +314,10 @@ __device__ __forceinline__ int choose64(const ga_experts_route_args& a, const Ro
             key[v] = there ? ordered(t.x[v]) : 0u;
             low[v] = 0u;
         }
+        // groups go by the largest key, without a bias a logit: scores of 64 bits can be
+        // alike where logits differ; only the sum of two is one of scores
+        if (!a.bias && a.group_rank == 1)
+            score[v] = (double)t.x[v];
         if (!there)
             score[v] = (double)kMinus;
     }

@@ -110,6 +110,54 @@ def test_route_by_keys_that_32_bits_do_not_tell_apart(dev, experts, groups, scor
                     far + rng.integers(0, 3, experts) * abs(far) * 2.0 ** -23, scores=scores)
 
 
+def few_scores(scores, most):
+    """Logits of several experts that differ while their scores in 64 bits do not, by ranges: `most`
+    is 900 or less where their type has too few bits."""
+    if scores == "sigmoid":
+        return [(35.0, 90.0), (-most, -746.0), (-1e-20, 1e-20)]
+    return [(-most, -746.0), (0.0, 1e-20)]  # beside an expert of logit 0 or 1
+
+
+# experts 512 and up, and more than 16 choices: a token a wave
+@pytest.mark.parametrize("experts,groups,kept,top", [
+    (12, 3, 1, 2), (12, 4, 2, 3), (64, 8, 3, 6), (60, 10, 7, 9), (256, 16, 5, 16), (192, 8, 3, 20),
+    (320, 20, 4, 8), (512, 8, 4, 10), (1024, 64, 9, 33)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_groups_by_their_largest_logit(dev, experts, groups, kept, top, dtype, scores):
+    """Without a bias, groups by their largest expert go by its logit, also where 64 bits do not tell the
+    scores apart."""
+    rng = np.random.default_rng(experts + top)
+    size = experts // groups
+    for lo, hi in few_scores(scores, 900.0):
+        for equal in (False, True):
+            x = rng.uniform(lo, hi, (24, experts))
+            if equal:  # as many again as another one of their token
+                at = rng.integers(0, experts, x.shape)
+                x = np.where(rng.random(x.shape) < 0.5, x, np.take_along_axis(x, at, 1))
+            if scores == "softmax":
+                first = rng.integers(0, groups, 24) * size  # in any group
+                x[np.arange(24), first] = 0.0 if lo < 0 else 1.0
+            x[:4, rng.random(experts) < 0.3] = -np.inf
+            for renormalise in (True, False):
+                check_route(dev, x, top, dtype, scores=scores, groups=groups, top_groups=kept,
+                            group_rank=1, renormalise=renormalise)
+
+
+@pytest.mark.parametrize("experts", [12, 300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_groups_of_saturated_sigmoids(dev, experts, dtype):
+    """Three groups, two of them kept, logits whose sigmoid is 1 in 64 bits: far apart, and, of two equal
+    ones, near each other."""
+    size = experts // 3
+    x = np.full((2, experts), -1.0, np.float32)
+    x[0, [0, size, 2 * size]] = 40, 41, 60
+    x[1, [0, size, size + 1, 2 * size]] = 40, 44, 44, 48
+    ids, _ = ex.route(torch.from_numpy(x).to(dtype).to(dev), 3, scores="sigmoid", groups=3,
+                      top_groups=2)
+    assert host(ids).tolist() == [[2 * size, size, size + 1], [2 * size, size, size + 1]]
+
+
 def test_route_of_the_largest_logits(dev):
     """Of bf16 its own largest value is what an infinity counts as."""
     x = np.zeros((3, 70), np.float32)
