@@ -302,6 +302,64 @@ def test_product_of_one_row_gathered_many_times(dev, k):
     check_product(dev, a, sfa, b, sfb, np.array([0, 250, 430]), rows, "one row, K %d" % k, CUTS)
 
 
+@pytest.mark.parametrize("counts", ["single", "few", "wave", "skewed"])
+@pytest.mark.parametrize("n,k", [(144, 2816), (33, 3456), (72, 4224)])
+@pytest.mark.parametrize("gathered", [False, True])
+def test_product_of_long_k(dev, counts, n, k, gathered):
+    """22, 27 and 33 steps: a wave's ring of few rows comes round more than once in each of two and
+    four pieces of K, the last of them shorter."""
+    c = COUNTS[counts]
+    starts = np.concatenate([[0], np.cumsum(c)])
+    total = int(starts[-1]) + 3
+    rng = np.random.default_rng(n + k)
+    m = max(1, total // 2) if gathered else total
+    a, sfa, b, sfb = operands(m, len(c), n, k, seed=n + k)
+    rows = None
+    if gathered:
+        rows = rng.integers(0, m, total)
+        rows[rng.random(total) < 0.1] = -1
+    check_product(dev, a, sfa, b, sfb, starts, rows, "%s %dx%d" % (counts, n, k), CUTS)
+
+
+def strided(x, strides):
+    """x in memory of its own with these strides (elements)."""
+    size = 1 + sum((n - 1) * s for n, s in zip(x.shape, strides))
+    view = torch.empty(size, dtype=x.dtype, device=x.device).as_strided(x.shape, strides)
+    view.copy_(x)
+    return view
+
+
+@pytest.mark.parametrize("far", ["b", "out", "a", "gathered", "scales"])
+def test_product_past_4_gib(dev, far):
+    """Operands of which the last expert's weights, the last rows or their scales lie past 2^32 bytes, and
+    gathered rows up to the last offset that a call takes (256 of 0xE00000 bytes)."""
+    c, n, k = [3, 0, 140, 113, 64], 80, 384
+    starts = np.concatenate([[0], np.cumsum(c)])
+    total = int(starts[-1])
+    rng = np.random.default_rng(7)
+    rows = rng.permutation(np.arange(total) % 256) if far == "gathered" else None
+    a, sfa, b, sfb = operands(total if rows is None else 256, len(c), n, k, seed=5)
+    want, mass, _ = H.product(a, sfa, b, sfb, starts, rows)
+    A, S, B, T = on(a, dev), on(sfa, dev), on(b, dev), on(sfb, dev)
+    out = torch.empty((total, n), dtype=torch.bfloat16, device=dev)
+    if far == "b":
+        B = strided(B, (3 << 29, 1 << 20, 1))
+    elif far == "out":
+        out = strided(out, ((1 << 23) + 3, 1))
+    elif far in ("a", "gathered"):
+        A = strided(A, (0xE00000, 1))
+    else:
+        S, T = strided(S, ((1 << 28) + 8, 1)), strided(T, (3 << 28, 1 << 22, 1))
+    args = [A, S, B, T, on(starts.astype(np.int32), dev),
+            None if rows is None else on(rows.astype(np.int32), dev)]
+    for cut in CUTS:
+        out.fill_(5.0)
+        ex.product(*args, out=out, cut=cut)
+        bits = host(out.contiguous().view(torch.int16)).view(np.uint16)
+        _, st = bf16_compare(bits, want, mass)
+        assert_parity(st, "far %s cut %d" % (far, cut))
+
+
 def test_product_of_strided_operands(dev):
     c = [40, 0, 9]
     starts = on(np.array([0, 40, 40, 49], np.int32), dev)
@@ -489,6 +547,19 @@ def test_combine_of_strided_rows(dev):
         assert (np.abs(host(out) - want) <= 2.0 ** -21 * mass).all()
         out.fill_(9.0)
         assert (O == 9.0).all()
+
+
+def test_rows_past_4_gib(dev):
+    """Activation and sum of rows of which the last lie past 2^32 bytes."""
+    rng = np.random.default_rng(4)
+    x = torch.from_numpy(rng.standard_normal((20, 512)).astype(np.float32)).to(dev)
+    q, s = ex.activate(strided(x, ((3 << 25) + 1, 1)))
+    assert all(torch.equal(u, v) for u, v in zip((q, s), ex.activate(x)))
+    y, place = x.bfloat16(), on(rng.integers(0, 20, (30, 3)).astype(np.int32), dev)
+    w = on(rng.standard_normal((30, 3)).astype(np.float32), dev)
+    out = strided(torch.zeros((30, 512), device=dev), ((3 << 24) + 5, 1))
+    ex.combine(strided(y, ((3 << 26) + 3, 1)), place, w, out=out)
+    assert torch.equal(out.contiguous(), ex.combine(y, place, w, dtype=torch.float32))
 
 
 # ---- together --------------------------------------------------------------------------
