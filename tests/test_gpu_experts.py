@@ -620,6 +620,51 @@ def test_layer(dev, tokens, first, mine):
     assert (got[idle] == 0).all()
 
 
+class Shard(Layer):
+    """A layer by one cut of its products."""
+
+    def rows(self, x, cut):
+        """The layer's rows before their sum, their first rows, places and weights."""
+        ids, w = ex.route(x.float() @ self.gate.t(), self.top)
+        starts, tokens, place = ex.arrange(ids, self.mine, self.first)
+        h = ex.product(*ops.quant_fp8_1x128(x), self.w1, self.s1, starts, tokens, cut=cut)
+        q, s = ex.activate(h, starts)
+        return ex.product(q, s, self.w2, self.s2, starts, cut=cut), starts, place, w
+
+
+@pytest.mark.parametrize("cut", CUTS[1:])
+def test_shards_by_the_same_cut_have_the_same_rows(dev, cut):
+    """By one cut a row's sums do not depend on the experts that are held, so a shard has the whole's rows bit
+    by bit, and sums differ by the order of their `top` fused steps alone, in the whole and in the
+    parts."""
+    whole = Shard(dev, 640, 512, 12, 4)
+    x = torch.randn((70, 640), device=dev).bfloat16()
+    y, starts, place, w = whole.rows(x, cut)
+    want = ex.combine(y, place, w, dtype=torch.float32).double()
+    mass = ex.combine(y.abs(), place, w, dtype=torch.float32).double()
+    total = torch.zeros_like(want)
+    for first in (0, 3, 6, 9):
+        part = Shard(dev, 640, 512, 12, 4, first, 3)
+        yp, sp, pp, wp = part.rows(x, cut)
+        lo, hi = int(starts[first]), int(starts[first + 3])
+        assert int(sp[-1]) == hi - lo and torch.equal(yp[:hi - lo], y[lo:hi])
+        total += ex.combine(yp, pp, wp, dtype=torch.float32).double()
+    assert ((total - want).abs() <= 2 * 4 * 2.0 ** -24 * mass).all()
+
+
+@pytest.mark.parametrize("cuts", [(2, 3, 1, 8), (7, 5, 0, 2), (0, 0, 0, 0)])
+def test_shards_by_other_cuts_add_up(dev, cuts):
+    """A cut that sums K in other pieces changes h by a step of bfloat16 and so a code by a step: the parts'
+    sum is held to the layer in float64, within the bound of test_layer."""
+    x = torch.randn((40, 640), device=dev).bfloat16()
+    want = Shard(dev, 640, 512, 12, 4).plain(x)
+    got = torch.zeros_like(want)
+    for first, cut in zip((0, 3, 6, 9), cuts):
+        y, _, place, w = Shard(dev, 640, 512, 12, 4, first, 3).rows(x, cut)
+        got += ex.combine(y, place, w).double()
+    assert (got - want).norm() <= 0.104 * want.norm()
+
+
 def test_layer_on_another_stream_and_in_a_graph(dev):
     layer = Layer(dev, 256, 256, 12, 4, seed=1)
     inputs = [torch.randn((33, 256), device=dev).to(torch.bfloat16) for _ in range(4)]
