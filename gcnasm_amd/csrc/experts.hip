@@ -886,9 +886,9 @@ __device__ __forceinline__ void load8(const void* x, size_t i, float (&v)[8])
     }
 }
 
-// g / (1 + exp(-g)), off by at most 2^-21.4 of itself (the hardware's exponential 2^-23, five
-// roundings): the exponential's argument in two parts, a Newton step for the reciprocal. Zero where
-// 1 / (1 + exp(-g)) is below the least normal number; -inf gives NaN, +inf itself.
+// g / (1 + exp(-g)) for g from -87 on, off by at most 2^-21.4 of itself (the hardware's exponential
+// 2^-23, four roundings): the exponential's argument in two parts, a Newton step for the
+// reciprocal. +inf gives itself.
 __device__ __forceinline__ float gated(float g)
 {
     constexpr float kLog2e = 0x1.715476p+0f, kLess = 0x1.4ae0c0p-26f; // to fp32, and what it leaves
@@ -901,6 +901,16 @@ __device__ __forceinline__ float gated(float g)
     float r = __builtin_amdgcn_rcpf(d);
     r = fmaf(fmaf(-d, r, 1.0f), r, r);
     return g * r;
+}
+
+// The same for g below -87, where 1 / (1 + exp(-g)), exp(g) there, is denormal though the result is not:
+// exp(g + 20), of which the argument is exact, and the rest behind the product. Denormal from g =
+// -91.8 down, zero from -108.7; -inf gives NaN.
+constexpr float kFar = -87.0f;
+
+__device__ __forceinline__ float gated_far(float g)
+{
+    return g * expf(g + 20.0f) * 0x1.1b4866p-29f; // exp(-20)
 }
 
 template <int IN>
@@ -933,9 +943,20 @@ __global__ __launch_bounds__(256) void activate_kernel(const void* __restrict__ 
     for (int u = 0; u < U; u++) {
         const long long r = r0 + u * 4 + wave;
         float y[8];
+        float least = gate[u][0];
+#pragma unroll
+        for (int j = 1; j < 8; j++)
+            least = fminf(least, gate[u][j]);
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            y[j] = gated(gate[u][j]) * up[u][j];
+            y[j] = gated(gate[u][j]);
+        if (__builtin_amdgcn_ballot_w64(least < kFar) != 0)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                y[j] = gate[u][j] < kFar ? gated_far(gate[u][j]) : y[j];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            y[j] *= up[u][j];
         bool nan;
         const float s = ds_scale(__uint_as_float(block_amax<16, 8>(y, nan)));
         const ScaleDiv d(s);

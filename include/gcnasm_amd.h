@@ -811,10 +811,12 @@ typedef struct ga_experts_product_args {
 ga_status ga_experts_product(const ga_experts_product_args* args, void* stream);
 
 /* Between an expert's products: x [rows, 2 * inner] (fp32 or bf16, rows stride_x elements
- * apart), its first half the gate g, the second u: y = u * g / (1 + exp(-g)) in fp32
- * (off by at most 2^-21 of itself; zero from 2^-126 |g u| down), quantised as by ga_quant_fp8_1x128: q [rows, inner] E4M3 (rows stride_q bytes apart), scales
- * [inner / 128, rows] (rows stride_scales elements apart). inner % 128 == 0. limit: device address of a row count (starts + experts), rows
- * from it on are not looked at and nothing of theirs is written; NULL: all rows. */
+ * apart), its first half the gate g, the second u: y = u * g / (1 + exp(-g)) in fp32 (off by at
+ * most 2^-21 of itself; by a denormal number's step more where g / (1 + exp(-g)) is one, from g =
+ * -91.8 down), quantised as by ga_quant_fp8_1x128: q [rows, inner] E4M3 (rows stride_q bytes
+ * apart), scales [inner / 128, rows] (rows stride_scales elements apart). inner % 128 == 0.
+ * limit: device address of a row count (starts + experts), rows from it on are not looked at and
+ * nothing of theirs is written; NULL: all rows. */
 ga_status ga_experts_activate(const void* x, int in_dtype, int rows, int inner, long long stride_x,
                               void* q, long long stride_q, float* scales, long long stride_scales,
                               const int* limit, void* stream);

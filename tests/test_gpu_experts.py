@@ -455,6 +455,26 @@ def test_activate(dev, rows, inner, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_activate_of_gates_far_below_zero(dev, dtype):
+    """Gates down to -91.5, to which g / (1 + exp(-g)) is a normal number (2^-126) though exp(g) or exp(-g)
+    is none: blocks of such gates alone, and beside others."""
+    rng = np.random.default_rng(9)
+    x = np.empty((50, 768), np.float32)
+    x[:, :384] = rng.uniform(-91.5, -86.5, (50, 384))
+    x[25:, :384:3] = rng.standard_normal((25, 128))
+    x[:, 384:] = 1e6 * rng.standard_normal((50, 384))  # so that scales are normal numbers too
+    x[40:, 128:256] = -89.0
+    x = torch.from_numpy(x).to(dtype)
+    q, s = ex.activate(x.to(dev))
+    check_activate(host(x.double()), q, s)
+    assert (host(s) < 2.0 ** -99)[:, :25].all() and (host(q)[:25] & 0x7F).max() == 0x7E
+    # further on: denormal numbers, and zero
+    x[:, :384] = -120.0
+    q, s = ex.activate(x.to(dev))
+    assert (s == 1).all() and (q & 0x7F == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_activate_of_strided_and_unaligned_rows(dev, dtype):
     rng = np.random.default_rng(2)
     for width, first in ((520, 8), (515, 3), (513, 1)):
