@@ -80,8 +80,9 @@ __device__ __forceinline__ float unordered(uint32_t k)
 constexpr int kRouteWaves = 4;
 constexpr float kMinus = -__builtin_inff();
 
-// What keys of scores are off by in 32 bits, apart from the sum's rounding: an exponential's
-// argument, the exponential and the sum of up to 1024 of them, at most 2^-19 of a score in all.
+// What keys of scores are off by in 32 bits, apart from the rounding of score + bias: an exponential's
+// argument, the exponential and the sum of up to 1024 of them, at most 2^-19 of a score in all,
+// taken twice. (What is too wide here sends more tokens to 64 bits, what is too narrow would choose wrongly.)
 constexpr float kScoreError = 0x1p-18f;
 
 // A logit: -inf where it is not there (-inf, NaN), +inf as its type's largest finite value.
@@ -115,6 +116,10 @@ __device__ __forceinline__ float weight_of(const ga_experts_route_args& a, float
     return expf(e) / (1.0f + expf(-fabsf(x)));
 }
 
+// By the hardware's exponential, also for the sum that divides a softmax's weights: its argument x log2(e)
+// rounded to 24 bits is off by 1.25 |x| 2^-24 of a term, of the sum, where terms weigh by their size, by
+// 1.25 ln(1024) 2^-24, with the exponential's own 2^-23 at most 11 2^-24; the sum's additions in fp32 (16
+// a lane, 6 between lanes) can take twice that.
 __device__ __forceinline__ float score_of(float x, bool softmax, float largest)
 {
     return softmax ? __expf(x - largest) : __builtin_amdgcn_rcpf(1.0f + __expf(-x));

@@ -14,8 +14,7 @@ inline long long most_expert_tiles(long long rows, long long experts, int height
     return rows < full ? rows : full;
 }
 
-// Rows first .. last - 1 of expert e; `index` of this expert's `tiles` tiles, `before` tiles of
-// experts before it.
+// Rows first .. last - 1 of an expert, which has `tiles` tiles; `before` tiles of experts before it.
 struct ExpertTile {
     int expert, first, last;
     int before, tiles;
@@ -42,7 +41,8 @@ __device__ __forceinline__ int wave_scan(int x, const Op& op)
 // The tiles of all experts, and the expert of one of them. First rows are taken as the nearest of
 // 0 .. rows, and where they decrease as the largest before, so that there are no more tiles than
 // most_expert_tiles(). Every lane of a wave calls it: a lane has a run of P experts in registers, a
-// scan over the wave gives the tiles before them. pick(total) says which tile (uniform; outside 0 .. total - 1: none, and false is returned).
+// scan over the wave gives the tiles before them. pick(total) says which tile (uniform; outside
+// 0 .. total - 1: none, and false is returned).
 template <int P, class Pick>
 __device__ __forceinline__ bool find_expert_run(const int* __restrict__ starts, int experts, int rows,
                                                 int height, int lane, const Pick& pick,

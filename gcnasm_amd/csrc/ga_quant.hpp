@@ -161,8 +161,9 @@ __device__ __forceinline__ float ds_scale(float amax) { return amax > 0.0f ? ama
 // way. The sign is taken from x, so -0 stays -0. tests/scale_div_check.c
 // restates this arithmetic on the CPU and compares it with IEEE division
 // (every bf16 x and random fp32 x under scales over the whole range; 1.4e9
-// quotients without a mismatch). Other scales (subnormal, infinite) divide. Five VALU instructions per element instead
-// of the IEEE division's ten; the choice is made once per scale.
+// quotients without a mismatch). Other scales (subnormal, infinite) divide. Five
+// VALU instructions per element instead of the IEEE division's ten; the choice is
+// made once per scale.
 struct ScaleDiv {
     float s, r;
     bool fast;

@@ -20,7 +20,10 @@ namespace ga {
 namespace {
 
 // Operands span less than this, so an offset kNowhere is past the end of a descriptor, and
-// stays so when the steps along K are added: such a load gives zeros.
+// stays so when the steps along K are added: such a load gives zeros. The copies past K can take
+// the scales' sum past 2^32. In the hardware's two offsets that is out of range too (checked on
+// MI355X); added up in 32 bits it may come to lie in the operand again, and what is copied
+// from there is not used.
 constexpr uint32_t kNowhere = 0xF0000000u;
 constexpr unsigned long long kMostBytes = 0xE0000000ull;
 constexpr unsigned long long kMostScaleBytes = 0x0FFF0000ull;
@@ -528,13 +531,16 @@ struct ExpertCut {
 };
 
 // The cut with the smallest estimated time. The counts are on the GPU, so the tiles are those of
-// rows spread over the experts by chance. A call takes its rounds of workgroups (a last one that is
+// rows spread over the experts by chance, and all rows count as live: of a process that holds some of the
+// experts they are too many (1/2, 1/4, 1/8 of them held, 120 problems by chance: 8, 11, 10 % slower than
+// the fastest cut on average, at the worst 1.95 times; `cut` names another). A call takes its rounds of workgroups (a last one that is
 // not full counts as between its part and a whole one) or, where that is longer, its tiles at full
 // rate; about where they are equal it takes longer than both, as the fourth root of the sum of
 // fourth powers does. The coefficients are a fit to 2359 problems measured on MI355X with every
 // cut (2-256 experts, 1-4000 rows each, N 64-7168, K 256-7168): the cut it picks is on average 2 %
-// slower than the fastest, at the worst 1.4 times, of 99 in 100 at most 1.26. One cut for all
-// would cost between 1.2 and 3 times: 256 experts of 7168x512 with 4 rows each take 132 us in
+// slower than the fastest, at the worst 1.43 times, of 99 in 100 at most 1.26; of 200 others by chance,
+// K from 128 on, 5 %, at the worst 1.31. One cut for all takes 1.34 (64x64) to 1.92 (16x32)
+// times the fastest on average: 256 experts of 7168x512 with 4 rows each take 132 us in
 // 16x256, 250 in 128x256, 342 in 16x32 workgroups; 8 of 2048x7168 with 300 rows 173 in 16x32, 62 in
 // 128x256, 83 in 256x256; 64 of 4096x4096 with 64 rows 498, 198, 198, and 285 in 64x256; with 1024
 // rows 6450, 1315, 1100; 60 of 99x6272 with 1354 rows 400, 143, 151, and 104 in 128x128.
