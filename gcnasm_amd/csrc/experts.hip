@@ -159,6 +159,14 @@ __device__ __forceinline__ void two_largest(const ga_experts_route_args& a, cons
     }
 }
 
+// The value of a group in 32 bits. Two keys can have a sum below the least number, which may not
+// become that of a group that is not there; values so far out are within what they can be off by, so that
+// 64 bits decide.
+__device__ __forceinline__ float group_value(const ga_experts_route_args& a, float b1, float b2)
+{
+    return a.group_rank == 2 && b2 > kMinus ? fmaxf(b1 + b2, -0x1.FFFFFEp127f) : b1;
+}
+
 // The groups that are kept, a bit at each one's first lane (group << shift), by their values.
 template <class T>
 __device__ __forceinline__ uint64_t kept_groups(const ga_experts_route_args& a, const T* by, int lane,
@@ -186,7 +194,7 @@ __device__ __forceinline__ uint64_t kept_groups_packed(const ga_experts_route_ar
 {
     float b1, b2;
     two_largest(a, by, lane, shift, b1, b2);
-    const float value = a.group_rank == 2 && b2 > kMinus ? b1 + b2 : b1;
+    const float value = group_value(a, b1, b2);
     const int g = lane >> shift;
     const bool there =
         g < a.groups && (lane & ((1 << shift) - 1)) == 0 && value > kMinus;
@@ -598,7 +606,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows_kernel(ga_experts
         const int shift = 31 - __builtin_clz(16 / a.groups); // log2 of the lanes of a group
         float b1, b2;
         two_largest(a, f, r, shift, b1, b2);
-        const float value = a.group_rank == 2 && b2 > kMinus ? b1 + b2 : b1;
+        const float value = group_value(a, b1, b2);
         const int g = r >> shift;
         const bool leads = g < a.groups && (r & ((1 << shift) - 1)) == 0 && value > kMinus;
         const float top = row_max(leads ? value : kMinus);

@@ -158,6 +158,28 @@ def test_route_groups_of_saturated_sigmoids(dev, experts, dtype):
     assert host(ids).tolist() == [[2 * size, size, size + 1], [2 * size, size, size + 1]]
 
 
+@pytest.mark.parametrize("experts,groups,kept,top", [
+    (6, 3, 2, 2), (8, 4, 3, 5), (48, 16, 9, 16), (256, 16, 12, 7), (60, 20, 11, 9), (128, 8, 5, 20),
+    (600, 60, 41, 64)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_of_biases_next_to_the_lowest_number(dev, experts, groups, kept, top, scores):
+    """Finite biases of which two have a sum below the least number of 32 bits, as masks put them in: groups
+    that have none but such experts left are still there."""
+    rng = np.random.default_rng(experts)
+    most = float(np.finfo(np.float32).max)
+    size = experts // groups
+    for masked, missing in itertools.product((0.3, 0.9, 1.0), (0.0, 0.5, 0.9)):
+        b = 0.1 * rng.standard_normal(experts)
+        whole = np.repeat(rng.random(groups) < masked, size)  # groups at a time
+        b[whole] = rng.choice([-most, -3e38, -2e38], whole.sum())
+        x = rng.standard_normal((40, experts))
+        x[rng.random(x.shape) < missing] = -np.inf
+        x[0] = np.where(np.arange(experts) == 0, 1.0, np.where(whole, x[0], -np.inf))
+        for dtype, rank in itertools.product((torch.float32, torch.bfloat16), (1, 2)):
+            check_route(dev, x, top, dtype, b, scores=scores, groups=groups, top_groups=kept,
+                        group_rank=rank)
+
+
 def test_route_of_the_largest_logits(dev):
     """Of bf16 its own largest value is what an infinity counts as."""
     x = np.zeros((3, 70), np.float32)
