@@ -95,9 +95,12 @@ def main(argv=None):
     p.add_argument("--steps", type=int, default=100)
     p.add_argument("--graph", action="store_true", help="capture the step into a graph")
     a = p.parse_args(argv)
+    if not 1 <= a.shards <= a.experts or not 0 <= a.shard < a.shards:
+        p.error("--shard must be 0 .. shards - 1, --shards 1 .. experts")
     device = torch.device("cuda")
-    held = a.experts // a.shards
-    layer = Layer(a.hidden, a.inner, a.experts, a.top, device, a.shard * held, held, a.groups,
+    first = a.shard * a.experts // a.shards
+    held = (a.shard + 1) * a.experts // a.shards - first
+    layer = Layer(a.hidden, a.inner, a.experts, a.top, device, first, held, a.groups,
                   a.top_groups, a.scores)
     step = Graph(layer, a.tokens, a.hidden, device) if a.graph else layer
     g = torch.Generator(device).manual_seed(1)

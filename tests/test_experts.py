@@ -1,6 +1,8 @@
 """The experts' C entries without a GPU: what they refuse before any device call, and calls with
 nothing to do."""
 import ctypes
+import importlib.util
+import os
 
 import numpy as np
 import pytest
@@ -106,6 +108,19 @@ def test_nothing_to_do_is_no_error():
     assert product(rows=0, a=None, sfa=None, a_rows=0) == 0
     assert l.ga_experts_activate(None, 1, 0, 256, 512, None, 256, None, 0, None, None) == 0
     assert l.ga_experts_combine(0x1000, 9, 100, 100, None, None, 0, 3, None, 0, 100, None) == 0
+
+
+@pytest.mark.parametrize("args", [["--shards", "0"], ["--shards", "9", "--experts", "8"],
+                                  ["--shards", "2", "--shard", "2"], ["--shard", "-1"]])
+def test_shards_that_the_example_refuses(args, capsys):
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples",
+                        "experts_layer.py")
+    spec = importlib.util.spec_from_file_location("experts_layer_cpu", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    with pytest.raises(SystemExit):
+        example.main(args)
+    assert "--shard" in capsys.readouterr().err
 
 
 def test_null_arguments():

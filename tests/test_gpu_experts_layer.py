@@ -35,6 +35,18 @@ def test_runs(dev, example, args, capsys):
     assert "a step" in capsys.readouterr().out
 
 
+@pytest.mark.parametrize("experts,shards", [(10, 3), (7, 7), (9, 2)])
+def test_every_expert_is_one_shards(dev, example, experts, shards):
+    held = []
+    for i in range(shards):
+        layer, _ = example.main(["--tokens", "3", "--hidden", "128", "--inner", "128", "--experts",
+                                 str(experts), "--top", "2", "--steps", "1", "--shards", str(shards),
+                                 "--shard", str(i)])
+        assert len(layer.w1) == layer.held
+        held += range(layer.first, layer.first + layer.held)
+    assert held == list(range(experts))
+
+
 def test_a_step(dev, example):
     """Rounding activations to e4m3 twice is off by up to 2^-4 of an element each, at the most
     2^-4 / sqrt(3) of the root mean square; two such errors come to 0.052 of the output's norm, and twice
